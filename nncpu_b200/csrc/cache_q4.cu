@@ -1,0 +1,227 @@
+// Keys and values in 4 bits: the append to the paged cache (with the heads' norms and rotation on the way), and the way back to
+// numbers.  cache_q4.cuh says how the pages lie.
+//
+// The norm and the rotation are those of the 16- and 32-bit caches (crates/nncpu/src/model/forward.rs:278-351): q leaves as the
+// attention reads it, a key is normed and rotated and a value taken as it is before they are cut to 4 bits.
+
+#include <math.h>
+
+#define NN_LIB cache_q4
+#include "common.cuh"
+#include "cache_q4.cuh"
+
+namespace {
+
+struct Append {
+    const void* qkv;        // [n, ld]: heads of q, then of k, then of v
+    int qkv_dt, ld;
+    const void* q_gamma;    // [D] or null
+    const void* k_gamma;
+    int g_dt;
+    double eps;
+    const float2* cs;       // [n, half] (cos, sin), or null: the pairs (i, i + half) of a head's first 2 half lanes turn
+    int half;
+    const int* tok_seq;
+    const int* tok_pos;
+    const int* block_table; // [*, bt_stride]
+    int bt_stride;
+    uint8_t* k_pages;       // [n_pages, n_kv, 40 D]
+    uint8_t* v_pages;
+    int n_pages;
+    void* q_out;            // [n, n_heads D]
+    int q_dt;
+    int n, n_heads, n_kv, D;
+    float temp_coef;        // c != 0: the query at position p times 1 + c ln(floor((p + 1) / temp_every) + 1)
+    int temp_every;
+};
+
+__device__ __forceinline__ double warp_sum64(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// The page of a token's key, or -1 (a padding row, a position without a page).
+__device__ __forceinline__ int page_of(const int* block_table, int bt_stride, int n_pages, int seq, int pos) {
+    if (seq < 0 || pos < 0 || pos / kPage >= bt_stride) return -1;
+    const int p = block_table[(size_t)seq * bt_stride + pos / kPage];
+    return p < n_pages ? p : -1;
+}
+
+// One head of one token, a warp's job; lane l holds lanes l, l + 32, ... of the head (one of every group).
+template <int NG, typename F>
+__device__ __forceinline__ void norm_rotate(F (&x)[NG], const void* gamma, int g_dt, F eps, const float2* cs, int half, F* row, int lane) {
+    constexpr int D = 32 * NG;
+    if (gamma != nullptr) {
+        F s = 0;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) s += x[g] * x[g];
+        if constexpr (sizeof(F) == 8) s = warp_sum64(s);
+        else s = warp_sum(s);
+        const F r = F(1) / sqrt(s / F(D) + eps);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) x[g] = x[g] * r * F(ld_f(gamma, 32 * g + lane, g_dt));
+    }
+    if (cs != nullptr) {
+        __syncwarp();
+#pragma unroll
+        for (int g = 0; g < NG; ++g) row[32 * g + lane] = x[g];
+        __syncwarp();
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const int i = 32 * g + lane;
+            if (i < 2 * half) {
+                const bool second = i >= half;
+                const float2 t = cs[second ? i - half : i];
+                const F other = row[second ? i - half : i + half];
+                x[g] = second ? x[g] * F(t.x) + other * F(t.y) : x[g] * F(t.x) - other * F(t.y);
+            }
+        }
+    }
+}
+
+// A warp per (token, head of q, k or v).
+template <int NG>
+__global__ void __launch_bounds__(256) append_kernel(const Append a) {
+    constexpr int D = 32 * NG;
+    __shared__ double rows[8][D];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int per_tok = a.n_heads + 2 * a.n_kv;
+    const long item = (long)blockIdx.x * 8 + warp;
+    if (item >= (long)a.n * per_tok) return;
+    const int t = (int)(item / per_tok), h = (int)(item % per_tok);
+    const int seq = a.tok_seq[t], pos = a.tok_pos[t];
+    float x[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) x[g] = ld_f(a.qkv, (size_t)t * a.ld + (size_t)h * D + 32 * g + lane, a.qkv_dt);
+    const float2* cs = a.cs == nullptr ? nullptr : a.cs + (size_t)t * a.half;
+    if (h < a.n_heads) {
+        norm_rotate<NG, float>(x, a.q_gamma, a.g_dt, (float)a.eps, cs, a.half, reinterpret_cast<float*>(rows[warp]), lane);
+        float times = 1.0f;
+        if (a.temp_coef != 0.0f) times = 1.0f + a.temp_coef * logf(floorf((float)(pos + 1) / (float)a.temp_every) + 1.0f);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) st_f(a.q_out, ((size_t)t * a.n_heads + h) * D + 32 * g + lane, a.q_dt, x[g] * times);
+        return;
+    }
+    const bool value = h >= a.n_heads + a.n_kv;
+    const int kvh = (h - a.n_heads) - (value ? a.n_kv : 0);
+    const int page = page_of(a.block_table, a.bt_stride, a.n_pages, seq, pos);
+    if (page < 0) return;
+    if (!value) {
+        // In 64 bits: a key next to the border of two codes takes one or the other by its last bit.  B200's 64-bit rate is half of
+        // its 32-bit one, and the kernel is bound by its loads and stores.
+        double y[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) y[g] = x[g];
+        norm_rotate<NG, double>(y, a.k_gamma, a.g_dt, a.eps, cs, a.half, rows[warp], lane);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) x[g] = (float)y[g];
+    }
+    const int at = pos % kPage;
+    uint8_t* base = (value ? a.v_pages : a.k_pages) + ((size_t)page * a.n_kv + kvh) * q4_page_bytes(D);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        const float v = q4_in_range(x[g]);
+        const bool bad = __any_sync(0xffffffffu, v != v);
+        float lo = v, hi = v;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        if (bad) lo = hi = __int_as_float(0x7FC00000);
+        const Q4Scale s = q4_scale(lo, hi);
+        uint32_t w = q4_code(v, s);
+        if (value) {
+            w <<= 4 * (lane & 3);
+            w |= __shfl_xor_sync(0xffffffffu, w, 1);
+            w |= __shfl_xor_sync(0xffffffffu, w, 2);
+            if ((lane & 3) == 0)
+                reinterpret_cast<uint16_t*>(base)[2 * q4_value_word(at, lane >> 2, g, NG) + (at & 1)] = (uint16_t)w;
+        } else {
+            w <<= 4 * (lane & 7);
+            w |= __shfl_xor_sync(0xffffffffu, w, 1);
+            w |= __shfl_xor_sync(0xffffffffu, w, 2);
+            w |= __shfl_xor_sync(0xffffffffu, w, 4);
+            if ((lane & 7) == 0) reinterpret_cast<uint32_t*>(base)[q4_key_word(at, lane >> 3, g, NG)] = w;
+        }
+        if (lane == 0)
+            reinterpret_cast<__half2*>(base + q4_scales_at(D))[at * NG + g] = __halves2half2(s.d, s.m);
+    }
+}
+
+// The number of lane `i` of position `at` in a page.
+template <bool VALUES>
+__device__ __forceinline__ float page_number(const uint8_t* base, int at, int i, int D) {
+    const int NG = D / kGroup, g = i >> 5;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(base);
+    const float2 dm = __half22float2(reinterpret_cast<const __half2*>(base + q4_scales_at(D))[at * NG + g]);
+    const uint32_t code = VALUES ? words[q4_value_word(at, (i & 31) >> 2, g, NG)] >> (16 * (at & 1) + 4 * (i & 3))
+                                 : words[q4_key_word(at, (i & 31) >> 3, g, NG)] >> (4 * (i & 7));
+    return q4_number(code & 15, dm);
+}
+
+// What the cache holds of given tokens: a warp per (token, head), keys by grid.y 0, values by 1.
+__global__ void __launch_bounds__(256) read_kernel(const uint8_t* k_pages, const uint8_t* v_pages, int n_pages, const int* block_table,
+                                                   int bt_stride, const int* tok_seq, const int* tok_pos, void* k_out, void* v_out,
+                                                   int out_dt, int n, int n_kv, int D) {
+    const long item = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (item >= (long)n * n_kv) return;
+    const int t = (int)(item / n_kv), h = (int)(item % n_kv);
+    const int pos = tok_pos[t];
+    const int page = page_of(block_table, bt_stride, n_pages, tok_seq[t], pos);
+    const bool values = blockIdx.y == 1;
+    void* out = values ? v_out : k_out;
+    const uint8_t* base = (values ? v_pages : k_pages) + ((size_t)max(page, 0) * n_kv + h) * q4_page_bytes(D);
+    for (int i = lane; i < D; i += 32) {
+        const float v = page < 0 ? 0.0f : values ? page_number<true>(base, pos % kPage, i, D) : page_number<false>(base, pos % kPage, i, D);
+        st_f(out, ((size_t)t * n_kv + h) * D + i, out_dt, v);
+    }
+}
+
+}  // namespace
+
+static bool q4_lanes_ok(int D) { return D >= 32 && D <= 256 && D % 32 == 0; }
+
+extern "C" int nncpu_qk_norm_rope_append_q4(const void* qkv, int qkv_dt, int ld, const void* q_gamma, const void* k_gamma, int g_dt,
+                                            double eps, const float* cos_sin, int half, const int* tok_seq, const int* tok_pos,
+                                            const int* block_table, int bt_stride, uint8_t* k_pages, uint8_t* v_pages, int n_pages,
+                                            void* q_out, int q_dt, int n, int n_heads, int n_kv, int D, float temp_coef,
+                                            int temp_every, cudaStream_t stream) {
+    NN_CHECK(q4_lanes_ok(D), "qk_norm_rope_append_q4: heads of %d lanes (whole groups of 32, at most 256)", D);
+    NN_CHECK(n >= 0 && n_heads > 0 && n_kv >= 0 && ld >= (n_heads + 2 * n_kv) * D, "qk_norm_rope_append_q4: %d heads over %d in rows of %d", n_heads, n_kv, ld);
+    NN_CHECK(half >= 0 && 2 * half <= D, "qk_norm_rope_append_q4: %d rotated pairs in a head of %d lanes", half, D);
+    NN_CHECK(n_kv == 0 || (bt_stride > 0 && n_pages > 0 && k_pages != nullptr && v_pages != nullptr), "qk_norm_rope_append_q4: no pages to append to");
+    NN_CHECK(temp_coef == 0.0f || temp_every > 0, "qk_norm_rope_append_q4: a temperature every %d positions", temp_every);
+    if (n == 0) return 0;
+    Append a{qkv, qkv_dt, ld, q_gamma, k_gamma, g_dt, eps, reinterpret_cast<const float2*>(cos_sin), half, tok_seq, tok_pos, block_table,
+             bt_stride, k_pages, v_pages, n_pages, q_out, q_dt, n, n_heads, n_kv, D, temp_coef, temp_every};
+    const long items = (long)n * (n_heads + 2 * n_kv);
+    const dim3 grid((unsigned)((items + 7) / 8));
+    switch (D / 32) {
+        case 1: append_kernel<1><<<grid, 256, 0, stream>>>(a); break;
+        case 2: append_kernel<2><<<grid, 256, 0, stream>>>(a); break;
+        case 3: append_kernel<3><<<grid, 256, 0, stream>>>(a); break;
+        case 4: append_kernel<4><<<grid, 256, 0, stream>>>(a); break;
+        case 5: append_kernel<5><<<grid, 256, 0, stream>>>(a); break;
+        case 6: append_kernel<6><<<grid, 256, 0, stream>>>(a); break;
+        case 7: append_kernel<7><<<grid, 256, 0, stream>>>(a); break;
+        default: append_kernel<8><<<grid, 256, 0, stream>>>(a); break;
+    }
+    NN_LAUNCH_OK("qk_norm_rope_append_q4");
+    return 0;
+}
+
+extern "C" int nncpu_q4_read(const uint8_t* k_pages, const uint8_t* v_pages, int n_pages, const int* block_table, int bt_stride,
+                             const int* tok_seq, const int* tok_pos, void* k_out, void* v_out, int out_dt, int n, int n_kv, int D,
+                             cudaStream_t stream) {
+    NN_CHECK(q4_lanes_ok(D), "q4_read: heads of %d lanes (whole groups of 32, at most 256)", D);
+    NN_CHECK(n >= 0 && n_kv > 0 && bt_stride > 0 && n_pages > 0, "q4_read: %d tokens, %d heads, %d pages", n, n_kv, n_pages);
+    if (n == 0) return 0;
+    const long items = (long)n * n_kv;
+    read_kernel<<<dim3((unsigned)((items + 7) / 8), 2), 256, 0, stream>>>(k_pages, v_pages, n_pages, block_table, bt_stride, tok_seq, tok_pos,
+                                                                         k_out, v_out, out_dt, n, n_kv, D);
+    NN_LAUNCH_OK("q4_read");
+    return 0;
+}

@@ -26,7 +26,7 @@ CSRC = Path(__file__).resolve().parent.parent / "csrc"
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
               "-Xcompiler", "-fPIC", "-shared"]
 LIBRARIES = ("generic", "gemm_sm100", "linear_skinny", "attention_mma", "attention_tc", "recurrent", "state_space",
-             "linear_f32", "attention_f32")
+             "linear_f32", "attention_f32", "cache_q4", "attention_q4", "token_logprobs")
 
 _loaded: Dict[str, ctypes.CDLL] = {}
 _lock = threading.Lock()

@@ -1558,3 +1558,196 @@ def sample_temperature(logits, uniforms, out, temperature: float) -> None:
     scratch = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
     _call("generic", "nncpu_sample_temperature", _ptr(logits), _ptr(uniforms), _ptr(out), _i(n), _i(vocab),
           _f(temperature), _ptr(scratch), ctypes.c_long(need), _stream())
+
+
+# -- keys and values in 4 bits -------------------------------------------------------------------------------------------
+
+Q4_GROUP = 32      # neighbouring lanes of a head that share a step and a least value
+
+
+def q4_supported(head_dim: int) -> bool:
+    """Whether a cache of 4 bits holds heads of ``head_dim`` lanes: whole groups of 32, at most 256 lanes."""
+    return 0 < head_dim <= 256 and head_dim % Q4_GROUP == 0
+
+
+def q4_page_bytes(head_dim: int) -> int:
+    """Bytes of a page's keys (or values) of one head: 64 positions of 4 bits a lane and two float16 numbers a group."""
+    return 64 * head_dim * 5 // 8
+
+
+def _need(cond: bool, fn: str, what: str) -> None:
+    if not cond:
+        raise InvalidArgument(f"{fn}: {what}")
+
+
+def _on_current_device(fn: str, *tensors) -> None:
+    """The kernels are launched on the current device's stream: every tensor has to live there."""
+    on = {t.device for t in tensors if t is not None and not (t.is_meta and _dry)}
+    _need(len(on) == 1, fn, f"tensors on several devices ({', '.join(sorted(map(str, on)))})")
+    dev = on.pop()
+    if dev.type == "cuda":
+        _need(dev.index == torch.cuda.current_device(), fn, f"tensors on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _int32(fn: str, **tensors) -> None:
+    for name, t in tensors.items():
+        _need(t.dtype == torch.int32, fn, f"{name} holds int32, not {t.dtype}")
+
+
+def _q4_pages(fn: str, k_pages, v_pages, n_kv: int, head_dim: int) -> None:
+    _need(q4_supported(head_dim), fn, f"heads of {head_dim} lanes (a cache of 4 bits holds whole groups of {Q4_GROUP}, at most 256 lanes)")
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        _need(t.dtype == torch.uint8 and t.dim() == 3 and t.shape[1:] == (n_kv, q4_page_bytes(head_dim)) and t.is_contiguous(), fn,
+              f"{name} are contiguous uint8 [pages, {n_kv}, {q4_page_bytes(head_dim)}], not {t.dtype} {list(t.shape)}")
+        _need(_aligned(t), fn, f"{name} do not start on a 16-byte boundary")
+    _need(k_pages.shape == v_pages.shape, fn, f"{k_pages.shape[0]} pages of keys and {v_pages.shape[0]} of values")
+
+
+def _q4_places(fn: str, n: int, block_table, tok_seq, tok_pos) -> None:
+    _int32(fn, block_table=block_table, tok_seq=tok_seq, tok_pos=tok_pos)
+    _need(block_table.dim() == 2 and block_table.shape[1] > 0, fn, f"a block table of shape {list(block_table.shape)}")
+    _need(tok_seq.numel() >= n and tok_pos.numel() >= n, fn, f"{n} tokens, {tok_seq.numel()} sequences and {tok_pos.numel()} positions of them")
+
+
+def qk_norm_rope_append_q4(qkv, q_gamma, k_gamma, eps: float, cos_sin, tok_seq, tok_pos, block_table, k_pages, v_pages, q_out,
+                           n_heads: int, n_kv: int, head_dim: int, q_temp=None) -> None:
+    """``qk_norm_rope_append`` for a cache of 4 bits: per-head norm and rotation of q and k, q to ``q_out`` and the tokens' keys and
+    values, cut to 4 bits, to their pages.  qkv [n, >= (n_heads + 2 n_kv) * head_dim] holds the heads of q, of k and of v;
+    ``cos_sin`` float32 [n, half, 2] turns the pairs (i, i + half); pages uint8 [n_pages, n_kv, ``q4_page_bytes``].
+
+    A head's lanes are cut in groups of 32.  With lo and hi the group's least and greatest number, a lane is d c + lo,
+    d = (hi - lo) / 15 and lo both float16, and c = round((x - lo) / d) one of 0 to 15: a number is off by at most half a step d (and
+    lo's rounding).  Numbers beyond +-65504 count as that; a group with a NaN is NaN.  Keys are normed and rotated in 64 bits, so
+    that a code does not hang on the order of a sum.  ``n_kv`` 0: qkv holds q only and nothing is appended.  A token of sequence -1, or
+    whose position has no page, is not appended; two tokens at one place leave either.  ``q_temp`` as in ``qk_norm_rope_append``."""
+    fn = "qk_norm_rope_append_q4"
+    n = q_out.shape[0]
+    half = 0 if cos_sin is None else cos_sin.shape[1]
+    coef, every = q_temp if q_temp is not None else (0.0, 1)
+    _need(q_out.shape == (n, n_heads * head_dim) and qkv.dim() == 2 and qkv.shape[0] == n
+          and qkv.shape[1] >= (n_heads + 2 * n_kv) * head_dim, fn,
+          f"{n_heads} heads over {n_kv} of {head_dim} lanes in rows of {list(qkv.shape)}, queries to {list(q_out.shape)}")
+    _need(q4_supported(head_dim), fn, f"heads of {head_dim} lanes (a cache of 4 bits holds whole groups of {Q4_GROUP}, at most 256 lanes)")
+    _need(cos_sin is None or (cos_sin.dtype == torch.float32 and cos_sin.shape == (n, half, 2) and 2 * half <= head_dim), fn,
+          "the rotation is float32 [tokens, pairs, 2], at most half a head's lanes of pairs")
+    _need(all(g is None or g.numel() == head_dim for g in (q_gamma, k_gamma)) and (q_gamma is None or k_gamma is None
+          or q_gamma.dtype == k_gamma.dtype), fn, f"norm weights of {head_dim} lanes and one type")
+    _int32(fn, tok_seq=tok_seq, tok_pos=tok_pos)
+    _need(tok_seq.numel() >= n and tok_pos.numel() >= n, fn, f"{n} tokens, {tok_seq.numel()} sequences and {tok_pos.numel()} positions of them")
+    if n_kv:
+        _q4_pages(fn, k_pages, v_pages, n_kv, head_dim)
+        _q4_places(fn, n, block_table, tok_seq, tok_pos)
+    else:
+        k_pages = v_pages = block_table = None
+    _on_current_device(fn, qkv, q_gamma, k_gamma, cos_sin, tok_seq, tok_pos, block_table, k_pages, v_pages, q_out)
+    g = q_gamma if q_gamma is not None else k_gamma
+    _call("cache_q4", "nncpu_qk_norm_rope_append_q4", _ptr(qkv), _i(_code(qkv)), _i(qkv.shape[1]), _ptr(q_gamma), _ptr(k_gamma),
+          _i(_code(g)), ctypes.c_double(float(eps)), _ptr(cos_sin), _i(half), _ptr(tok_seq), _ptr(tok_pos), _ptr(block_table),
+          _i(block_table.shape[1] if n_kv else 0), _ptr(k_pages), _ptr(v_pages), _i(k_pages.shape[0] if n_kv else 0), _ptr(q_out),
+          _i(_code(q_out)), _i(n), _i(n_heads), _i(n_kv), _i(head_dim), _f(coef), _i(every), _stream())
+
+
+def q4_read(k_pages, v_pages, block_table, tok_seq, tok_pos, k_out, v_out) -> None:
+    """What a cache of 4 bits holds of given tokens, as numbers: keys and values of the token at position tok_pos[t] of sequence
+    tok_seq[t] to ``k_out`` and ``v_out`` [n, n_kv * head_dim] (float32 or bfloat16).  A token of sequence -1, or without a page: zeros."""
+    fn = "q4_read"
+    n, n_kv = k_out.shape[0], k_pages.shape[1]
+    head_dim = k_out.shape[1] // n_kv
+    _q4_pages(fn, k_pages, v_pages, n_kv, head_dim)
+    _q4_places(fn, n, block_table, tok_seq, tok_pos)
+    _need(k_out.shape == v_out.shape == (n, n_kv * head_dim) and k_out.dtype == v_out.dtype, fn,
+          f"keys to {k_out.dtype} {list(k_out.shape)}, values to {v_out.dtype} {list(v_out.shape)}")
+    _on_current_device(fn, k_pages, v_pages, block_table, tok_seq, tok_pos, k_out, v_out)
+    _call("cache_q4", "nncpu_q4_read", _ptr(k_pages), _ptr(v_pages), _i(k_pages.shape[0]), _ptr(block_table), _i(block_table.shape[1]),
+          _ptr(tok_seq), _ptr(tok_pos), _ptr(k_out), _ptr(v_out), _i(_code(k_out)), _i(n), _i(n_kv), _i(head_dim), _stream())
+
+
+def _attention_q4_check(fn: str, q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads: int, n_kv: int, head_dim: int,
+                        window: int, keep: int, cap: float, sinks) -> int:
+    n = q.shape[0]
+    _need(n_heads > 0 and n_kv > 0 and n_heads % n_kv == 0, fn, f"{n_heads} heads over {n_kv}")
+    _q4_pages(fn, k_pages, v_pages, n_kv, head_dim)
+    _q4_places(fn, n, block_table, tok_seq, tok_pos)
+    _need(q.shape == out.shape == (n, n_heads * head_dim) and q.dtype == out.dtype, fn,
+          f"queries {q.dtype} {list(q.shape)}, output {out.dtype} {list(out.shape)}, {n_heads} heads of {head_dim} lanes")
+    _need(keep >= 0 and (keep == 0 or window > 0) and cap >= 0.0, fn, f"{keep} kept keys with a window of {window}, a cap of {cap}")
+    _need(sinks is None or (sinks.dtype == torch.float32 and sinks.numel() == n_heads), fn, f"sinks are float32 [{n_heads}]")
+    _on_current_device(fn, q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, sinks)
+    return n
+
+
+def _q4_longest(block_table, longest: int, window: int, keep: int) -> int:
+    """At least as many keys as a token walks through: what the tables have room for, or the window with the pages at its ends."""
+    room = block_table.shape[1] * 64
+    room = min(room, longest) if longest else room
+    return max(1, min(room, abs(window) + keep + 128) if window else room)
+
+
+def attention_q4_scratch_floats(n_tok: int, n_heads: int, n_kv: int, head_dim: int, dtype, longest: int) -> int:
+    """Floats of scratch that ``attention_q4`` needs at these sizes."""
+    lib = library.load("attention_q4")
+    lib.nncpu_attention_q4_scratch.restype = ctypes.c_long
+    return lib.nncpu_attention_q4_scratch(_i(n_tok), _i(n_heads), _i(n_kv), _i(head_dim), _i(_DT[dtype]), _i(longest))
+
+
+def attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads: int, n_kv: int, head_dim: int, scale: float,
+                 window: int = 0, slope_base: float = 0.0, sinks=None, keep: int = 0, cap: float = 0.0, head_gate=None,
+                 longest: int = 0, scratch=None) -> None:
+    """Causal attention of each token over its sequence's pages of a cache of 4 bits, token by token (decode steps, and a few tokens a
+    sequence); q and out [n, n_heads * head_dim] of one type.  The options are those of ``attention``.  ``longest``: at least as many
+    keys as any token sees (0: as the block tables have room for).  ``scratch``: float32, ``attention_q4_scratch_floats``
+    elements for the same ``longest`` (None: taken from the allocator).  A token of sequence -1 gives zeros; a page that
+    is not there (an id outside the pages) holds no keys."""
+    n = _attention_q4_check("attention_q4", q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads, n_kv, head_dim, window,
+                            keep, cap, sinks)
+    longest = _q4_longest(block_table, longest, window, keep)
+    if scratch is None and not _dry:
+        need = attention_q4_scratch_floats(n, n_heads, n_kv, head_dim, q.dtype, longest)
+        scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
+    _need(scratch is None or scratch.dtype == torch.float32, "attention_q4", "scratch is float32")
+    _call("attention_q4", "nncpu_attention_q4", _ptr(q), _i(_code(q)), _ptr(k_pages), _ptr(v_pages), _i(k_pages.shape[0]),
+          _ptr(block_table), _i(block_table.shape[1]), _ptr(tok_seq), _ptr(tok_pos), _ptr(out), _ptr(scratch),
+          _l(0 if scratch is None else scratch.numel()), _i(n), _i(n_heads), _i(n_kv), _i(head_dim), _f(scale), _i(window), _i(keep),
+          _f(slope_base), _ptr(sinks), _f(cap), *_head_gate(head_gate, n, n_heads), _i(longest), _stream())
+
+
+def attention_q4_prompt(q, k_pages, v_pages, block_table, cu_seqlens, tok_seq, tok_pos, out, n_seqs: int, n_heads: int, n_kv: int,
+                        head_dim: int, scale: float, longest: int, status, window: int = 0, slope_base: float = 0.0, sinks=None,
+                        keep: int = 0, cap: float = 0.0, head_gate=None) -> None:
+    """``attention_q4`` for prompts and portions of them: any number of tokens a sequence, at consecutive positions (``cu_seqlens``
+    int32 [n_seqs + 1]: each sequence's first token).  ``longest``: at least as many keys as any token sees."""
+    fn = "attention_q4_prompt"
+    _int32(fn, cu_seqlens=cu_seqlens)
+    _need(n_seqs > 0 and cu_seqlens.numel() >= n_seqs + 1 and longest > 0, fn, f"{n_seqs} sequences, {cu_seqlens.numel()} places, {longest} keys")
+    attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads, n_kv, head_dim, scale, window, slope_base, sinks, keep,
+                 cap, head_gate, longest)
+
+
+# -- log probabilities ---------------------------------------------------------------------------------------------------
+
+LOGPROBS_MAX_TOP = 64
+
+
+def token_logprobs(logits, targets, logprobs, entropy, top=None, ids=None) -> None:
+    """For every row of ``logits`` [n, vocab] (float32 or bfloat16): ``logprobs`` float32 [n], the log probability of token
+    targets[r] (int32) under the row's softmax; ``entropy`` float32 [n], in nats; with ``top`` float32 [n, k] and ``ids`` int32 [n, k]
+    (k up to 64) the k most probable tokens, by (log probability descending, id ascending).
+
+    A NaN counts as -inf; a token of -inf has log probability -inf.  A row with nothing above -inf gives -inf for every token and an
+    entropy of 0; one with a logit of +inf gives NaN (and its order).  A target outside the vocabulary gives NaN."""
+    fn = "token_logprobs"
+    _need(logits.dim() == 2 and logits.shape[1] > 0, fn, f"logits of shape {list(logits.shape)}")
+    n, vocab = logits.shape
+    _int32(fn, targets=targets)
+    _need(targets.shape == (n,) and logprobs.shape == (n,) and entropy.shape == (n,) and logprobs.dtype == entropy.dtype == torch.float32, fn,
+          f"{n} rows: targets int32 [{n}], logprobs and entropy float32 [{n}]")
+    _need((top is None) == (ids is None), fn, "top and ids come together")
+    k = 0
+    if top is not None:
+        k = top.shape[1] if top.dim() == 2 else -1
+        _int32(fn, ids=ids)
+        _need(top.shape == ids.shape == (n, k) and top.dtype == torch.float32, fn, f"top float32 and ids int32 [{n}, k]")
+        _need(0 < k <= min(LOGPROBS_MAX_TOP, vocab), fn, f"the best {k} of {vocab} (1 to {LOGPROBS_MAX_TOP})")
+    _on_current_device(fn, logits, targets, logprobs, entropy, top, ids)
+    _call("token_logprobs", "nncpu_token_logprobs", _ptr(logits), _i(_code(logits)), _ptr(targets), _ptr(logprobs), _ptr(entropy), _ptr(top),
+          _ptr(ids), _i(n), _i(vocab), _i(k), _stream())
