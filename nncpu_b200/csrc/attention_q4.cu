@@ -1,10 +1,11 @@
 // Causal attention over the 4-bit cache (cache_q4.cuh says how its pages lie), token by token: every token of the step attends to
 // the pages of its sequence up to its own position (crates/nncpu/src/model/forward.rs:383-426).
 //
+//   stream_kernel: bfloat16 queries, heads of up to 128 lanes, on the tensor cores, straight from the codes (see there).
 //   any_kernel: any type of queries, any whole number of 32-lane groups; 32-bit arithmetic on numbers taken out of the pages.
 //     A block takes one token, up to eight query heads of one key/value head and a split of their pages, turns a page of keys and
 //     then one of values into 32-bit numbers in shared memory and works on those.
-// Splits meet in merge_kernel, in the order of their keys.
+// Parts of a token's keys meet in a second kernel, in the order of the keys.
 
 #include <math.h>
 
@@ -50,6 +51,552 @@ __device__ __forceinline__ float closing_factor(const AttnQ4& p, int t, int h, f
     float inv = l > 0.0f ? 1.0f / l : 0.0f;
     if (p.head_gate != nullptr) inv *= 1.0f / (1.0f + expf(0.0f - p.head_gate[(size_t)t * p.gate_ld + h]));
     return inv;
+}
+
+// ---------------------------------------------------------------------------
+// stream_kernel.  With a key j's lanes k = d_g c + m_g (g the lane's group of 32) and likewise for values,
+//   score_j = sum_g d_jg (sum_x q_x c_jx) + sum_g m_jg (sum_x q_x),    out_x = sum_j (p_j d_jg) (c_jx - 8) + sum_j p_j (m_jg + 8 d_jg),
+// so the tensor cores multiply the codes themselves, whole numbers and exact in float16: 16 keys are the rows of
+// m16n8k16 (a group of lanes is two of its steps), the query heads that share the key/value head its columns.
+//   * A code becomes a float16 number without a conversion: 0x6400 | c is 1024 + c, and with the code four bits further up
+//     0x5400 | 16 c is 64 + c; one AND-OR (and a shift every other time) makes two of them.
+//   * A key group's sum, in 32 bits, is multiplied by d.  The rest, sum_g m_g (sum q) less what the 1024 and 64 added,
+//     sum_g d_g off_g, is itself a product of a key's eight numbers (d_0, m_0, d_1, ...) with numbers of the query: one more
+//     tensor-core step per 16 keys, the query's side in two float16 parts (22 bits).
+//   * Of the values 1032 or 72 is subtracted at once, which is exact: a sum over thousands of keys of numbers around 1024
+//     would lose what is left of c - 8.  sum_j p_j d_jg and sum_j p_j m_jg are a tensor-core step as well.
+//   * Queries enter as float16 times a power of two per head that makes the greatest at most 1 (exact for all but what is
+//     2^-14 below it).  Weights are float16 with 11 bits: p is taken against a reference below the maximum so that p and p d
+//     lie in float16's middle, and the reference moves when a weight passes 2^15 or a step passes what it allows.
+// Rounded below 32 bits are: a weight p, and p d, both to 11 bits.
+//
+// A warp of the block takes 16 of a page's 64 keys: it brings their codes and scales (2.5 KB for D = 128) to its own ring in
+// shared memory by 16-byte cp.async and shares nothing with the other warps until a token's pages are done, when the four
+// parts meet in shared memory.
+//
+// The pages of all (token, key/value head) pairs lie in one row, of which every block takes an equal share, wherever that
+// begins and ends: unequal sequences cost nothing, and there is one wave of blocks.  A pair that lies within one block is finished by it; of
+// the others every block leaves its part (its first and its last pair at most) in scratch for stream_merge_kernel.
+// ---------------------------------------------------------------------------
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kStreamWarps = 4;
+constexpr int kStreamStages = 4;            // pages of a warp's ring
+
+struct Stream {
+    int heads;              // query heads of a pair (a part of those that share a key/value head where these are many)
+    int chunks;             // such parts of a key/value head
+    int pairs;              // n_kv * chunks: pairs of a token
+    int min_pages;          // pages that a block takes at least
+    int blocks;             // blocks of the launch
+    float scale2;           // scale * log2(e)
+    ScoreCap cap;
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// ldmatrix, two 8x8 tiles transposed: lane l of the first 16 gives the address of row l.
+__device__ __forceinline__ void ldmatrix_x2_trans(uint32_t& a, uint32_t& b, uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ float low_half(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w & 0xFFFF))); }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Codes I and I + 4 of a word as float16 numbers: 1024 + c for even I, 64 + c for odd I.
+template <int I>
+__device__ __forceinline__ uint32_t codes_at(uint32_t w) {
+    uint32_t d;
+    if (I >= 2) w >>= 8;
+    if (I % 2 == 0) asm("lop3.b32 %0, %1, 0x000F000F, 0x64006400, 0xEA;" : "=r"(d) : "r"(w));     // (a & b) | c
+    else asm("lop3.b32 %0, %1, 0x00F000F0, 0x54005400, 0xEA;" : "=r"(d) : "r"(w));
+    return d;
+}
+// The same as c - 8.
+template <int I>
+__device__ __forceinline__ uint32_t centred_at(uint32_t w) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(codes_at<I>(w)), "r"(I % 2 == 0 ? 0x64086408u : 0x54805480u));
+    return d;
+}
+
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t (&w)[N], const uint8_t* p) {
+    if constexpr (N == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x; w[1] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    }
+}
+
+// The pages that a token sees (none for a row of no sequence).
+__device__ __forceinline__ int pages_of(const AttnQ4& p, int t) {
+    const int pos = p.tok_pos[t];
+    if (p.tok_seq[t] < 0 || pos < 0) return 0;
+    return PageWalk(first_visible_key(pos, p.window), pos, p.keep).n;
+}
+
+// How the row of pages is cut: its length, the blocks that share it, and where a block's share begins.
+struct Row {
+    long pages;
+    int blocks;
+    __device__ __forceinline__ long start(int b) const { return pages * b / blocks; }
+    __device__ __forceinline__ int block_of(long page) const { return (int)(((page + 1) * blocks - 1) / pages); }
+};
+// (Every warp by itself, 32 tokens at a time.)
+__device__ __forceinline__ Row row_of(const AttnQ4& p, const Stream& st, int lane) {
+    int sum = 0;
+    for (int t = lane; t < p.n; t += 32) sum += pages_of(p, t);
+    long total = sum;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    Row row;
+    row.pages = total * st.pairs;
+    const long b = (row.pages + st.min_pages - 1) / st.min_pages;
+    row.blocks = (int)(b < st.blocks ? b : st.blocks);
+    return row;
+}
+
+// A place in the row of pages: page i of the n that pair y of token t walks through.
+struct Place {
+    int t, y, i, n;
+    // to the next pair with pages
+    __device__ __forceinline__ void next_pair(const AttnQ4& p, const Stream& st) {
+        i = 0;
+        if (++y == st.pairs) {
+            y = 0;
+            do { ++t; } while (t < p.n && (n = pages_of(p, t)) == 0);
+        }
+    }
+};
+__device__ __forceinline__ Place place_of(const AttnQ4& p, const Stream& st, long page, int lane) {
+    long before = 0;
+    for (int t0 = 0;; t0 += 32) {
+        const int n = t0 + lane < p.n ? pages_of(p, t0 + lane) : 0;
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const unsigned beyond = __ballot_sync(0xffffffffu, before + (long)upto * st.pairs > page);
+        if (beyond != 0 || t0 + 32 >= p.n) {
+            const int l = beyond != 0 ? __ffs(beyond) - 1 : 31;
+            const int nl = __shfl_sync(0xffffffffu, n, l), at = __shfl_sync(0xffffffffu, upto, l) - nl;
+            const long rest = page - before - (long)at * st.pairs;
+            Place w;
+            w.t = t0 + l;
+            w.n = nl;
+            w.y = (int)(rest / max(nl, 1));
+            w.i = (int)(rest - (long)w.y * nl);
+            return w;
+        }
+        before += (long)__shfl_sync(0xffffffffu, upto, 31) * st.pairs;
+    }
+}
+
+// The reference lies `room` below the greatest score when it moves, so that weights start at 2^room; it moves when one passes
+// 2^(room + kLag).  With steps of at most 1 room is 11: weights of 2^11 to 2^15 and what is 2^-25 of them are normal numbers of
+// float16, and so is p d.  Greater steps (they are at most 8 736: numbers lie within +-65 504) leave less.
+constexpr float kLag = 4.0f;
+__device__ __forceinline__ float headroom(float d_max) { return d_max <= 1.0f ? 11.0f : 11.0f - ceilf(log2f(d_max)); }
+
+template <int NG, int NT>
+__global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 3 : 2) stream_kernel(const AttnQ4 p, const Stream st) {
+    constexpr int D = 32 * NG, COLS = 8 * NT;
+    constexpr int kCodes = 256 * NG, kScales = 64 * NG;          // bytes of a warp's 16 keys
+    constexpr int kVCodes = kCodes, kKScales = 2 * kCodes, kVScales = 2 * kCodes + kScales, kStage = 2 * (kCodes + kScales);   // a ring's stage
+    constexpr unsigned kPageBytes = 40 * D;
+    extern __shared__ __align__(128) uint8_t stream_smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    uint8_t* ring = stream_smem + warp * kStreamStages * kStage;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    float* meet = reinterpret_cast<float*>(stream_smem + kStreamWarps * kStreamStages * kStage);   // [warps][COLS][D + 2]
+
+    // rows of no sequence are zeros
+    for (int t = blockIdx.x; t < p.n; t += gridDim.x)
+        if (pages_of(p, t) == 0)
+            for (int i = threadIdx.x; i < p.n_heads * D; i += 32 * kStreamWarps)
+                reinterpret_cast<__nv_bfloat16*>(p.out)[(size_t)t * p.n_heads * D + i] = __float2bfloat16_rn(0.0f);
+    const Row row = row_of(p, st, lane);
+    if ((int)blockIdx.x >= row.blocks) return;
+    const long first_page = row.start(blockIdx.x);
+    const int n_mine = (int)(row.start(blockIdx.x + 1) - first_page);
+    Place here = place_of(p, st, first_page, lane), ahead = here;
+    int fetched = 0;
+    unsigned there = 0;                     // bit s: stage s holds a page (and not one that is missing)
+    int ids = -1, ids_left = 0;             // the next ids_left pages of the pair that is being fetched: lane l holds the id of the l-th
+    const uint8_t *k_at = nullptr, *v_at = nullptr, *s_at = nullptr;   // this lane's first 16 bytes of a page: keys, values, scales
+    const unsigned stride = (unsigned)p.n_kv * kPageBytes;
+
+    // asks for this warp's keys of the next page (nothing for a page that is not there)
+    auto fetch = [&](int stage) {
+        if (fetched < n_mine) {
+            if (ids_left == 0) {
+                const int pos = p.tok_pos[ahead.t];
+                const PageWalk walk(first_visible_key(pos, p.window), pos, p.keep);
+                ids_left = min(32, ahead.n - ahead.i);
+                const int pi = walk.page(min(ahead.i + lane, ahead.n - 1));
+                ids = pi < p.bt_stride ? p.block_table[(size_t)p.tok_seq[ahead.t] * p.bt_stride + pi] : -1;
+                if (ids >= p.n_pages) ids = -1;
+                const size_t head = (size_t)(ahead.y / st.chunks) * kPageBytes;
+                k_at = p.k_pages + head + warp * kCodes + lane * 16;
+                v_at = p.v_pages + head + warp * kCodes + lane * 16;
+                s_at = (lane < 4 * NG ? p.k_pages : p.v_pages) + head + 32 * D + warp * kScales + (lane < 4 * NG ? lane : lane - 4 * NG) * 16;
+            }
+            const int id = __shfl_sync(0xffffffffu, ids, 0);
+            ids = __shfl_down_sync(0xffffffffu, ids, 1);
+            if (id >= 0) {
+                there |= 1u << stage;
+                const size_t at = (size_t)(unsigned)id * stride;
+                const uint32_t dst = ring_at + stage * kStage + lane * 16;
+#pragma unroll
+                for (int k = 0; k < (16 * NG + 31) / 32; ++k)
+                    if (16 * NG % 32 == 0 || k * 32 + lane < 16 * NG) {
+                        cp_async16(dst + k * 512, k_at + at + k * 512);
+                        cp_async16(dst + kVCodes + k * 512, v_at + at + k * 512);
+                    }
+                if (NG == 4 || lane < 8 * NG) cp_async16(dst + kKScales, s_at + at);
+            } else {
+                there &= ~(1u << stage);
+            }
+            ++fetched;
+            --ids_left;
+            if (++ahead.i == ahead.n) ahead.next_pair(p, st);
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < kStreamStages - 1; ++s) fetch(s);
+
+    int stage = 0;
+    for (int done = 0; done < n_mine;) {
+        // -- a pair, or the part of it that lies here
+        const int t = here.t, take = min(here.n - here.i, n_mine - done);
+        const int kvh = here.y / st.chunks, h0 = kvh * (p.n_heads / p.n_kv) + here.y % st.chunks * st.heads;
+        const int nh = min(st.heads, (kvh + 1) * (p.n_heads / p.n_kv) - h0);
+        const int pos = p.tok_pos[t], first = first_visible_key(pos, p.window);
+        const PageWalk walk(first, pos, p.keep);
+        // Queries as the right-hand operand: head r of the column tile, the lanes of word (c, g), in the order of the codes' pairs.
+        uint32_t qb[NT][NG][4];
+        uint32_t qhi[NT], qlo[NT];     // the right-hand operand of (d_c, m_c): (-off, sum of q) of group c and head r, in two parts
+        float col[NT][2];              // what scores of heads 2 c and 2 c + 1 are multiplied by
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            uint4 w[NG];
+            float top = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                w[g] = make_uint4(0, 0, 0, 0);
+                if (8 * nt + r < nh)
+                    w[g] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + ((size_t)t * p.n_heads + h0 + 8 * nt + r) * D +
+                                                           32 * g + 8 * c);
+                const float2 a = two_bf16(w[g].x), b = two_bf16(w[g].y), e = two_bf16(w[g].z), f = two_bf16(w[g].w);
+                top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))),
+                                       fmaxf(fmaxf(fabsf(e.x), fabsf(e.y)), fmaxf(fabsf(f.x), fabsf(f.y)))));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // 2^e with top < 2^e (from the exponent's bits; of zeros and the smallest numbers 2^-100)
+            const int e = max((int)(__float_as_uint(top) >> 23), 27) - 126;
+            const float down = __int_as_float((127 - min(e, 126)) << 23), up = __int_as_float((127 + min(e, 126)) << 23);
+            float qs = 0.0f, off = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const float2 a = two_bf16(w[g].x), b = two_bf16(w[g].y), x = two_bf16(w[g].z), y = two_bf16(w[g].w);
+                qb[nt][g][0] = pack_f16(a.x * down, x.x * down);
+                qb[nt][g][1] = pack_f16(a.y * down, x.y * down);
+                qb[nt][g][2] = pack_f16(b.x * down, y.x * down);
+                qb[nt][g][3] = pack_f16(b.y * down, y.y * down);
+                // the sums are those of the numbers as they are multiplied
+                const float2 t0 = __half22float2(*reinterpret_cast<const __half2*>(&qb[nt][g][0])), t1 = __half22float2(*reinterpret_cast<const __half2*>(&qb[nt][g][1]));
+                const float2 t2 = __half22float2(*reinterpret_cast<const __half2*>(&qb[nt][g][2])), t3 = __half22float2(*reinterpret_cast<const __half2*>(&qb[nt][g][3]));
+                float even = (t0.x + t0.y) + (t2.x + t2.y), odd = (t1.x + t1.y) + (t3.x + t3.y);
+#pragma unroll
+                for (int k = 1; k <= 2; k <<= 1) {
+                    even += __shfl_xor_sync(0xffffffffu, even, k);
+                    odd += __shfl_xor_sync(0xffffffffu, odd, k);
+                }
+                if (g == c) {
+                    qs = even + odd;
+                    off = 0.0f - (1024.0f * even + 64.0f * odd);
+                }
+            }
+            qhi[nt] = pack_f16(off, qs);
+            const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&qhi[nt]));
+            qlo[nt] = pack_f16(off - hi.x, qs - hi.y);
+            const float by = st.cap.out > 0.0f ? up : up * st.scale2;
+            col[nt][0] = __shfl_sync(0xffffffffu, by, 8 * c);
+            col[nt][1] = __shfl_sync(0xffffffffu, by, 8 * c + 4);
+        }
+        float slope2[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) slope2[nt][e] = p.slope_base != 0.0f ? slope_of(p, h0 + 8 * nt + 2 * c + e) * kLog2e : 0.0f;
+        float o[NT][2 * NG][4];
+        float od[NT][4];               // row r: sum of p d (r even) or p m (r odd) of group r / 2, heads 2 c and 2 c + 1
+        float m[NT][2], l[NT][2];      // reference and sum of the weights
+        float d_max = 1.0f, room = 11.0f;     // greatest step that the references leave room for, and how much that is
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int k = 0; k < 2 * NG; ++k) o[nt][k][0] = o[nt][k][1] = o[nt][k][2] = o[nt][k][3] = 0.0f;
+            od[nt][0] = od[nt][1] = od[nt][2] = od[nt][3] = 0.0f;
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.0f;
+        }
+        for (int i = 0; i < take; ++i) {
+            cp_async_wait<kStreamStages - 2>();
+            __syncwarp();
+            uint8_t* at = ring + stage * kStage;
+            const bool missing = (there >> stage & 1) == 0;
+            fetch((stage + kStreamStages - 1) % kStreamStages);
+            stage = (stage + 1) % kStreamStages;
+            const int key0 = walk.page(here.i + i) * kPage + 16 * warp;
+            if (missing || key0 > pos || (key0 + 15 < first && key0 >= p.keep)) continue;      // none of these keys is seen
+            const bool full = key0 >= first && key0 + 15 <= pos;
+            if (!full) {
+                // what is not seen may hold anything, NaN too: its weight will be zero, and so must its numbers be
+                const int key = key0 + lane;
+                if (lane < 16 && (key > pos || (key < first && key >= p.keep)))
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) *reinterpret_cast<uint32_t*>(at + kVScales + lane * 4 * NG + g * 4) = 0;
+                __syncwarp();
+            }
+            // -- scores
+            uint32_t kw[2][NG], ks[2][NG];
+            lds_words<NG>(kw[0], at + r * 16 * NG + c * 4 * NG);
+            lds_words<NG>(kw[1], at + (r + 8) * 16 * NG + c * 4 * NG);
+            lds_words<NG>(ks[0], at + kKScales + r * 4 * NG);
+            lds_words<NG>(ks[1], at + kKScales + (r + 8) * 4 * NG);
+            uint32_t dm[2] = {0, 0};
+            if (NG == 4 || c < NG) {
+                dm[0] = *reinterpret_cast<const uint32_t*>(at + kKScales + r * 4 * NG + c * 4);
+                dm[1] = *reinterpret_cast<const uint32_t*>(at + kKScales + (r + 8) * 4 * NG + c * 4);
+            }
+            // row r of the values' (d, m): those of keys 2 c, 2 c + 1 and of 2 c + 8, 2 c + 9
+            uint32_t sd[2] = {0, 0};
+            if constexpr (NG == 4) {
+                ldmatrix_x2_trans(sd[0], sd[1], (uint32_t)__cvta_generic_to_shared(at) + kVScales + (lane & 15) * 16);
+            } else if (r < 2 * NG) {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(at + kVScales) + 4 * c * NG + r;
+                sd[0] = h[0] | (uint32_t)h[2 * NG] << 16;
+                sd[1] = h[16 * NG] | (uint32_t)h[18 * NG] << 16;
+            }
+            float z[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0.0f;
+                mma_f16(z[nt], dm[0], dm[1], dm[0], dm[1], qhi[nt], qlo[nt]);
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const uint32_t a[2][4] = {{codes_at<0>(kw[0][g]), codes_at<0>(kw[1][g]), codes_at<1>(kw[0][g]), codes_at<1>(kw[1][g])},
+                                          {codes_at<2>(kw[0][g]), codes_at<2>(kw[1][g]), codes_at<3>(kw[0][g]), codes_at<3>(kw[1][g])}};
+                const float d0 = low_half(ks[0][g]), d1 = low_half(ks[1][g]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    mma_f16(acc, a[0][0], a[0][1], a[0][2], a[0][3], qb[nt][g][0], qb[nt][g][1]);
+                    mma_f16(acc, a[1][0], a[1][1], a[1][2], a[1][3], qb[nt][g][2], qb[nt][g][3]);
+                    z[nt][0] = fmaf(acc[0], d0, z[nt][0]);
+                    z[nt][1] = fmaf(acc[1], d0, z[nt][1]);
+                    z[nt][2] = fmaf(acc[2], d1, z[nt][2]);
+                    z[nt][3] = fmaf(acc[3], d1, z[nt][3]);
+                }
+            }
+            // -- weights
+            const float2 steps = __half22float2(__hmax2(*reinterpret_cast<const __half2*>(&sd[0]), *reinterpret_cast<const __half2*>(&sd[1])));
+            const float step = (r & 1) == 0 ? fmaxf(steps.x, steps.y) : 0.0f;
+            bool moves = step > d_max;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v = z[nt][e] * col[nt][e & 1];
+                    if (st.cap.out > 0.0f) v = capped_score(v, st.cap);
+                    if (!full || p.slope_base != 0.0f) {
+                        const int key = key0 + r + 8 * (e >> 1);
+                        v -= slope2[nt][e & 1] * (float)(pos - key);
+                        if (key > pos || (key < first && key >= p.keep)) v = -INFINITY;
+                    }
+                    z[nt][e] = v;
+                    moves |= v > m[nt][e & 1] + (room + kLag);
+                }
+            if (__any_sync(0xffffffffu, moves)) {
+                float d = step;
+#pragma unroll
+                for (int x = 1; x < 32; x <<= 1) d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, x));
+                d_max = fmaxf(d_max, d);
+                const float less = room - headroom(d_max);
+                room -= less;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = fmaxf(z[nt][e], z[nt][e + 2]);
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                        const float to = fmaxf(m[nt][e] + less, mx - room), corr = to == -INFINITY ? 1.0f : fast_exp2(m[nt][e] - to);
+                        m[nt][e] = to;
+                        l[nt][e] *= corr;
+                        od[nt][e] *= corr;
+#pragma unroll
+                        for (int k = 0; k < 2 * NG; ++k) {
+                            o[nt][k][e] *= corr;
+                            o[nt][k][e + 2] *= corr;
+                        }
+                    }
+            }
+            uint32_t pb[NT][2];                // the weights as a right-hand operand: keys 2 c, 2 c + 1 (and + 8) of head r
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    z[nt][e] = fast_exp2(z[nt][e] - (m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1]));
+                    l[nt][e & 1] += z[nt][e];
+                }
+                pb[nt][0] = movmatrix_trans(pack_f16(z[nt][0], z[nt][1]));
+                pb[nt][1] = movmatrix_trans(pack_f16(z[nt][2], z[nt][3]));
+                mma_f16(od[nt], sd[0], 0u, sd[1], 0u, pb[nt][0], pb[nt][1]);
+            }
+            // -- values
+            uint32_t vw[2][NG];
+            lds_words<NG>(vw[0], at + kVCodes + (r * 4 + c) * 4 * NG);
+            lds_words<NG>(vw[1], at + kVCodes + 128 * NG + (r * 4 + c) * 4 * NG);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const uint32_t a[2][4] = {{centred_at<0>(vw[0][g]), centred_at<1>(vw[0][g]), centred_at<0>(vw[1][g]), centred_at<1>(vw[1][g])},
+                                          {centred_at<2>(vw[0][g]), centred_at<3>(vw[0][g]), centred_at<2>(vw[1][g]), centred_at<3>(vw[1][g])}};
+                const uint32_t d0 = __shfl_sync(0xffffffffu, sd[0], 8 * g + c), d1 = __shfl_sync(0xffffffffu, sd[1], 8 * g + c);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint32_t b0 = mul_f16x2(pb[nt][0], d0), b1 = mul_f16x2(pb[nt][1], d1);
+                    mma_f16(o[nt][2 * g], a[0][0], a[0][1], a[0][2], a[0][3], b0, b1);
+                    mma_f16(o[nt][2 * g + 1], a[1][0], a[1][1], a[1][2], a[1][3], b0, b1);
+                }
+            }
+        }
+        // -- the four warps' parts meet
+        __syncthreads();                 // (the last pair's have been read)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
+                float* to = meet + (warp * COLS + 8 * nt + 2 * c + e) * (D + 2);
+                if (r == 0) {
+                    to[D] = m[nt][e];
+                    to[D + 1] = l[nt][e];
+                }
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const float b = fmaf(8.0f, __shfl_sync(0xffffffffu, od[nt][e], 8 * g + c), __shfl_sync(0xffffffffu, od[nt][e], 8 * g + 4 + c));
+                    float* lanes = to + 32 * g + 4 * r;
+                    lanes[0] = o[nt][2 * g][e] + b;
+                    lanes[1] = o[nt][2 * g][e + 2] + b;
+                    lanes[2] = o[nt][2 * g + 1][e] + b;
+                    lanes[3] = o[nt][2 * g + 1][e + 2] + b;
+                }
+            }
+        __syncthreads();
+        const bool whole = take == here.n;
+        const int slot = 2 * blockIdx.x + (here.i > 0 ? 0 : 1);      // (a pair that began in an earlier block is this one's first)
+        float* part = p.part + (size_t)slot * COLS * (D + 2);
+        for (int x = threadIdx.x; x < nh * D; x += 32 * kStreamWarps) {
+            const int h = x / D, d = x % D;
+            float mx = -INFINITY, sum = 0.0f, out = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kStreamWarps; ++w) mx = fmaxf(mx, meet[(w * COLS + h) * (D + 2) + D]);
+#pragma unroll
+            for (int w = 0; w < kStreamWarps; ++w) {
+                const float* from = meet + (w * COLS + h) * (D + 2);
+                const float f = from[D] == -INFINITY ? 0.0f : exp2f(from[D] - mx);
+                sum = fmaf(from[D + 1], f, sum);
+                out = fmaf(from[d], f, out);
+            }
+            if (whole) {
+                const float f = closing_factor(p, t, h0 + h, mx / kLog2e, sum);
+                reinterpret_cast<__nv_bfloat16*>(p.out)[((size_t)t * p.n_heads + h0 + h) * D + d] = __float2bfloat16_rn(out * f);
+            } else {
+                part[h * (D + 2) + d] = out;
+                if (d == 0) {
+                    part[h * (D + 2) + D] = mx;
+                    part[h * (D + 2) + D + 1] = sum;
+                }
+            }
+        }
+        done += take;
+        here.i += take;
+        if (here.i == here.n) here.next_pair(p, st);
+    }
+    cp_async_wait<0>();
+}
+
+// The parts of a pair that lies in several blocks, in the order of its keys.  grid = (n, pairs), 128 threads.
+__global__ void __launch_bounds__(128) stream_merge_kernel(const AttnQ4 p, const Stream st, int cols) {
+    const int t = blockIdx.x, y = blockIdx.y, lane = threadIdx.x & 31;
+    const int n = pages_of(p, t);
+    if (n == 0) return;
+    const Row row = row_of(p, st, lane);
+    int before = 0;
+    for (int i = lane; i < t; i += 32) before += pages_of(p, i);
+    long at = before;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) at += __shfl_xor_sync(0xffffffffu, at, o);
+    at = at * st.pairs + (long)y * n;
+    const int b0 = row.block_of(at), b1 = row.block_of(at + n - 1);
+    if (b0 == b1) return;                // that block has finished it
+    const int kvh = y / st.chunks, h0 = kvh * (p.n_heads / p.n_kv) + y % st.chunks * st.heads;
+    const int nh = min(st.heads, (kvh + 1) * (p.n_heads / p.n_kv) - h0), D = p.D;
+    for (int x = threadIdx.x; x < nh * D; x += 128) {
+        const int h = x / D, d = x % D;
+        float mx = -INFINITY, sum = 0.0f, out = 0.0f;
+        for (int b = b0; b <= b1; ++b)
+            mx = fmaxf(mx, p.part[((size_t)(2 * b + (b == b0 ? 1 : 0)) * cols + h) * (D + 2) + D]);
+        for (int b = b0; b <= b1; ++b) {
+            const float* from = p.part + ((size_t)(2 * b + (b == b0 ? 1 : 0)) * cols + h) * (D + 2);
+            const float f = from[D] == -INFINITY ? 0.0f : exp2f(from[D] - mx);
+            sum = fmaf(from[D + 1], f, sum);
+            out = fmaf(from[d], f, out);
+        }
+        const float f = closing_factor(p, t, h0 + h, mx / kLog2e, sum);
+        reinterpret_cast<__nv_bfloat16*>(p.out)[((size_t)t * p.n_heads + h0 + h) * D + d] = __float2bfloat16_rn(out * f);
+    }
 }
 
 // Pages of a token's walk that split s takes: [first, end).
@@ -216,9 +763,54 @@ static bool sizes_ok(int n, int n_heads, int n_kv, int D) {
     return n >= 0 && n_heads > 0 && n_kv > 0 && n_heads % n_kv == 0 && D >= 32 && D <= 256 && D % 32 == 0;
 }
 
+// Whether the tensor-core kernel takes these sizes.
+static bool streams(int dt, int D) { return dt == DT_BF16 && D <= 128; }
+
+// Blocks of a token's pages' row, all of which run at once, and how the heads of a key/value head are dealt with.
+constexpr int kStreamMinPages = 4;
+static int stream_tiles(int n_heads, int n_kv) { return n_heads / n_kv > 8 ? 2 : 1; }
+static int stream_smem(int D, int tiles) {
+    return kStreamWarps * (kStreamStages * 20 * D + 8 * tiles * (D + 2) * (int)sizeof(float));
+}
+typedef void (*StreamKernel)(AttnQ4, Stream);
+static StreamKernel stream_kernel_of(int D, int tiles) {
+    switch (D / 32 * 2 + tiles - 1) {
+        case 2: return stream_kernel<1, 1>;
+        case 3: return stream_kernel<1, 2>;
+        case 4: return stream_kernel<2, 1>;
+        case 5: return stream_kernel<2, 2>;
+        case 6: return stream_kernel<3, 1>;
+        case 7: return stream_kernel<3, 2>;
+        case 8: return stream_kernel<4, 1>;
+        default: return stream_kernel<4, 2>;
+    }
+}
+// Blocks of one kernel that the current device runs at once (asked once for each).
+static int stream_blocks(int D, int tiles) {
+    static int known[64][10] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sm_count();
+    int& n = known[dev][D / 32 * 2 + tiles - 1];
+    if (n == 0) {
+        const StreamKernel k = stream_kernel_of(D, tiles);
+        int per = 0;
+        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, stream_smem(D, tiles)) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, k, 32 * kStreamWarps, stream_smem(D, tiles)) != cudaSuccess || per < 1) {
+            cudaGetLastError();
+            per = 1;
+        }
+        n = per * sm_count();
+    }
+    return n;
+}
+
 // Floats of scratch for a call of these sizes, `longest` the most keys that a token may see.
 extern "C" long nncpu_attention_q4_scratch(int n, int n_heads, int n_kv, int D, int dt, int longest) {
     if (n <= 0 || !sizes_ok(n, n_heads, n_kv, D)) return 0;
+    if (streams(dt, D)) {
+        const int tiles = stream_tiles(n_heads, n_kv);
+        return 2L * stream_blocks(D, tiles) * 8 * tiles * (D + 2);
+    }
     const int s = any_splits(n, n_heads, n_kv, longest);
     return s > 1 ? (long)n * n_heads * s * (D + 2) : 0;
 }
@@ -237,9 +829,21 @@ extern "C" int nncpu_attention_q4(const void* q, int dt, const uint8_t* k_pages,
     if (n == 0) return 0;
     AttnQ4 p{q, dt, k_pages, v_pages, n_pages, block_table, bt_stride, tok_seq, tok_pos, out, part, n, n_heads, n_kv, D, scale, window, keep,
              slope_base, sinks, cap, head_gate, gate_ld, any_splits(n, n_heads, n_kv, longest)};
-    const int group = n_heads / n_kv, chunks = (group + kAnyHeads - 1) / kAnyHeads;
+    const int group = n_heads / n_kv;
+    if (streams(dt, D)) {
+        NN_CHECK((uintptr_t)q % 16 == 0, "attention_q4: the queries do not start on a 16-byte boundary");
+        const int tiles = stream_tiles(n_heads, n_kv), chunks = (group + 8 * tiles - 1) / (8 * tiles);
+        NN_CHECK(n_kv <= 65535 / chunks, "attention_q4: %d key/value heads in %d parts", n_kv, chunks);
+        Stream st{(group + chunks - 1) / chunks, chunks, n_kv * chunks, kStreamMinPages, stream_blocks(D, tiles), scale * kLog2e, score_cap(scale, cap)};
+        stream_kernel_of(D, tiles)<<<st.blocks, 32 * kStreamWarps, stream_smem(D, tiles), stream>>>(p, st);
+        NN_LAUNCH_OK("attention_q4");
+        stream_merge_kernel<<<dim3((unsigned)n, (unsigned)st.pairs), 128, 0, stream>>>(p, st, 8 * tiles);
+        NN_LAUNCH_OK("attention_q4 (merge)");
+        return 0;
+    }
+    const int chunks = (group + kAnyHeads - 1) / kAnyHeads;
     const size_t smem = sizeof(float) * ((size_t)kPage * (D + 1) + (size_t)kAnyHeads * (D + kPage + 3));
-    NN_CHECK((long)n * p.n_splits < (1L << 31) && n_kv * chunks <= 65535 && n_heads <= 65535, "attention_q4: %d tokens in %d splits", n, p.n_splits);
+    NN_CHECK((long)n * p.n_splits < (1L << 31) && n_kv <= 65535 / chunks && n_heads <= 65535, "attention_q4: %d tokens in %d splits", n, p.n_splits);
     static bool done[64];
     if (first_use_on_this_device(done)) {
         const cudaError_t e = cudaFuncSetAttribute(any_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
