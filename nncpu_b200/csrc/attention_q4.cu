@@ -70,17 +70,18 @@ __device__ __forceinline__ float closing_factor(const AttnQ4& p, int t, int h, f
 //     lie in float16's middle, and the reference moves when a weight passes 2^15 or a step passes what it allows.
 // Rounded below 32 bits are: a weight p, and p d, both to 11 bits.
 //
-// A warp of the block takes 16 of a page's 64 keys: it brings their codes and scales (2.5 KB for D = 128) to its own ring in
-// shared memory by 16-byte cp.async and shares nothing with the other warps until a token's pages are done, when the four
-// parts meet in shared memory.
+// A block is two warps, each of which takes one half of every page: it brings its 32 keys' codes and scales (5 KB for D = 128) to its
+// own ring in shared memory by 16-byte cp.async and shares nothing with the other until a pair's pages are done, when
+// the first adds what the second leaves in shared memory.
 //
 // The pages of all (token, key/value head) pairs lie in one row, of which every block takes an equal share, wherever that
 // begins and ends: unequal sequences cost nothing, and there is one wave of blocks.  A pair that lies within one block is finished by it; of
 // the others every block leaves its part (its first and its last pair at most) in scratch for stream_merge_kernel.
 // ---------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kStreamWarps = 4;
-constexpr int kStreamStages = 4;            // pages of a warp's ring
+constexpr int kStreamWarps = 2;
+constexpr int kStreamStages = 3;            // pages of a warp's ring
+constexpr int kTiles = 2;                   // tensor-core tiles of 16 keys that a warp has of a page
 
 struct Stream {
     int heads;              // query heads of a pair (a part of those that share a key/value head where these are many)
@@ -234,16 +235,16 @@ constexpr float kLag = 4.0f;
 __device__ __forceinline__ float headroom(float d_max) { return d_max <= 1.0f ? 11.0f : 11.0f - ceilf(log2f(d_max)); }
 
 template <int NG, int NT>
-__global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 3 : 2) stream_kernel(const AttnQ4 p, const Stream st) {
+__global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_kernel(const AttnQ4 p, const Stream st) {
     constexpr int D = 32 * NG, COLS = 8 * NT;
-    constexpr int kCodes = 256 * NG, kScales = 64 * NG;          // bytes of a warp's 16 keys
-    constexpr int kVCodes = kCodes, kKScales = 2 * kCodes, kVScales = 2 * kCodes + kScales, kStage = 2 * (kCodes + kScales);   // a ring's stage
+    constexpr int kCodes = 256 * NG, kScales = 64 * NG;          // bytes of a tile's 16 keys
+    constexpr int kVCodes = kTiles * kCodes, kKScales = 2 * kVCodes, kVScales = kKScales + kTiles * kScales, kStage = 2 * kTiles * (kCodes + kScales);
     constexpr unsigned kPageBytes = 40 * D;
     extern __shared__ __align__(128) uint8_t stream_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     uint8_t* ring = stream_smem + warp * kStreamStages * kStage;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-    float* meet = reinterpret_cast<float*>(stream_smem + kStreamWarps * kStreamStages * kStage);   // [warps][COLS][D + 2]
+    float* meet = reinterpret_cast<float*>(stream_smem + kStreamWarps * kStreamStages * kStage);   // [COLS][D + 4]: lanes, reference, sum
 
     // rows of no sequence are zeros
     for (int t = blockIdx.x; t < p.n; t += gridDim.x)
@@ -257,47 +258,49 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 3 : 2) stream_ker
     Place here = place_of(p, st, first_page, lane), ahead = here;
     int fetched = 0;
     unsigned there = 0;                     // bit s: stage s holds a page (and not one that is missing)
-    int ids = -1, ids_left = 0;             // the next ids_left pages of the pair that is being fetched: lane l holds the id of the l-th
-    const uint8_t *k_at = nullptr, *v_at = nullptr, *s_at = nullptr;   // this lane's first 16 bytes of a page: keys, values, scales
+    int ids = -1, id_at = 0, id_end = 0;    // lane l holds the page l of the next 32 of the pair that is being fetched; the next one, and how many
+    const uint8_t *kc = nullptr, *vc = nullptr, *ks = nullptr, *vs = nullptr;   // this lane's first 16 bytes of a page: codes and scales
     const unsigned stride = (unsigned)p.n_kv * kPageBytes;
 
     // asks for this warp's keys of the next page (nothing for a page that is not there)
     auto fetch = [&](int stage) {
         if (fetched < n_mine) {
-            if (ids_left == 0) {
+            if (id_at == id_end) {
                 const int pos = p.tok_pos[ahead.t];
                 const PageWalk walk(first_visible_key(pos, p.window), pos, p.keep);
-                ids_left = min(32, ahead.n - ahead.i);
+                id_at = 0;
+                id_end = min(32, ahead.n - ahead.i);
                 const int pi = walk.page(min(ahead.i + lane, ahead.n - 1));
                 ids = pi < p.bt_stride ? p.block_table[(size_t)p.tok_seq[ahead.t] * p.bt_stride + pi] : -1;
                 if (ids >= p.n_pages) ids = -1;
-                const size_t head = (size_t)(ahead.y / st.chunks) * kPageBytes;
-                k_at = p.k_pages + head + warp * kCodes + lane * 16;
-                v_at = p.v_pages + head + warp * kCodes + lane * 16;
-                s_at = (lane < 4 * NG ? p.k_pages : p.v_pages) + head + 32 * D + warp * kScales + (lane < 4 * NG ? lane : lane - 4 * NG) * 16;
+                const size_t head = (size_t)(ahead.y / st.chunks) * kPageBytes + lane * 16;
+                kc = p.k_pages + head + warp * kTiles * kCodes;
+                vc = p.v_pages + head + warp * kTiles * kCodes;
+                ks = p.k_pages + head + 32 * D + warp * kTiles * kScales;
+                vs = p.v_pages + head + 32 * D + warp * kTiles * kScales;
             }
-            const int id = __shfl_sync(0xffffffffu, ids, 0);
-            ids = __shfl_down_sync(0xffffffffu, ids, 1);
+            const int id = __shfl_sync(0xffffffffu, ids, id_at++);
             if (id >= 0) {
                 there |= 1u << stage;
                 const size_t at = (size_t)(unsigned)id * stride;
                 const uint32_t dst = ring_at + stage * kStage + lane * 16;
 #pragma unroll
-                for (int k = 0; k < (16 * NG + 31) / 32; ++k)
-                    if (16 * NG % 32 == 0 || k * 32 + lane < 16 * NG) {
-                        cp_async16(dst + k * 512, k_at + at + k * 512);
-                        cp_async16(dst + kVCodes + k * 512, v_at + at + k * 512);
-                    }
-                if (NG == 4 || lane < 8 * NG) cp_async16(dst + kKScales, s_at + at);
+                for (int k = 0; k < kTiles * NG / 2; ++k) cp_async16(dst + k * 512, kc + at + k * 512);
+#pragma unroll
+                for (int k = 0; k < kTiles * NG / 2; ++k) cp_async16(dst + kVCodes + k * 512, vc + at + k * 512);
+                if (NG == 4 || lane < 8 * NG) {
+                    cp_async16(dst + kKScales, ks + at);
+                    cp_async16(dst + kVScales, vs + at);
+                }
             } else {
                 there &= ~(1u << stage);
             }
             ++fetched;
-            --ids_left;
             if (++ahead.i == ahead.n) ahead.next_pair(p, st);
         }
         cp_async_commit();
     };
+    static_assert(kTiles == 2, "a tile's copies are counted in whole rounds of a warp");
 #pragma unroll
     for (int s = 0; s < kStreamStages - 1; ++s) fetch(s);
 
@@ -329,9 +332,9 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 3 : 2) stream_ker
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // 2^e with top < 2^e (from the exponent's bits; of zeros and the smallest numbers 2^-100)
-            const int e = max((int)(__float_as_uint(top) >> 23), 27) - 126;
-            const float down = __int_as_float((127 - min(e, 126)) << 23), up = __int_as_float((127 + min(e, 126)) << 23);
+            // 2^e with top < 2^e (from the exponent's bits; of zeros and the smallest numbers 2^-99)
+            const int e = min(max((int)(__float_as_uint(top) >> 23), 27) - 126, 126);
+            const float down = __int_as_float((127 - e) << 23), up = __int_as_float((127 + e) << 23);
             float qs = 0.0f, off = 0.0f;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
@@ -361,101 +364,122 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 3 : 2) stream_ker
             col[nt][0] = __shfl_sync(0xffffffffu, by, 8 * c);
             col[nt][1] = __shfl_sync(0xffffffffu, by, 8 * c + 4);
         }
-        float slope2[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) slope2[nt][e] = p.slope_base != 0.0f ? slope_of(p, h0 + 8 * nt + 2 * c + e) * kLog2e : 0.0f;
         float o[NT][2 * NG][4];
-        float od[NT][4];               // row r: sum of p d (r even) or p m (r odd) of group r / 2, heads 2 c and 2 c + 1
-        float m[NT][2], l[NT][2];      // reference and sum of the weights
+        // row r: sum of p d (r even) or p m (r odd) of group r / 2; row 8: of p; heads 2 c and 2 c + 1
+        float od[NT][4];
+        float m[NT][2];                       // the weights' reference (0 until a key has been seen)
         float d_max = 1.0f, room = 11.0f;     // greatest step that the references leave room for, and how much that is
+        bool fresh = true;                    // no key has been seen
+        const uint32_t ones = r == 0 ? 0x3C003C00u : 0u;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int k = 0; k < 2 * NG; ++k) o[nt][k][0] = o[nt][k][1] = o[nt][k][2] = o[nt][k][3] = 0.0f;
             od[nt][0] = od[nt][1] = od[nt][2] = od[nt][3] = 0.0f;
-            m[nt][0] = m[nt][1] = -INFINITY;
-            l[nt][0] = l[nt][1] = 0.0f;
+            m[nt][0] = m[nt][1] = 0.0f;
         }
+        int pi = walk.page(here.i);
         for (int i = 0; i < take; ++i) {
             cp_async_wait<kStreamStages - 2>();
             __syncwarp();
             uint8_t* at = ring + stage * kStage;
             const bool missing = (there >> stage & 1) == 0;
-            fetch((stage + kStreamStages - 1) % kStreamStages);
-            stage = (stage + 1) % kStreamStages;
-            const int key0 = walk.page(here.i + i) * kPage + 16 * warp;
-            if (missing || key0 > pos || (key0 + 15 < first && key0 >= p.keep)) continue;      // none of these keys is seen
-            const bool full = key0 >= first && key0 + 15 <= pos;
+            fetch(stage == 0 ? kStreamStages - 1 : stage - 1);
+            stage = stage == kStreamStages - 1 ? 0 : stage + 1;
+            const int key0 = pi * kPage + 16 * kTiles * warp;
+            pi = here.i + i + 1 == walk.n_kept ? walk.lo : pi + 1;
+            if (missing || key0 > pos || (key0 + 16 * kTiles - 1 < first && key0 >= p.keep)) continue;      // none of these keys is seen
+            const bool full = key0 >= first && key0 + 16 * kTiles - 1 <= pos;
             if (!full) {
                 // what is not seen may hold anything, NaN too: its weight will be zero, and so must its numbers be
                 const int key = key0 + lane;
-                if (lane < 16 && (key > pos || (key < first && key >= p.keep)))
+                if (key > pos || (key < first && key >= p.keep))
 #pragma unroll
                     for (int g = 0; g < NG; ++g) *reinterpret_cast<uint32_t*>(at + kVScales + lane * 4 * NG + g * 4) = 0;
                 __syncwarp();
             }
             // -- scores
-            uint32_t kw[2][NG], ks[2][NG];
-            lds_words<NG>(kw[0], at + r * 16 * NG + c * 4 * NG);
-            lds_words<NG>(kw[1], at + (r + 8) * 16 * NG + c * 4 * NG);
-            lds_words<NG>(ks[0], at + kKScales + r * 4 * NG);
-            lds_words<NG>(ks[1], at + kKScales + (r + 8) * 4 * NG);
-            uint32_t dm[2] = {0, 0};
-            if (NG == 4 || c < NG) {
-                dm[0] = *reinterpret_cast<const uint32_t*>(at + kKScales + r * 4 * NG + c * 4);
-                dm[1] = *reinterpret_cast<const uint32_t*>(at + kKScales + (r + 8) * 4 * NG + c * 4);
-            }
-            // row r of the values' (d, m): those of keys 2 c, 2 c + 1 and of 2 c + 8, 2 c + 9
-            uint32_t sd[2] = {0, 0};
-            if constexpr (NG == 4) {
-                ldmatrix_x2_trans(sd[0], sd[1], (uint32_t)__cvta_generic_to_shared(at) + kVScales + (lane & 15) * 16);
-            } else if (r < 2 * NG) {
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(at + kVScales) + 4 * c * NG + r;
-                sd[0] = h[0] | (uint32_t)h[2 * NG] << 16;
-                sd[1] = h[16 * NG] | (uint32_t)h[18 * NG] << 16;
-            }
-            float z[NT][4];
+            float z[kTiles][NT][4];
+            uint32_t sd[kTiles][2];
+            float step = 0.0f;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0.0f;
-                mma_f16(z[nt], dm[0], dm[1], dm[0], dm[1], qhi[nt], qlo[nt]);
-            }
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const uint32_t a[2][4] = {{codes_at<0>(kw[0][g]), codes_at<0>(kw[1][g]), codes_at<1>(kw[0][g]), codes_at<1>(kw[1][g])},
-                                          {codes_at<2>(kw[0][g]), codes_at<2>(kw[1][g]), codes_at<3>(kw[0][g]), codes_at<3>(kw[1][g])}};
-                const float d0 = low_half(ks[0][g]), d1 = low_half(ks[1][g]);
+            for (int kt = 0; kt < kTiles; ++kt) {
+                const uint8_t* kcode = at + kt * kCodes + r * 16 * NG + c * 4 * NG;
+                const uint8_t* kscale = at + kKScales + kt * kScales + r * 4 * NG;
+                uint32_t kw[2][NG], kd[2][NG], dm[2] = {0, 0};
+                lds_words<NG>(kw[0], kcode);
+                lds_words<NG>(kw[1], kcode + 128 * NG);
+                lds_words<NG>(kd[0], kscale);
+                lds_words<NG>(kd[1], kscale + 32 * NG);
+                if (NG == 4 || c < NG) {
+                    dm[0] = *reinterpret_cast<const uint32_t*>(kscale + c * 4);
+                    dm[1] = *reinterpret_cast<const uint32_t*>(kscale + 32 * NG + c * 4);
+                }
+                // row r of the values' (d, m): those of keys 2 c, 2 c + 1 and of 2 c + 8, 2 c + 9
+                if constexpr (NG == 4) {
+                    ldmatrix_x2_trans(sd[kt][0], sd[kt][1], (uint32_t)__cvta_generic_to_shared(at) + kVScales + kt * kScales + (lane & 15) * 16);
+                } else {
+                    sd[kt][0] = sd[kt][1] = 0;
+                    if (r < 2 * NG) {
+                        const uint16_t* h = reinterpret_cast<const uint16_t*>(at + kVScales + kt * kScales) + 4 * c * NG + r;
+                        sd[kt][0] = h[0] | (uint32_t)h[2 * NG] << 16;
+                        sd[kt][1] = h[16 * NG] | (uint32_t)h[18 * NG] << 16;
+                    }
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_f16(acc, a[0][0], a[0][1], a[0][2], a[0][3], qb[nt][g][0], qb[nt][g][1]);
-                    mma_f16(acc, a[1][0], a[1][1], a[1][2], a[1][3], qb[nt][g][2], qb[nt][g][3]);
-                    z[nt][0] = fmaf(acc[0], d0, z[nt][0]);
-                    z[nt][1] = fmaf(acc[1], d0, z[nt][1]);
-                    z[nt][2] = fmaf(acc[2], d1, z[nt][2]);
-                    z[nt][3] = fmaf(acc[3], d1, z[nt][3]);
+                    z[kt][nt][0] = z[kt][nt][1] = z[kt][nt][2] = z[kt][nt][3] = 0.0f;
+                    mma_f16(z[kt][nt], dm[0], dm[1], dm[0], dm[1], qhi[nt], qlo[nt]);
                 }
-            }
-            // -- weights
-            const float2 steps = __half22float2(__hmax2(*reinterpret_cast<const __half2*>(&sd[0]), *reinterpret_cast<const __half2*>(&sd[1])));
-            const float step = (r & 1) == 0 ? fmaxf(steps.x, steps.y) : 0.0f;
-            bool moves = step > d_max;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+                for (int g = 0; g < NG; ++g) {
+                    const uint32_t a[2][4] = {{codes_at<0>(kw[0][g]), codes_at<0>(kw[1][g]), codes_at<1>(kw[0][g]), codes_at<1>(kw[1][g])},
+                                              {codes_at<2>(kw[0][g]), codes_at<2>(kw[1][g]), codes_at<3>(kw[0][g]), codes_at<3>(kw[1][g])}};
+                    const float d0 = low_half(kd[0][g]), d1 = low_half(kd[1][g]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = z[nt][e] * col[nt][e & 1];
-                    if (st.cap.out > 0.0f) v = capped_score(v, st.cap);
-                    if (!full || p.slope_base != 0.0f) {
-                        const int key = key0 + r + 8 * (e >> 1);
-                        v -= slope2[nt][e & 1] * (float)(pos - key);
-                        if (key > pos || (key < first && key >= p.keep)) v = -INFINITY;
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma_f16(acc, a[0][0], a[0][1], a[0][2], a[0][3], qb[nt][g][0], qb[nt][g][1]);
+                        mma_f16(acc, a[1][0], a[1][1], a[1][2], a[1][3], qb[nt][g][2], qb[nt][g][3]);
+                        z[kt][nt][0] = fmaf(acc[0], d0, z[kt][nt][0]);
+                        z[kt][nt][1] = fmaf(acc[1], d0, z[kt][nt][1]);
+                        z[kt][nt][2] = fmaf(acc[2], d1, z[kt][nt][2]);
+                        z[kt][nt][3] = fmaf(acc[3], d1, z[kt][nt][3]);
                     }
-                    z[nt][e] = v;
-                    moves |= v > m[nt][e & 1] + (room + kLag);
                 }
+                const float2 f = __half22float2(__hmax2(*reinterpret_cast<const __half2*>(&sd[kt][0]), *reinterpret_cast<const __half2*>(&sd[kt][1])));
+                step = fmaxf(step, fmaxf(f.x, f.y));
+            }
+            if (r & 1) step = 0.0f;
+            // -- weights: first what 2 is raised to
+            bool moves = fresh | (step > d_max);
+            if (full && p.slope_base == 0.0f && st.cap.out == 0.0f) {
+#pragma unroll
+                for (int kt = 0; kt < kTiles; ++kt)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            z[kt][nt][e] = fmaf(z[kt][nt][e], col[nt][e & 1], 0.0f - m[nt][e & 1]);
+                            moves |= z[kt][nt][e] > room + kLag;
+                        }
+            } else {
+#pragma unroll
+                for (int kt = 0; kt < kTiles; ++kt)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = key0 + 16 * kt + r + 8 * (e >> 1);
+                            float v = z[kt][nt][e] * col[nt][e & 1];
+                            if (st.cap.out > 0.0f) v = capped_score(v, st.cap);
+                            if (p.slope_base != 0.0f) v -= slope_of(p, h0 + 8 * nt + 2 * c + (e & 1)) * kLog2e * (float)(pos - key);
+                            v -= m[nt][e & 1];
+                            if (key > pos || (key < first && key >= p.keep)) v = -INFINITY;
+                            z[kt][nt][e] = v;
+                            moves |= v > room + kLag;
+                        }
+            }
             if (__any_sync(0xffffffffu, moves)) {
                 float d = step;
 #pragma unroll
@@ -467,98 +491,113 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 3 : 2) stream_ker
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float mx = fmaxf(z[nt][e], z[nt][e + 2]);
+                        float mx = -INFINITY;
+#pragma unroll
+                        for (int kt = 0; kt < kTiles; ++kt) mx = fmaxf(mx, fmaxf(z[kt][nt][e], z[kt][nt][e + 2]));
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                        const float to = fmaxf(m[nt][e] + less, mx - room), corr = to == -INFINITY ? 1.0f : fast_exp2(m[nt][e] - to);
-                        m[nt][e] = to;
-                        l[nt][e] *= corr;
+                        // by how much the reference rises (the first time it may fall)
+                        float rise = fresh ? mx - room : fmaxf(less, mx - room);
+                        if (mx == -INFINITY) rise = fresh ? 0.0f : less;
+                        const float corr = fresh ? 1.0f : fast_exp2(0.0f - rise);
+                        m[nt][e] += rise;
                         od[nt][e] *= corr;
+                        od[nt][e + 2] *= corr;
+#pragma unroll
+                        for (int kt = 0; kt < kTiles; ++kt) {
+                            z[kt][nt][e] -= rise;
+                            z[kt][nt][e + 2] -= rise;
+                        }
 #pragma unroll
                         for (int k = 0; k < 2 * NG; ++k) {
                             o[nt][k][e] *= corr;
                             o[nt][k][e + 2] *= corr;
                         }
                     }
-            }
-            uint32_t pb[NT][2];                // the weights as a right-hand operand: keys 2 c, 2 c + 1 (and + 8) of head r
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    z[nt][e] = fast_exp2(z[nt][e] - (m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1]));
-                    l[nt][e & 1] += z[nt][e];
-                }
-                pb[nt][0] = movmatrix_trans(pack_f16(z[nt][0], z[nt][1]));
-                pb[nt][1] = movmatrix_trans(pack_f16(z[nt][2], z[nt][3]));
-                mma_f16(od[nt], sd[0], 0u, sd[1], 0u, pb[nt][0], pb[nt][1]);
+                fresh = false;
             }
             // -- values
-            uint32_t vw[2][NG];
-            lds_words<NG>(vw[0], at + kVCodes + (r * 4 + c) * 4 * NG);
-            lds_words<NG>(vw[1], at + kVCodes + 128 * NG + (r * 4 + c) * 4 * NG);
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const uint32_t a[2][4] = {{centred_at<0>(vw[0][g]), centred_at<1>(vw[0][g]), centred_at<0>(vw[1][g]), centred_at<1>(vw[1][g])},
-                                          {centred_at<2>(vw[0][g]), centred_at<3>(vw[0][g]), centred_at<2>(vw[1][g]), centred_at<3>(vw[1][g])}};
-                const uint32_t d0 = __shfl_sync(0xffffffffu, sd[0], 8 * g + c), d1 = __shfl_sync(0xffffffffu, sd[1], 8 * g + c);
+            for (int kt = 0; kt < kTiles; ++kt) {
+                uint32_t pb[NT][2];            // the weights as a right-hand operand: keys 2 c, 2 c + 1 (and + 8) of head r
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const uint32_t b0 = mul_f16x2(pb[nt][0], d0), b1 = mul_f16x2(pb[nt][1], d1);
-                    mma_f16(o[nt][2 * g], a[0][0], a[0][1], a[0][2], a[0][3], b0, b1);
-                    mma_f16(o[nt][2 * g + 1], a[1][0], a[1][1], a[1][2], a[1][3], b0, b1);
+                    pb[nt][0] = movmatrix_trans(pack_f16(fast_exp2(z[kt][nt][0]), fast_exp2(z[kt][nt][1])));
+                    pb[nt][1] = movmatrix_trans(pack_f16(fast_exp2(z[kt][nt][2]), fast_exp2(z[kt][nt][3])));
+                    mma_f16(od[nt], sd[kt][0], ones, sd[kt][1], ones, pb[nt][0], pb[nt][1]);
+                }
+                const uint8_t* vcode = at + kVCodes + kt * kCodes + (r * 4 + c) * 4 * NG;
+                uint32_t vw[2][NG];
+                lds_words<NG>(vw[0], vcode);
+                lds_words<NG>(vw[1], vcode + 128 * NG);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const uint32_t a[2][4] = {{centred_at<0>(vw[0][g]), centred_at<1>(vw[0][g]), centred_at<0>(vw[1][g]), centred_at<1>(vw[1][g])},
+                                              {centred_at<2>(vw[0][g]), centred_at<3>(vw[0][g]), centred_at<2>(vw[1][g]), centred_at<3>(vw[1][g])}};
+                    const uint32_t d0 = __shfl_sync(0xffffffffu, sd[kt][0], 8 * g + c), d1 = __shfl_sync(0xffffffffu, sd[kt][1], 8 * g + c);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint32_t b0 = mul_f16x2(pb[nt][0], d0), b1 = mul_f16x2(pb[nt][1], d1);
+                        mma_f16(o[nt][2 * g], a[0][0], a[0][1], a[0][2], a[0][3], b0, b1);
+                        mma_f16(o[nt][2 * g + 1], a[1][0], a[1][1], a[1][2], a[1][3], b0, b1);
+                    }
                 }
             }
         }
-        // -- the four warps' parts meet
-        __syncthreads();                 // (the last pair's have been read)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
-                float* to = meet + (warp * COLS + 8 * nt + 2 * c + e) * (D + 2);
-                if (r == 0) {
-                    to[D] = m[nt][e];
-                    to[D + 1] = l[nt][e];
-                }
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const float b = fmaf(8.0f, __shfl_sync(0xffffffffu, od[nt][e], 8 * g + c), __shfl_sync(0xffffffffu, od[nt][e], 8 * g + 4 + c));
-                    float* lanes = to + 32 * g + 4 * r;
-                    lanes[0] = o[nt][2 * g][e] + b;
-                    lanes[1] = o[nt][2 * g][e + 2] + b;
-                    lanes[2] = o[nt][2 * g + 1][e] + b;
-                    lanes[3] = o[nt][2 * g + 1][e + 2] + b;
-                }
-            }
-        __syncthreads();
+        // -- the warps' parts meet: thread (r, c) holds lanes 32 g + 4 r to + 3 of heads 2 c and 2 c + 1
+        __syncthreads();                 // (the last pair's part has been read)
         const bool whole = take == here.n;
         const int slot = 2 * blockIdx.x + (here.i > 0 ? 0 : 1);      // (a pair that began in an earlier block is this one's first)
-        float* part = p.part + (size_t)slot * COLS * (D + 2);
-        for (int x = threadIdx.x; x < nh * D; x += 32 * kStreamWarps) {
-            const int h = x / D, d = x % D;
-            float mx = -INFINITY, sum = 0.0f, out = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kStreamWarps; ++w) mx = fmaxf(mx, meet[(w * COLS + h) * (D + 2) + D]);
+        for (int pass = 0; pass < 2; ++pass) {
+            if (pass == 1) __syncthreads();
+            if (warp == 1 - pass)
 #pragma unroll
-            for (int w = 0; w < kStreamWarps; ++w) {
-                const float* from = meet + (w * COLS + h) * (D + 2);
-                const float f = from[D] == -INFINITY ? 0.0f : exp2f(from[D] - mx);
-                sum = fmaf(from[D + 1], f, sum);
-                out = fmaf(from[d], f, out);
-            }
-            if (whole) {
-                const float f = closing_factor(p, t, h0 + h, mx / kLog2e, sum);
-                reinterpret_cast<__nv_bfloat16*>(p.out)[((size_t)t * p.n_heads + h0 + h) * D + d] = __float2bfloat16_rn(out * f);
-            } else {
-                part[h * (D + 2) + d] = out;
-                if (d == 0) {
-                    part[h * (D + 2) + D] = mx;
-                    part[h * (D + 2) + D + 1] = sum;
-                }
-            }
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int h = 8 * nt + 2 * c + e;
+                        float* other = meet + h * (D + 4);
+                        const float sum = __shfl_sync(0xffffffffu, od[nt][e + 2], c), ref = fresh ? -INFINITY : m[nt][e];
+                        float f0 = 1.0f, f1 = 0.0f, top = ref, total = sum;
+                        if (pass == 1) {
+                            top = fmaxf(ref, other[D]);
+                            f0 = ref == -INFINITY ? 0.0f : exp2f(ref - top);
+                            f1 = other[D] == -INFINITY ? 0.0f : exp2f(other[D] - top);
+                            total = fmaf(other[D + 1], f1, sum * f0);
+                            if (whole && h < nh) f0 *= closing_factor(p, t, h0 + h, top / kLog2e, total), f1 *= closing_factor(p, t, h0 + h, top / kLog2e, total);
+                        }
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) {
+                            const float b = fmaf(8.0f, __shfl_sync(0xffffffffu, od[nt][e], 8 * g + c), __shfl_sync(0xffffffffu, od[nt][e], 8 * g + 4 + c));
+                            const int d = 32 * g + 4 * r;
+                            float4 v = make_float4(o[nt][2 * g][e] + b, o[nt][2 * g][e + 2] + b, o[nt][2 * g + 1][e] + b, o[nt][2 * g + 1][e + 2] + b);
+                            if (pass == 0) {
+                                *reinterpret_cast<float4*>(other + d) = v;
+                                continue;
+                            }
+                            const float4 w = *reinterpret_cast<const float4*>(other + d);
+                            v = make_float4(fmaf(w.x, f1, v.x * f0), fmaf(w.y, f1, v.y * f0), fmaf(w.z, f1, v.z * f0), fmaf(w.w, f1, v.w * f0));
+                            if (h >= nh) continue;
+                            if (whole) {
+                                __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+                                uint2 packed = make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
+                                __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + ((size_t)t * p.n_heads + h0 + h) * D + d;
+                                *reinterpret_cast<uint2*>(out) = packed;
+                            } else {
+                                *reinterpret_cast<float4*>(p.part + ((size_t)slot * COLS + h) * (D + 4) + d) = v;
+                            }
+                        }
+                        if (r == 0 && pass == 0) {
+                            other[D] = top;
+                            other[D + 1] = total;
+                        }
+                        if (r == 0 && pass == 1 && !whole && h < nh) {
+                            float* part = p.part + ((size_t)slot * COLS + h) * (D + 4);
+                            part[D] = top;
+                            part[D + 1] = total;
+                        }
+                    }
         }
         done += take;
         here.i += take;
@@ -587,9 +626,9 @@ __global__ void __launch_bounds__(128) stream_merge_kernel(const AttnQ4 p, const
         const int h = x / D, d = x % D;
         float mx = -INFINITY, sum = 0.0f, out = 0.0f;
         for (int b = b0; b <= b1; ++b)
-            mx = fmaxf(mx, p.part[((size_t)(2 * b + (b == b0 ? 1 : 0)) * cols + h) * (D + 2) + D]);
+            mx = fmaxf(mx, p.part[((size_t)(2 * b + (b == b0 ? 1 : 0)) * cols + h) * (D + 4) + D]);
         for (int b = b0; b <= b1; ++b) {
-            const float* from = p.part + ((size_t)(2 * b + (b == b0 ? 1 : 0)) * cols + h) * (D + 2);
+            const float* from = p.part + ((size_t)(2 * b + (b == b0 ? 1 : 0)) * cols + h) * (D + 4);
             const float f = from[D] == -INFINITY ? 0.0f : exp2f(from[D] - mx);
             sum = fmaf(from[D + 1], f, sum);
             out = fmaf(from[d], f, out);
@@ -770,7 +809,7 @@ static bool streams(int dt, int D) { return dt == DT_BF16 && D <= 128; }
 constexpr int kStreamMinPages = 4;
 static int stream_tiles(int n_heads, int n_kv) { return n_heads / n_kv > 8 ? 2 : 1; }
 static int stream_smem(int D, int tiles) {
-    return kStreamWarps * (kStreamStages * 20 * D + 8 * tiles * (D + 2) * (int)sizeof(float));
+    return kStreamWarps * kStreamStages * 40 * D + 8 * tiles * (D + 4) * (int)sizeof(float);
 }
 typedef void (*StreamKernel)(AttnQ4, Stream);
 static StreamKernel stream_kernel_of(int D, int tiles) {
@@ -809,7 +848,7 @@ extern "C" long nncpu_attention_q4_scratch(int n, int n_heads, int n_kv, int D, 
     if (n <= 0 || !sizes_ok(n, n_heads, n_kv, D)) return 0;
     if (streams(dt, D)) {
         const int tiles = stream_tiles(n_heads, n_kv);
-        return 2L * stream_blocks(D, tiles) * 8 * tiles * (D + 2);
+        return 2L * stream_blocks(D, tiles) * 8 * tiles * (D + 4);
     }
     const int s = any_splits(n, n_heads, n_kv, longest);
     return s > 1 ? (long)n * n_heads * s * (D + 2) : 0;
@@ -831,7 +870,8 @@ extern "C" int nncpu_attention_q4(const void* q, int dt, const uint8_t* k_pages,
              slope_base, sinks, cap, head_gate, gate_ld, any_splits(n, n_heads, n_kv, longest)};
     const int group = n_heads / n_kv;
     if (streams(dt, D)) {
-        NN_CHECK((uintptr_t)q % 16 == 0, "attention_q4: the queries do not start on a 16-byte boundary");
+        NN_CHECK((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)part % 16 == 0,
+                 "attention_q4: bfloat16 queries, output and scratch start on 16-byte boundaries");
         const int tiles = stream_tiles(n_heads, n_kv), chunks = (group + 8 * tiles - 1) / (8 * tiles);
         NN_CHECK(n_kv <= 65535 / chunks, "attention_q4: %d key/value heads in %d parts", n_kv, chunks);
         Stream st{(group + chunks - 1) / chunks, chunks, n_kv * chunks, kStreamMinPages, stream_blocks(D, tiles), scale * kLog2e, score_cap(scale, cap)};
