@@ -36,6 +36,11 @@
 // row (crates/nncpu/src/model/forward.rs:141-160,383-426); softmax runs in 32-bit here
 // as there.
 //
+// Keys and values may be float16 instead (kHalf: a 4-bit cache's, taken out of its codes by cache_q4.cu; eight times finer than
+// bfloat16, and within float16's range by that cache's format).  Both operands of a product are of one type, so a row's thread then turns
+// its query into float16 in shared memory, times a power of two that makes its greatest lane at most 1, which is
+// exact for all but what is 2^-14 below that; the power of two goes into the factor of the row's scores.  The weights are float16 too.
+//
 // Every wait on an mbarrier is bounded in time; a wait that runs out sets
 // *status, the other roles run into their own limits, copies in flight are
 // waited for and the block frees its tensor memory on the common exit.
@@ -147,6 +152,45 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+    return d;
+}
+
+// A query row in its swizzled tile, bfloat16 to float16 in place (the order of its 16-byte pieces does not matter; the lanes
+// of a warp start at different ones, so that eight rows' pieces lie in eight groups of banks).  Returns 2^e, which the row was divided by.
+template <int kSlabs, int kSlabBytes>
+__device__ __forceinline__ float query_to_half(uint8_t* row) {
+    const int turn = threadIdx.x & 7;
+    float top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kSlabs; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint4 u = *reinterpret_cast<const uint4*>(row + s * kSlabBytes + ((j + turn) & 7) * 16);
+            const float2 a = two_bf16(u.x), b = two_bf16(u.y), c = two_bf16(u.z), d = two_bf16(u.w);
+            top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))),
+                                   fmaxf(fmaxf(fabsf(c.x), fabsf(c.y)), fmaxf(fabsf(d.x), fabsf(d.y)))));
+        }
+    // top < 2^e by the exponent's bits (of zeros and the smallest numbers 2^-99)
+    const int e = min(max((int)(__float_as_uint(top) >> 23), 27) - 126, 126);
+    const float down = __int_as_float((127 - e) << 23);
+#pragma unroll
+    for (int s = 0; s < kSlabs; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint4* at = reinterpret_cast<uint4*>(row + s * kSlabBytes + ((j + turn) & 7) * 16);
+            const uint4 u = *at;
+            const float2 a = two_bf16(u.x), b = two_bf16(u.y), c = two_bf16(u.z), d = two_bf16(u.w);
+            *at = make_uint4(pack_f16(a.x * down, a.y * down), pack_f16(b.x * down, b.y * down), pack_f16(c.x * down, c.y * down),
+                             pack_f16(d.x * down, d.y * down));
+        }
+    return __int_as_float((127 + e) << 23);
+}
+
+// Instruction descriptor of float16 inputs (bfloat16's has a bit for each operand's type).
+__host__ __device__ constexpr uint32_t instr_desc_16(bool half, int m, int n) { return instr_desc_bf16(m, n) & ~(half ? (1u << 7) | (1u << 10) : 0u); }
 
 // P . V with P taken from tensor memory (the A operand) and V from shared memory.
 __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b_desc, uint32_t idesc,
@@ -174,7 +218,7 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t local_addr, uint32_t ra
 }
 
 // Threads: warp 0 producer, warp 1 tensor-core issue and tensor memory, then one warpgroup per head.
-template <int HD, int VD, int kStreams, bool kCap>
+template <int HD, int VD, int kStreams, bool kCap, bool kHalf>
 __global__ void __launch_bounds__(64 + 128 * kStreams, 1)
 prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const AttnParams p) {
@@ -204,7 +248,8 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     uint64_t* s_full = v_empty + kStages;                     // [kStreams]
     uint64_t* p_full = s_full + kStreams;                     // [kStreams]
     uint64_t* o_done = p_full + kStreams;                     // [kStreams]
-    uint32_t* tmem_slot = (uint32_t*)(o_done + kStreams);
+    uint64_t* q_ready = o_done + kStreams;                    // (kHalf) the queries are float16
+    uint32_t* tmem_slot = (uint32_t*)(q_ready + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // Launched to start while the kernel before it ends (its set-up needs nothing of that kernel; the step's
@@ -250,6 +295,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
+        mbar_init(q_ready, 128 * n_streams);
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&k_full[s], 1);
             mbar_init(&v_full[s], 1);
@@ -330,9 +376,9 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
     } else if (warp == 1) {
         if (lane == 0 && n_steps > 0) {
-            constexpr uint32_t idesc_s128 = instr_desc_bf16(kQRows, 128), idesc_s64 = instr_desc_bf16(kQRows, 64);
-            constexpr uint32_t idesc_o = instr_desc_bf16(kQRows, VD) | (1u << 16);   // B (V) is MN-major
-            bool ok = mbar_wait(q_full, 0);
+            constexpr uint32_t idesc_s128 = instr_desc_16(kHalf, kQRows, 128), idesc_s64 = instr_desc_16(kHalf, kQRows, 64);
+            constexpr uint32_t idesc_o = instr_desc_16(kHalf, kQRows, VD) | (1u << 16);   // B (V) is MN-major
+            bool ok = mbar_wait(kHalf ? q_ready : q_full, 0);
             if (!ok) atomicExch(p.status, kTimeoutQ);
             // S_t(i) = Q_t . K(i)^T into the head's S columns; K(i) has landed
             auto issue_scores = [&](int t, int i) {
@@ -417,10 +463,22 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         const int lim_hi = valid ? pos0 + row : key_hi;
         const int lim_lo = first_visible_key(lim_hi, p.window);
         const uint32_t tmem_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(t * kStreamCols);
+        bool ok = t < n_streams && n_steps > 0;   // the second warpgroup of a block with one head has nothing to do
+        float up = 1.0f;                          // (kHalf) the tensor core's scores are those of the query over this
+        if (kHalf && ok) {
+            ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0));
+            if (!ok && lane == 0) atomicExch(p.status, kTimeoutQ);
+            if (ok) {
+                if (quarter * 32 < n_rows) up = query_to_half<kSlabs, kQSlab>(smem_q + t * kQBytes + row * 128);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(q_ready);
+            }
+        }
         // the distance bias in the unit of the unscaled scores (the scale is applied with the reference maximum)
         const float bias_per_key = p.slope_base != 0.0f
-            ? exp2f(-p.slope_base * (float)(h + 1) / (float)p.n_heads) * 1.4426950408889634f / p.scale2 : 0.0f;
-        bool ok = t < n_streams && n_steps > 0;   // the second warpgroup of a block with one head has nothing to do
+            ? exp2f(-p.slope_base * (float)(h + 1) / (float)p.n_heads) * 1.4426950408889634f / (kHalf ? p.scale2 * up : p.scale2) : 0.0f;
+        const float score_mul = kHalf && !kCap ? p.score_mul * up : p.score_mul;
+        const float cap_x = kHalf ? p.cap_x * up : p.cap_x, cap_in = kHalf ? p.cap_in * up : p.cap_in;
         for (int i = 0; ok && i < n_steps; ++i) {
             ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], i & 1));
             if (!ok) {
@@ -456,10 +514,10 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 #pragma unroll
                     for (int c = 0; c < 64; ++c) big[c & 3] = fmaxf(big[c & 3], fabsf(__uint_as_float(u[c])));
                     const float most = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
-                    if (__all_sync(0xffffffffu, most <= p.cap_small)) {
+                    if (__all_sync(0xffffffffu, (kHalf ? most * up : most) <= p.cap_small)) {
                         constexpr float kTanh[6] = {0.9999824762f, -0.3329640925f, 0.1310810596f, -0.0478774495f, 0.0132463686f,
                                                     -0.0018748625f};
-                        const uint64_t k = pair_of(p.cap_x, p.cap_x);
+                        const uint64_t k = pair_of(cap_x, cap_x);
 #pragma unroll
                         for (int c = 0; c < 64; c += 2) {
                             const uint64_t x = mul_pair(pair_of(__uint_as_float(u[c]), __uint_as_float(u[c + 1])), k);
@@ -473,7 +531,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                     } else {
 #pragma unroll
                         for (int c = 0; c < 64; ++c) {
-                            const float e = fast_exp2(__uint_as_float(u[c]) * p.cap_in);
+                            const float e = fast_exp2(__uint_as_float(u[c]) * cap_in);
                             u[c] = __float_as_uint(fmaf(-2.0f, fast_rcp(1.0f + e), 1.0f));
                         }
                     }
@@ -495,11 +553,11 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                         load_half(hf, u);
 #pragma unroll
                         for (int c = 0; c < 64; c += 2) {
-                            const float e0 = fast_exp2(fmaf(__uint_as_float(u[c]), p.score_mul, neg_m));
-                            const float e1 = fast_exp2(fmaf(__uint_as_float(u[c + 1]), p.score_mul, neg_m));
+                            const float e0 = fast_exp2(fmaf(__uint_as_float(u[c]), score_mul, neg_m));
+                            const float e1 = fast_exp2(fmaf(__uint_as_float(u[c + 1]), score_mul, neg_m));
                             sm[c & 3] += e0;
                             sm[(c & 3) + 1] += e1;
-                            w[hf][c >> 1] = pack_bf16(e0, e1);
+                            w[hf][c >> 1] = kHalf ? pack_f16(e0, e1) : pack_bf16(e0, e1);
                         }
                     }
                 }
@@ -518,7 +576,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                         for (int c = 0; c < 64; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(u[c]));
                     }
                 }
-                const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.score_mul;   // the factor is positive
+                const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * score_mul;   // the factor is positive
                 float alpha = 1.0f;
                 if (tmax > m_ref) {
                     alpha = fast_exp2(m_ref - tmax);    // 0 when nothing was seen yet
@@ -723,7 +781,7 @@ struct MapCache {
 
 MapCache g_maps;
 
-template <int HD, int VD, int kStreams, bool kCap>
+template <int HD, int VD, int kStreams, bool kCap, bool kHalf>
 int launch_one(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, AttnParams p, int n_tok, int longest,
                int* splits_only, cudaStream_t stream) {
     // (splits_only: receives the number of blocks that would share a tile, and nothing is launched)
@@ -733,7 +791,7 @@ int launch_one(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& 
     constexpr int smem = (int)tmem_block_bytes(kStreams * kQRows * HD * 2 + kStages * kKeys * (HD + VD) * 2 + 256 + 1024, kStreams * kStreamCols);
     static bool configured[64] = {};
     if (first_use_on_this_device(configured)) {
-        const cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<HD, VD, kStreams, kCap>,
+        const cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<HD, VD, kStreams, kCap, kHalf>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         NN_CHECK(e == cudaSuccess, "attention (tensor cores): %d bytes of shared memory refused: %s", smem,
                  cudaGetErrorString(e));
@@ -768,7 +826,7 @@ int launch_one(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& 
             if (fit[dev][i] == 0) {
                 with_splits(n);
                 int clusters = 0;
-                if (cudaOccupancyMaxActiveClusters(&clusters, prefill_tc_kernel<HD, VD, kStreams, kCap>, &cfg) != cudaSuccess) {
+                if (cudaOccupancyMaxActiveClusters(&clusters, prefill_tc_kernel<HD, VD, kStreams, kCap, kHalf>, &cfg) != cudaSuccess) {
                     cudaGetLastError();
                     clusters = 0;
                 }
@@ -783,28 +841,31 @@ int launch_one(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& 
     }
     with_splits(1 << p.split_shift);
     cfg.numAttrs += overlap_attribute(attr + 1);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, prefill_tc_kernel<HD, VD, kStreams, kCap>, mq, mk, mv, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, prefill_tc_kernel<HD, VD, kStreams, kCap, kHalf>, mq, mk, mv, p);
     NN_CHECK(e == cudaSuccess, "attention prefill (tensor cores): launch failed: %s", cudaGetErrorString(e));
     return 0;
 }
 
-template <int HD, int VD>
+template <int HD, int VD, bool kHalf>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttnParams& p, int n_tok, int longest,
            int* splits_only, cudaStream_t stream) {
     // two heads to a block where a key/value head has two to give; one head per block otherwise
     const bool cap = p.cap_in != 0.0f;
     if (p.n_heads == p.n_kv)
-        return cap ? launch_one<HD, VD, 1, true>(mq, mk, mv, p, n_tok, longest, splits_only, stream)
-                   : launch_one<HD, VD, 1, false>(mq, mk, mv, p, n_tok, longest, splits_only, stream);
-    return cap ? launch_one<HD, VD, 2, true>(mq, mk, mv, p, n_tok, longest, splits_only, stream)
-               : launch_one<HD, VD, 2, false>(mq, mk, mv, p, n_tok, longest, splits_only, stream);
+        return cap ? launch_one<HD, VD, 1, true, kHalf>(mq, mk, mv, p, n_tok, longest, splits_only, stream)
+                   : launch_one<HD, VD, 1, false, kHalf>(mq, mk, mv, p, n_tok, longest, splits_only, stream);
+    return cap ? launch_one<HD, VD, 2, true, kHalf>(mq, mk, mv, p, n_tok, longest, splits_only, stream)
+               : launch_one<HD, VD, 2, false, kHalf>(mq, mk, mv, p, n_tok, longest, splits_only, stream);
 }
 
 int launch_any(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttnParams& p, int head_dim, int vp,
-               int n_tok, int longest, int* splits_only, cudaStream_t stream) {
-    if (head_dim == 64) return launch<64, 64>(mq, mk, mv, p, n_tok, longest, splits_only, stream);
-    if (vp == 64) return launch<128, 64>(mq, mk, mv, p, n_tok, longest, splits_only, stream);
-    return launch<128, 128>(mq, mk, mv, p, n_tok, longest, splits_only, stream);
+               bool half, int n_tok, int longest, int* splits_only, cudaStream_t stream) {
+    if (half)
+        return head_dim == 64 ? launch<64, 64, true>(mq, mk, mv, p, n_tok, longest, splits_only, stream)
+                              : launch<128, 128, true>(mq, mk, mv, p, n_tok, longest, splits_only, stream);
+    if (head_dim == 64) return launch<64, 64, false>(mq, mk, mv, p, n_tok, longest, splits_only, stream);
+    if (vp == 64) return launch<128, 64, false>(mq, mk, mv, p, n_tok, longest, splits_only, stream);
+    return launch<128, 128, false>(mq, mk, mv, p, n_tok, longest, splits_only, stream);
 }
 
 }  // namespace
@@ -820,12 +881,11 @@ extern "C" int nncpu_attention_prefill_tc_supported(int n_heads, int n_kv, int h
 // together with a distance bias); head_gate (or null): token t's n_heads logits at t * gate_ld, whose sigmoids multiply the
 // heads' outputs; longest: at least as many keys as any row sees (a tile may be split over its steps, see the head of this
 // file; 0: it is not).  *status receives a code if a wait runs out.
-extern "C" int nncpu_attention_prefill_tc(const void* q, const void* k_pages, const void* v_pages, int n_pages,
-                                          const int* block_table, int bt_stride, const int* cu_seqlens,
-                                          const int* tok_pos, void* out, int n_tok, int n_seqs, int n_heads, int n_kv,
-                                          int head_dim, int vp, int vo, float scale, int window, int keep,
-                                          float slope_base, const float* sinks, float cap, const float* head_gate,
-                                          int gate_ld, int longest, int* status, void* stream_) {
+// half: keys and values are float16 (pages of one row size).
+static int prefill_tc(bool half, const void* q, const void* k_pages, const void* v_pages, int n_pages,
+                      const int* block_table, int bt_stride, const int* cu_seqlens, const int* tok_pos, void* out, int n_tok, int n_seqs,
+                      int n_heads, int n_kv, int head_dim, int vp, int vo, float scale, int window, int keep, float slope_base,
+                      const float* sinks, float cap, const float* head_gate, int gate_ld, int longest, int* status, void* stream_) {
     NN_CHECK(nncpu_attention_prefill_tc_supported(n_heads, n_kv, head_dim),
              "attention (tensor cores): head size %d with %d heads over %d key/value heads is not supported "
              "(head size 64 or 128, heads a multiple of key/value heads)", head_dim, n_heads, n_kv);
@@ -867,7 +927,26 @@ extern "C" int nncpu_attention_prefill_tc(const void* q, const void* k_pages, co
     p.gate_ld = gate_ld;
     p.status = status;
     cudaStream_t stream = (cudaStream_t)stream_;
-    return launch_any(mq, mk, mv, p, head_dim, vp, n_tok, longest, nullptr, stream);
+    return launch_any(mq, mk, mv, p, head_dim, vp, half, n_tok, longest, nullptr, stream);
+}
+
+extern "C" int nncpu_attention_prefill_tc(const void* q, const void* k_pages, const void* v_pages, int n_pages, const int* block_table,
+                                          int bt_stride, const int* cu_seqlens, const int* tok_pos, void* out, int n_tok, int n_seqs,
+                                          int n_heads, int n_kv, int head_dim, int vp, int vo, float scale, int window, int keep,
+                                          float slope_base, const float* sinks, float cap, const float* head_gate, int gate_ld,
+                                          int longest, int* status, void* stream) {
+    return prefill_tc(false, q, k_pages, v_pages, n_pages, block_table, bt_stride, cu_seqlens, tok_pos, out, n_tok, n_seqs, n_heads, n_kv,
+                      head_dim, vp, vo, scale, window, keep, slope_base, sinks, cap, head_gate, gate_ld, longest, status, stream);
+}
+
+// The same with float16 keys and values, [n_pages, n_kv, 64, head_dim] both (queries and output bfloat16).
+extern "C" int nncpu_attention_prefill_tc_half(const void* q, const void* k_pages, const void* v_pages, int n_pages,
+                                               const int* block_table, int bt_stride, const int* cu_seqlens, const int* tok_pos,
+                                               void* out, int n_tok, int n_seqs, int n_heads, int n_kv, int head_dim, int vo, float scale,
+                                               int window, int keep, float slope_base, const float* sinks, float cap,
+                                               const float* head_gate, int gate_ld, int longest, int* status, void* stream) {
+    return prefill_tc(true, q, k_pages, v_pages, n_pages, block_table, bt_stride, cu_seqlens, tok_pos, out, n_tok, n_seqs, n_heads, n_kv,
+                      head_dim, head_dim, vo, scale, window, keep, slope_base, sinks, cap, head_gate, gate_ld, longest, status, stream);
 }
 
 // For tests: how many blocks would share a tile of such a step (the tiles of up to kAloneSteps steps among them are walked by one
@@ -882,5 +961,5 @@ extern "C" int nncpu_attention_prefill_tc_splits(int n_heads, int n_kv, int head
     p.cap_in = capped ? 1.0f : 0.0f;
     int splits = 0;
     const CUtensorMap none{};
-    return launch_any(none, none, none, p, head_dim, vp, n_tok, longest, &splits, nullptr) == 0 ? splits : 0;
+    return launch_any(none, none, none, p, head_dim, vp, false, n_tok, longest, &splits, nullptr) == 0 ? splits : 0;
 }

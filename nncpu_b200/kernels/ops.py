@@ -1580,13 +1580,55 @@ def _need(cond: bool, fn: str, what: str) -> None:
         raise InvalidArgument(f"{fn}: {what}")
 
 
-def _on_current_device(fn: str, *tensors) -> None:
-    """The kernels are launched on the current device's stream: every tensor has to live there."""
-    on = {t.device for t in tensors if t is not None and not (t.is_meta and _dry)}
-    _need(len(on) == 1, fn, f"tensors on several devices ({', '.join(sorted(map(str, on)))})")
-    dev = on.pop()
-    if dev.type == "cuda":
-        _need(dev.index == torch.cuda.current_device(), fn, f"tensors on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+# The calls below are made several times a layer and step, by steps that the host can hold up: each asks everything in one
+# condition first, and only where that fails looks for what to say.  Their C entry points have their argument types declared, so that
+# plain integers go through as pointers.
+_P, _I, _F, _L, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_long, ctypes.c_double
+_typed = {}
+
+
+def _launch(libname: str, fn: str, types, *args) -> None:
+    global _launches, _last_fn
+    found = _typed.get(fn)
+    if found is None:
+        lib = library.load(libname)
+        f = getattr(lib, fn)
+        f.argtypes = [*types, _P]
+        found = _typed[fn] = (f, lib)
+    if _dry:
+        return
+    dev = torch._C._cuda_getDevice()
+    stream = _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+    _last_fn = ""
+    if found[0](*args, stream) != 0:
+        raise ExtensionError(found[1].last_error().decode())
+    _launches += 1
+    _last_fn = fn
+
+
+def _at(t):
+    """A tensor's address (a shape-only one's: none)."""
+    return None if t is None or (t.is_meta and _dry) else t.data_ptr()
+
+
+def _one_place(fn: str, *tensors) -> None:
+    """Every tensor on the current device (whose stream the kernels are launched on), in rows without gaps."""
+    if _dry:
+        return
+    dev = tensors[0].get_device()
+    same = contiguous = True
+    for t in tensors:
+        if t is not None:
+            same = same and t.get_device() == dev
+            contiguous = contiguous and t.is_contiguous()
+    if not same:
+        raise InvalidArgument(f"{fn}: tensors on several devices ({', '.join(sorted({str(t.device) for t in tensors if t is not None}))})")
+    if not contiguous:
+        raise InvalidArgument(f"{fn}: kernels take contiguous tensors")
+    if dev < 0:
+        raise ExtensionError("the kernels run on the GPU: a tensor on the CPU was passed, and there is no CPU path")
+    if dev != torch._C._cuda_getDevice():
+        raise InvalidArgument(f"{fn}: tensors on cuda:{dev}, the current device is cuda:{torch._C._cuda_getDevice()}")
 
 
 def _int32(fn: str, **tensors) -> None:
@@ -1594,19 +1636,36 @@ def _int32(fn: str, **tensors) -> None:
         _need(t.dtype == torch.int32, fn, f"{name} holds int32, not {t.dtype}")
 
 
+def _q4_pages_ok(k_pages, v_pages, n_kv: int, head_dim: int) -> bool:
+    shape = k_pages.shape
+    return (k_pages.dtype is torch.uint8 and v_pages.dtype is torch.uint8 and v_pages.shape == shape and len(shape) == 3
+            and shape[1] == n_kv and shape[2] == 40 * head_dim and 0 < head_dim <= 256 and head_dim % Q4_GROUP == 0
+            and (_dry or (k_pages.data_ptr() | v_pages.data_ptr()) % 16 == 0))
+
+
 def _q4_pages(fn: str, k_pages, v_pages, n_kv: int, head_dim: int) -> None:
+    """Says what is wrong with a cache's pages."""
     _need(q4_supported(head_dim), fn, f"heads of {head_dim} lanes (a cache of 4 bits holds whole groups of {Q4_GROUP}, at most 256 lanes)")
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        _need(t.dtype == torch.uint8 and t.dim() == 3 and t.shape[1:] == (n_kv, q4_page_bytes(head_dim)) and t.is_contiguous(), fn,
-              f"{name} are contiguous uint8 [pages, {n_kv}, {q4_page_bytes(head_dim)}], not {t.dtype} {list(t.shape)}")
+        _need(t.dtype == torch.uint8 and t.dim() == 3 and t.shape[1:] == (n_kv, q4_page_bytes(head_dim)), fn,
+              f"{name} are uint8 [pages, {n_kv}, {q4_page_bytes(head_dim)}], not {t.dtype} {list(t.shape)}")
         _need(_aligned(t), fn, f"{name} do not start on a 16-byte boundary")
     _need(k_pages.shape == v_pages.shape, fn, f"{k_pages.shape[0]} pages of keys and {v_pages.shape[0]} of values")
 
 
+def _q4_places_ok(n: int, block_table, tok_seq, tok_pos) -> bool:
+    return (block_table.dtype is tok_seq.dtype is tok_pos.dtype is torch.int32 and block_table.dim() == 2 and block_table.shape[1] > 0
+            and tok_seq.numel() >= n and tok_pos.numel() >= n)
+
+
 def _q4_places(fn: str, n: int, block_table, tok_seq, tok_pos) -> None:
+    """Says what is wrong with the tokens' places."""
     _int32(fn, block_table=block_table, tok_seq=tok_seq, tok_pos=tok_pos)
     _need(block_table.dim() == 2 and block_table.shape[1] > 0, fn, f"a block table of shape {list(block_table.shape)}")
     _need(tok_seq.numel() >= n and tok_pos.numel() >= n, fn, f"{n} tokens, {tok_seq.numel()} sequences and {tok_pos.numel()} positions of them")
+
+
+_APPEND_Q4 = [_P, _I, _I, _P, _P, _I, _D, _P, _I, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _F, _I]
 
 
 def qk_norm_rope_append_q4(qkv, q_gamma, k_gamma, eps: float, cos_sin, tok_seq, tok_pos, block_table, k_pages, v_pages, q_out,
@@ -1620,60 +1679,81 @@ def qk_norm_rope_append_q4(qkv, q_gamma, k_gamma, eps: float, cos_sin, tok_seq, 
     lo's rounding).  Numbers beyond +-65504 count as that; a group with a NaN is NaN.  Keys are normed and rotated in 64 bits, so
     that a code does not hang on the order of a sum.  ``n_kv`` 0: qkv holds q only and nothing is appended.  A token of sequence -1, or
     whose position has no page, is not appended; two tokens at one place leave either.  ``q_temp`` as in ``qk_norm_rope_append``."""
-    fn = "qk_norm_rope_append_q4"
-    n = q_out.shape[0]
+    n, rows = q_out.shape[0], qkv.shape
     half = 0 if cos_sin is None else cos_sin.shape[1]
     coef, every = q_temp if q_temp is not None else (0.0, 1)
-    _need(q_out.shape == (n, n_heads * head_dim) and qkv.dim() == 2 and qkv.shape[0] == n
-          and qkv.shape[1] >= (n_heads + 2 * n_kv) * head_dim, fn,
-          f"{n_heads} heads over {n_kv} of {head_dim} lanes in rows of {list(qkv.shape)}, queries to {list(q_out.shape)}")
-    _need(q4_supported(head_dim), fn, f"heads of {head_dim} lanes (a cache of 4 bits holds whole groups of {Q4_GROUP}, at most 256 lanes)")
-    _need(cos_sin is None or (cos_sin.dtype == torch.float32 and cos_sin.shape == (n, half, 2) and 2 * half <= head_dim), fn,
-          "the rotation is float32 [tokens, pairs, 2], at most half a head's lanes of pairs")
-    _need(all(g is None or g.numel() == head_dim for g in (q_gamma, k_gamma)) and (q_gamma is None or k_gamma is None
-          or q_gamma.dtype == k_gamma.dtype), fn, f"norm weights of {head_dim} lanes and one type")
-    _int32(fn, tok_seq=tok_seq, tok_pos=tok_pos)
-    _need(tok_seq.numel() >= n and tok_pos.numel() >= n, fn, f"{n} tokens, {tok_seq.numel()} sequences and {tok_pos.numel()} positions of them")
-    if n_kv:
-        _q4_pages(fn, k_pages, v_pages, n_kv, head_dim)
-        _q4_places(fn, n, block_table, tok_seq, tok_pos)
-    else:
-        k_pages = v_pages = block_table = None
-    _on_current_device(fn, qkv, q_gamma, k_gamma, cos_sin, tok_seq, tok_pos, block_table, k_pages, v_pages, q_out)
+    if not (len(rows) == 2 and rows[0] == n and rows[1] >= (n_heads + 2 * n_kv) * head_dim and q_out.shape == (n, n_heads * head_dim)
+            and q4_supported(head_dim) and tok_seq.dtype is tok_pos.dtype is torch.int32 and tok_seq.numel() >= n and tok_pos.numel() >= n
+            and (cos_sin is None or (cos_sin.dtype is torch.float32 and cos_sin.shape == (n, half, 2) and 2 * half <= head_dim))
+            and (q_gamma is None or q_gamma.numel() == head_dim) and (k_gamma is None or k_gamma.numel() == head_dim)
+            and (q_gamma is None or k_gamma is None or q_gamma.dtype is k_gamma.dtype)
+            and (not n_kv or (_q4_pages_ok(k_pages, v_pages, n_kv, head_dim) and _q4_places_ok(n, block_table, tok_seq, tok_pos)))):
+        fn = "qk_norm_rope_append_q4"
+        _need(q4_supported(head_dim), fn, f"heads of {head_dim} lanes (a cache of 4 bits holds whole groups of {Q4_GROUP}, at most 256 lanes)")
+        _need(cos_sin is None or (cos_sin.dtype == torch.float32 and cos_sin.shape == (n, half, 2) and 2 * half <= head_dim), fn,
+              "the rotation is float32 [tokens, pairs, 2], at most half a head's lanes of pairs")
+        _need(all(g is None or g.numel() == head_dim for g in (q_gamma, k_gamma)) and (q_gamma is None or k_gamma is None
+              or q_gamma.dtype == k_gamma.dtype), fn, f"norm weights of {head_dim} lanes and one type")
+        if n_kv:
+            _q4_pages(fn, k_pages, v_pages, n_kv, head_dim)
+            _q4_places(fn, n, block_table, tok_seq, tok_pos)
+        _int32(fn, tok_seq=tok_seq, tok_pos=tok_pos)
+        _need(False, fn, f"{n_heads} heads over {n_kv} of {head_dim} lanes of {tok_seq.numel()} tokens in rows of {list(rows)}, "
+              f"queries to {list(q_out.shape)}")
     g = q_gamma if q_gamma is not None else k_gamma
-    _call("cache_q4", "nncpu_qk_norm_rope_append_q4", _ptr(qkv), _i(_code(qkv)), _i(qkv.shape[1]), _ptr(q_gamma), _ptr(k_gamma),
-          _i(_code(g)), ctypes.c_double(float(eps)), _ptr(cos_sin), _i(half), _ptr(tok_seq), _ptr(tok_pos), _ptr(block_table),
-          _i(block_table.shape[1] if n_kv else 0), _ptr(k_pages), _ptr(v_pages), _i(k_pages.shape[0] if n_kv else 0), _ptr(q_out),
-          _i(_code(q_out)), _i(n), _i(n_heads), _i(n_kv), _i(head_dim), _f(coef), _i(every), _stream())
+    if n_kv:
+        _one_place("qk_norm_rope_append_q4", qkv, q_gamma, k_gamma, cos_sin, tok_seq, tok_pos, block_table, k_pages, v_pages, q_out)
+        cache = (_at(block_table), block_table.shape[1], _at(k_pages), _at(v_pages), k_pages.shape[0])
+    else:
+        _one_place("qk_norm_rope_append_q4", qkv, q_gamma, k_gamma, cos_sin, tok_seq, tok_pos, q_out)
+        cache = (None, 0, None, None, 0)
+    _launch("cache_q4", "nncpu_qk_norm_rope_append_q4", _APPEND_Q4, _at(qkv), _code(qkv), rows[1], _at(q_gamma), _at(k_gamma), _code(g),
+            eps, _at(cos_sin), half, _at(tok_seq), _at(tok_pos), *cache, _at(q_out), _code(q_out), n, n_heads, n_kv, head_dim, coef, every)
+
+
+_READ_Q4 = [_P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I]
 
 
 def q4_read(k_pages, v_pages, block_table, tok_seq, tok_pos, k_out, v_out) -> None:
     """What a cache of 4 bits holds of given tokens, as numbers: keys and values of the token at position tok_pos[t] of sequence
     tok_seq[t] to ``k_out`` and ``v_out`` [n, n_kv * head_dim] (float32 or bfloat16).  A token of sequence -1, or without a page: zeros."""
-    fn = "q4_read"
-    n, n_kv = k_out.shape[0], k_pages.shape[1]
-    head_dim = k_out.shape[1] // n_kv
-    _q4_pages(fn, k_pages, v_pages, n_kv, head_dim)
-    _q4_places(fn, n, block_table, tok_seq, tok_pos)
-    _need(k_out.shape == v_out.shape == (n, n_kv * head_dim) and k_out.dtype == v_out.dtype, fn,
-          f"keys to {k_out.dtype} {list(k_out.shape)}, values to {v_out.dtype} {list(v_out.shape)}")
-    _on_current_device(fn, k_pages, v_pages, block_table, tok_seq, tok_pos, k_out, v_out)
-    _call("cache_q4", "nncpu_q4_read", _ptr(k_pages), _ptr(v_pages), _i(k_pages.shape[0]), _ptr(block_table), _i(block_table.shape[1]),
-          _ptr(tok_seq), _ptr(tok_pos), _ptr(k_out), _ptr(v_out), _i(_code(k_out)), _i(n), _i(n_kv), _i(head_dim), _stream())
+    (n, lanes), pages = k_out.shape, k_pages.shape
+    n_kv = pages[1]
+    head_dim = lanes // n_kv
+    if not (lanes == n_kv * head_dim and v_out.shape == (n, lanes) and k_out.dtype is v_out.dtype
+            and _q4_pages_ok(k_pages, v_pages, n_kv, head_dim) and _q4_places_ok(n, block_table, tok_seq, tok_pos)):
+        _q4_pages("q4_read", k_pages, v_pages, n_kv, head_dim)
+        _q4_places("q4_read", n, block_table, tok_seq, tok_pos)
+        _need(False, "q4_read", f"keys to {k_out.dtype} {list(k_out.shape)}, values to {v_out.dtype} {list(v_out.shape)}")
+    _one_place("q4_read", k_pages, v_pages, block_table, tok_seq, tok_pos, k_out, v_out)
+    _launch("cache_q4", "nncpu_q4_read", _READ_Q4, _at(k_pages), _at(v_pages), pages[0], _at(block_table), block_table.shape[1], _at(tok_seq),
+            _at(tok_pos), _at(k_out), _at(v_out), _code(k_out), n, n_kv, head_dim)
 
 
 def _attention_q4_check(fn: str, q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads: int, n_kv: int, head_dim: int,
                         window: int, keep: int, cap: float, sinks) -> int:
-    n = q.shape[0]
-    _need(n_heads > 0 and n_kv > 0 and n_heads % n_kv == 0, fn, f"{n_heads} heads over {n_kv}")
-    _q4_pages(fn, k_pages, v_pages, n_kv, head_dim)
-    _q4_places(fn, n, block_table, tok_seq, tok_pos)
-    _need(q.shape == out.shape == (n, n_heads * head_dim) and q.dtype == out.dtype, fn,
-          f"queries {q.dtype} {list(q.shape)}, output {out.dtype} {list(out.shape)}, {n_heads} heads of {head_dim} lanes")
-    _need(keep >= 0 and (keep == 0 or window > 0) and cap >= 0.0, fn, f"{keep} kept keys with a window of {window}, a cap of {cap}")
-    _need(sinks is None or (sinks.dtype == torch.float32 and sinks.numel() == n_heads), fn, f"sinks are float32 [{n_heads}]")
-    _on_current_device(fn, q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, sinks)
+    n, width = q.shape
+    if not (n_kv > 0 and n_heads > 0 and n_heads % n_kv == 0 and width == n_heads * head_dim and out.shape == (n, width) and q.dtype is out.dtype
+            and _q4_pages_ok(k_pages, v_pages, n_kv, head_dim) and _q4_places_ok(n, block_table, tok_seq, tok_pos)
+            and keep >= 0 and (keep == 0 or window > 0) and cap >= 0.0
+            and (sinks is None or (sinks.dtype is torch.float32 and sinks.numel() == n_heads))):
+        _need(n_heads > 0 and n_kv > 0 and n_heads % n_kv == 0, fn, f"{n_heads} heads over {n_kv}")
+        _q4_pages(fn, k_pages, v_pages, n_kv, head_dim)
+        _q4_places(fn, n, block_table, tok_seq, tok_pos)
+        _need(keep >= 0 and (keep == 0 or window > 0) and cap >= 0.0, fn, f"{keep} kept keys with a window of {window}, a cap of {cap}")
+        _need(sinks is None or (sinks.dtype == torch.float32 and sinks.numel() == n_heads), fn, f"sinks are float32 [{n_heads}]")
+        _need(False, fn, f"queries {q.dtype} {list(q.shape)}, output {out.dtype} {list(out.shape)}, {n_heads} heads of {head_dim} lanes")
     return n
+
+
+def _q4_gate(head_gate, n: int, n_heads: int):
+    """As ``_head_gate``, as plain numbers."""
+    if head_gate is None:
+        return None, 0
+    rows, col = head_gate
+    _need(rows.dtype == torch.float32 and rows.dim() == 2 and rows.is_contiguous() and rows.shape[0] == n and 0 <= col <= rows.shape[1] - n_heads,
+          "attention_q4", f"gate logits are float32 rows [{n}, at least {col + n_heads}]")
+    return (None if _dry else rows.data_ptr() + 4 * col), rows.shape[1]
 
 
 def _q4_longest(block_table, longest: int, window: int, keep: int) -> int:
@@ -1683,11 +1763,19 @@ def _q4_longest(block_table, longest: int, window: int, keep: int) -> int:
     return max(1, min(room, abs(window) + keep + 128) if window else room)
 
 
-def attention_q4_scratch_floats(n_tok: int, n_heads: int, n_kv: int, head_dim: int, dtype, longest: int) -> int:
-    """Floats of scratch that ``attention_q4`` needs at these sizes."""
+@functools.lru_cache(maxsize=4096)
+def _attention_q4_scratch(device: int, n_tok: int, n_heads: int, n_kv: int, head_dim: int, code: int, longest: int) -> int:
     lib = library.load("attention_q4")
     lib.nncpu_attention_q4_scratch.restype = ctypes.c_long
-    return lib.nncpu_attention_q4_scratch(_i(n_tok), _i(n_heads), _i(n_kv), _i(head_dim), _i(_DT[dtype]), _i(longest))
+    return lib.nncpu_attention_q4_scratch(_i(n_tok), _i(n_heads), _i(n_kv), _i(head_dim), _i(code), _i(longest))
+
+
+def attention_q4_scratch_floats(n_tok: int, n_heads: int, n_kv: int, head_dim: int, dtype, longest: int) -> int:
+    """Floats of scratch that ``attention_q4`` needs at these sizes on the current device."""
+    return _attention_q4_scratch(torch._C._cuda_getDevice(), n_tok, n_heads, n_kv, head_dim, _DT[dtype], longest)
+
+
+_ATTENTION_Q4 = [_P, _I, _P, _P, _I, _P, _I, _P, _P, _P, _P, _L, _I, _I, _I, _I, _F, _I, _I, _F, _P, _F, _P, _I, _I]
 
 
 def attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads: int, n_kv: int, head_dim: int, scale: float,
@@ -1700,32 +1788,114 @@ def attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_head
     is not there (an id outside the pages) holds no keys."""
     n = _attention_q4_check("attention_q4", q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads, n_kv, head_dim, window,
                             keep, cap, sinks)
+    _one_place("attention_q4", q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, sinks)
     longest = _q4_longest(block_table, longest, window, keep)
+    code = _code(q)
     if scratch is None and not _dry:
-        need = attention_q4_scratch_floats(n, n_heads, n_kv, head_dim, q.dtype, longest)
+        need = _attention_q4_scratch(q.get_device(), n, n_heads, n_kv, head_dim, code, longest)
         scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
-    _need(scratch is None or scratch.dtype == torch.float32, "attention_q4", "scratch is float32")
-    _call("attention_q4", "nncpu_attention_q4", _ptr(q), _i(_code(q)), _ptr(k_pages), _ptr(v_pages), _i(k_pages.shape[0]),
-          _ptr(block_table), _i(block_table.shape[1]), _ptr(tok_seq), _ptr(tok_pos), _ptr(out), _ptr(scratch),
-          _l(0 if scratch is None else scratch.numel()), _i(n), _i(n_heads), _i(n_kv), _i(head_dim), _f(scale), _i(window), _i(keep),
-          _f(slope_base), _ptr(sinks), _f(cap), *_head_gate(head_gate, n, n_heads), _i(longest), _stream())
+    _need(scratch is None or (scratch.dtype is torch.float32 and scratch.is_contiguous()), "attention_q4", "scratch is contiguous float32")
+    _launch("attention_q4", "nncpu_attention_q4", _ATTENTION_Q4, _at(q), code, _at(k_pages), _at(v_pages), k_pages.shape[0], _at(block_table),
+            block_table.shape[1], _at(tok_seq), _at(tok_pos), _at(out), _at(scratch), 0 if scratch is None else scratch.numel(), n, n_heads,
+            n_kv, head_dim, scale, window, keep, slope_base, _at(sinks), cap, *_q4_gate(head_gate, n, n_heads), longest)
+
+
+# Prompts take their sequences' keys and values out of the codes once, for all query tiles and heads, and attend to those: float16 for
+# the tcgen05 kernel, float32 for the 32-bit one.  So many positions at a time (of whole sequences, one at least).
+Q4_EXPAND_POSITIONS = 16384
+Q4_EXPAND_POSITIONS_F32 = 65536
+
+
+@functools.lru_cache(maxsize=4096)
+def _q4_prompt_plan(n: int, n_seqs: int, n_heads: int, n_kv: int, head_dim: int, bf16: bool, longest: int, slope_and_cap: bool):
+    """How a prompt attends: (lanes of the rows that the keys are taken out to, or 0: token by token; pages of a sequence; sequences
+    at a time; bytes of keys; of keys, values and table; of all)."""
+    width = (longest + 63) // 64
+    lanes = 0
+    if n <= n_seqs:
+        pass
+    elif bf16:
+        lanes = 64 if head_dim <= 64 else 128 if head_dim <= 128 and not slope_and_cap else 0
+        lanes = 0 if slope_and_cap else lanes
+    elif head_dim <= 128 and n_heads // n_kv <= 32 and n_seqs * width * 64 <= Q4_EXPAND_POSITIONS_F32:
+        lanes = head_dim
+    if lanes == 0:
+        return 0, width, 0, 0, 0, 0
+    at_once = max(1, min(n_seqs, Q4_EXPAND_POSITIONS // (width * 64))) if bf16 else n_seqs
+    kv_bytes = at_once * width * n_kv * 64 * lanes * (2 if bf16 else 4)
+    table = 2 * kv_bytes + (at_once * width * 4 + 255) // 256 * 256
+    return lanes, width, at_once, kv_bytes, table, table + (n * n_heads * lanes * 2 if bf16 and lanes != head_dim else 0)
+
+
+def attention_q4_prompt_scratch_bytes(n_tok: int, n_seqs: int, n_heads: int, n_kv: int, head_dim: int, dtype, longest: int,
+                                      slope_base: float = 0.0, cap: float = 0.0) -> int:
+    """Bytes of scratch that ``attention_q4_prompt`` needs at these sizes on the current device."""
+    plan = _q4_prompt_plan(n_tok, n_seqs, n_heads, n_kv, head_dim, dtype == torch.bfloat16, longest, slope_base != 0.0 and cap != 0.0)
+    return plan[5] if plan[0] else 4 * attention_q4_scratch_floats(n_tok, n_heads, n_kv, head_dim, dtype, longest)
+
+
+_EXPAND_Q4 = [_P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I]
+_PREFILL_HALF = [_P, _P, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _F, _P, _F, _P, _I, _I, _P]
 
 
 def attention_q4_prompt(q, k_pages, v_pages, block_table, cu_seqlens, tok_seq, tok_pos, out, n_seqs: int, n_heads: int, n_kv: int,
                         head_dim: int, scale: float, longest: int, status, window: int = 0, slope_base: float = 0.0, sinks=None,
-                        keep: int = 0, cap: float = 0.0, head_gate=None) -> None:
+                        keep: int = 0, cap: float = 0.0, head_gate=None, scratch=None) -> None:
     """``attention_q4`` for prompts and portions of them: any number of tokens a sequence, at consecutive positions (``cu_seqlens``
-    int32 [n_seqs + 1]: each sequence's first token).  ``longest``: at least as many keys as any token sees."""
+    int32 [n_seqs + 1]: each sequence's first token).  ``longest``: at least as many keys as any token sees.  ``status``: an int32 word on
+    the device that receives a code if a bounded wait runs out, as in ``attention_prefill_tc``.  ``scratch``: uint8,
+    ``attention_q4_prompt_scratch_bytes`` elements (None: taken from the allocator).  Here a page that is not there counts as zeros."""
     fn = "attention_q4_prompt"
-    _int32(fn, cu_seqlens=cu_seqlens)
-    _need(n_seqs > 0 and cu_seqlens.numel() >= n_seqs + 1 and longest > 0, fn, f"{n_seqs} sequences, {cu_seqlens.numel()} places, {longest} keys")
-    attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads, n_kv, head_dim, scale, window, slope_base, sinks, keep,
-                 cap, head_gate, longest)
+    n = _attention_q4_check(fn, q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads, n_kv, head_dim, window, keep, cap, sinks)
+    if not (cu_seqlens.dtype is torch.int32 and cu_seqlens.dim() == 1 and 0 < n_seqs < cu_seqlens.shape[0] and longest > 0
+            and block_table.shape[0] >= n_seqs and status.dtype is torch.int32 and status.numel() > 0):
+        _int32(fn, cu_seqlens=cu_seqlens, status=status)
+        _need(False, fn, f"{n_seqs} sequences, places {list(cu_seqlens.shape)}, tables {list(block_table.shape)}, {longest} keys")
+    _one_place(fn, q, k_pages, v_pages, block_table, cu_seqlens, tok_seq, tok_pos, out, sinks, status, scratch)
+    longest = min(longest, block_table.shape[1] * 64)
+    bf16 = _code(q) == 1
+    lanes, width, at_once, kv_bytes, table_end, need = _q4_prompt_plan(n, n_seqs, n_heads, n_kv, head_dim, bf16, longest,
+                                                                       slope_base != 0.0 and cap != 0.0)
+    if lanes == 0:
+        if scratch is not None:
+            scratch = scratch.view(torch.float32)
+        attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads, n_kv, head_dim, scale, window, slope_base, sinks, keep,
+                     cap, head_gate, longest, scratch)
+        return
+    if scratch is None:
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _need(scratch.dtype is torch.uint8 and scratch.dim() == 1 and scratch.numel() >= need and _aligned(scratch), fn,
+          f"scratch of {scratch.numel()} bytes ({need} are needed, from a 16-byte boundary)")
+    if n == 0:
+        return
+    base = _at(scratch) or 0
+    k_at, v_at, table_at = base, base + kv_bytes, base + 2 * kv_bytes
+    longer = bf16 and lanes != head_dim
+    gate, gate_ld = _q4_gate(head_gate, n, n_heads)
+    width_in = block_table.shape[1]
+    for b in range(0, n_seqs, at_once):
+        count = min(at_once, n_seqs - b)
+        table_in, cu = (_at(block_table) or 0) + 4 * b * width_in, (_at(cu_seqlens) or 0) + 4 * b
+        _launch("cache_q4", "nncpu_q4_expand", _EXPAND_Q4, _at(k_pages), _at(v_pages), k_pages.shape[0], table_in, width_in, cu, _at(tok_pos),
+                count, width, n_kv, head_dim, lanes, window, keep, bf16, k_at, v_at, table_at, _at(q) if longer and b == 0 else None,
+                base + table_end if longer else None, n, n_heads)
+        if bf16:
+            _launch("attention_tc", "nncpu_attention_prefill_tc_half", _PREFILL_HALF, base + table_end if longer else _at(q), k_at, v_at,
+                    count * width, table_at, width, cu, _at(tok_pos), _at(out), n, count, n_heads, n_kv, lanes, head_dim, scale, window, keep,
+                    slope_base, _at(sinks), cap, gate, gate_ld, longest, _at(status))
+        else:
+            _launch("attention_f32", "nncpu_attention_f32", _PROMPT_F32, _at(q), k_at, v_at, table_at, width, _at(tok_seq), _at(tok_pos),
+                    _at(out), None, n, n_heads, n_kv, head_dim, head_dim, head_dim, scale, window, keep, slope_base, _at(sinks), cap, gate,
+                    gate_ld, 0, 0, n_seqs, torch.cuda.get_device_properties(q.device).multi_processor_count if not _dry else 148)
+
+
+_PROMPT_F32 = [_P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _F, _P, _F, _P, _I, _I, _I, _I, _I]
 
 
 # -- log probabilities ---------------------------------------------------------------------------------------------------
 
 LOGPROBS_MAX_TOP = 64
+_LOGPROBS = [_P, _I, _P, _P, _P, _P, _P, _I, _I, _I]
 
 
 def token_logprobs(logits, targets, logprobs, entropy, top=None, ids=None) -> None:
@@ -1735,19 +1905,18 @@ def token_logprobs(logits, targets, logprobs, entropy, top=None, ids=None) -> No
 
     A NaN counts as -inf; a token of -inf has log probability -inf.  A row with nothing above -inf gives -inf for every token and an
     entropy of 0; one with a logit of +inf gives NaN (and its order).  A target outside the vocabulary gives NaN."""
-    fn = "token_logprobs"
-    _need(logits.dim() == 2 and logits.shape[1] > 0, fn, f"logits of shape {list(logits.shape)}")
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        _need(False, "token_logprobs", f"logits of shape {list(logits.shape)}")
     n, vocab = logits.shape
-    _int32(fn, targets=targets)
-    _need(targets.shape == (n,) and logprobs.shape == (n,) and entropy.shape == (n,) and logprobs.dtype == entropy.dtype == torch.float32, fn,
-          f"{n} rows: targets int32 [{n}], logprobs and entropy float32 [{n}]")
-    _need((top is None) == (ids is None), fn, "top and ids come together")
-    k = 0
-    if top is not None:
-        k = top.shape[1] if top.dim() == 2 else -1
-        _int32(fn, ids=ids)
-        _need(top.shape == ids.shape == (n, k) and top.dtype == torch.float32, fn, f"top float32 and ids int32 [{n}, k]")
-        _need(0 < k <= min(LOGPROBS_MAX_TOP, vocab), fn, f"the best {k} of {vocab} (1 to {LOGPROBS_MAX_TOP})")
-    _on_current_device(fn, logits, targets, logprobs, entropy, top, ids)
-    _call("token_logprobs", "nncpu_token_logprobs", _ptr(logits), _i(_code(logits)), _ptr(targets), _ptr(logprobs), _ptr(entropy), _ptr(top),
-          _ptr(ids), _i(n), _i(vocab), _i(k), _stream())
+    k = top.shape[1] if top is not None and top.dim() == 2 else 0
+    if not (targets.dtype is torch.int32 and targets.shape == (n,) and logprobs.shape == (n,) and entropy.shape == (n,)
+            and logprobs.dtype is entropy.dtype is torch.float32 and (top is None) == (ids is None)
+            and (top is None or (0 < k <= min(LOGPROBS_MAX_TOP, vocab) and top.shape == (n, k) and ids.shape == (n, k)
+                                 and top.dtype is torch.float32 and ids.dtype is torch.int32))):
+        fn = "token_logprobs"
+        _need((top is None) == (ids is None), fn, "top and ids come together")
+        _need(top is None or 0 < k <= min(LOGPROBS_MAX_TOP, vocab), fn, f"the best {k} of {vocab} (1 to {LOGPROBS_MAX_TOP})")
+        _need(False, fn, f"{n} rows: targets int32, logprobs and entropy float32 [{n}], top float32 and ids int32 [{n}, {k}]")
+    _one_place("token_logprobs", logits, targets, logprobs, entropy, top, ids)
+    _launch("token_logprobs", "nncpu_token_logprobs", _LOGPROBS, _at(logits), _code(logits), _at(targets), _at(logprobs), _at(entropy), _at(top),
+            _at(ids), n, vocab, k)
