@@ -3,6 +3,13 @@
 //   the k best by (x descending, index ascending).
 // A NaN counts as -inf, as everywhere in the choice of a token (crates/nncpu/src/model/forward.rs:1003-1011); a lane of -inf has
 // probability 0 and adds nothing to the entropy.
+//
+// One pass over the logits, which is what bounds it: a thread keeps (maximum, sum, weighted sum) of what it has seen and
+// follows the maximum 16 logits (32 of bfloat16) at a time.  Alternatives ride along: a warp keeps its best 32 as sorted keys
+// (the order of the logit's bits above the complement of the index), one a lane, and a bar that a logit must reach to be
+// looked at: the k-th best of what any warp of the block has seen.  The first bar is the k-th largest of the lanes' first
+// maxima, so that few logits ever pass; those that do gather in shared memory and are sorted into the list 32 at a time.
+// Where there are few rows several blocks, a cluster, share one, each a stretch of it, and meet in distributed shared memory.
 
 #include <math.h>
 
@@ -13,7 +20,6 @@ namespace {
 
 struct Rows {
     const void* logits;      // [n, vocab]
-    int dt;
     const int* targets;      // [n]
     float* logprobs;         // [n]
     float* entropy;          // [n]
@@ -22,70 +28,320 @@ struct Rows {
     int n, vocab, k;
 };
 
-__device__ __forceinline__ float logit(const Rows& p, size_t row, int i) {
-    const float x = ld_f(p.logits, row * p.vocab + i, p.dt);
-    return x != x ? -INFINITY : x;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMaxTop = 32;
+constexpr int kMaxSplits = 16;      // blocks of a cluster
+constexpr int kVectors = 4;         // 16-byte vectors of a thread's turn
+typedef unsigned long long Key;
+
+__device__ __forceinline__ Key key_of(float x, int i) {
+    const uint32_t b = __float_as_uint(x + 0.0f);     // (zeros of both signs are equal)
+    return (Key)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t)~i;
+}
+__device__ __forceinline__ float logit_of(Key key) {
+    const uint32_t u = (uint32_t)(key >> 32);
+    return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
 }
 
-constexpr int kThreads = 512;
+// A warp's keys, one a lane, into descending order.
+__device__ __forceinline__ Key step(Key a, int stride, bool larger, int lane) {
+    const Key b = __shfl_xor_sync(0xffffffffu, a, stride);
+    return larger == (a > b) ? a : b;
+}
+__device__ __forceinline__ Key sort32(Key a, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int stride = size >> 1; stride > 0; stride >>= 1)
+            a = step(a, stride, ((lane & stride) == 0) == ((lane & size) == 0 || size == 32), lane);
+    return a;
+}
+// The best 32 of two descending lists, descending.
+__device__ __forceinline__ Key merge32(Key a, Key b, int lane) {
+    b = __shfl_xor_sync(0xffffffffu, b, 31);
+    a = a > b ? a : b;
+#pragma unroll
+    for (int stride = 16; stride > 0; stride >>= 1) a = step(a, stride, (lane & stride) == 0, lane);
+    return a;
+}
 
-__global__ void __launch_bounds__(kThreads) rows_kernel(const Rows p) {
-    __shared__ float scratch[33];
-    __shared__ unsigned long long best;
-    const size_t row = blockIdx.x;
-    float m = -INFINITY;
-    for (int i = threadIdx.x; i < p.vocab; i += kThreads) m = fmaxf(m, logit(p, row, i));
-    m = block_max(m, scratch);
-    float s = 0.0f, e = 0.0f;
-    for (int i = threadIdx.x; i < p.vocab; i += kThreads) {
-        const float x = logit(p, row, i);
-        if (x > -INFINITY) {
-            const float y = x - m, w = expf(y);
-            s += w;
-            e = fmaf(w, y, e);
+struct Sums {
+    float m, s, e;      // maximum, sum of w = e^(x - m), sum of w (x - m)
+};
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
+    Sums r;
+    r.m = fmaxf(a.m, b.m);
+    if (r.m == -INFINITY) return Sums{-INFINITY, 0.0f, 0.0f};
+    const float da = a.m - r.m, db = b.m - r.m;
+    const float fa = a.m == -INFINITY ? 0.0f : expf(da), fb = b.m == -INFINITY ? 0.0f : expf(db);
+    r.s = a.s * fa + b.s * fb;
+    r.e = (fa == 0.0f ? 0.0f : fa * fmaf(a.s, da, a.e)) + (fb == 0.0f ? 0.0f : fb * fmaf(b.s, db, b.e));
+    return r;
+}
+
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t remote_of(const void* local, uint32_t rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ float ld_remote(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ Key ld_remote_key(uint32_t at) {
+    Key v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+    return v;
+}
+
+template <bool BF16, bool TOP>
+__global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Rows p, int splits) {
+    constexpr int E = BF16 ? 8 : 4;              // logits of a vector
+    __shared__ Key waiting[TOP ? kWarps : 1][64];
+    __shared__ Key lists[TOP ? kWarps : 1][32];
+    __shared__ Sums sums[kWarps];
+    __shared__ Sums whole;
+    __shared__ int bar_bits;                     // the bar, as an integer of the same order
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const size_t row = blockIdx.x / splits;
+    const int split = blockIdx.x % splits;
+    const int size = BF16 ? 2 : 4;
+    const char* base = reinterpret_cast<const char*>(p.logits) + row * p.vocab * size;
+    // vectors lie on 16-byte boundaries; vector v holds logits E v - shift to E v - shift + E - 1 of the row
+    const int shift = (int)((uintptr_t)base % 16) / size;
+    const int n_vec = (p.vocab + shift + E - 1) / E;
+    const int v0 = (int)((long)n_vec * split / splits), v1 = (int)((long)n_vec * (split + 1) / splits);
+    if (TOP) {
+        if (tid == 0) bar_bits = 0x80000000;     // below everything
+        __syncthreads();
+    }
+    Sums mine{-INFINITY, 0.0f, 0.0f};
+    Key list = 0;                                // this lane's of the warp's best 32
+    Key last = 0;                                // the k-th of them
+    int n_waiting = 0;
+    float bar = -INFINITY;
+    bool first = true;
+    auto settle = [&]() {                        // sorts what waits into the list
+        __syncwarp();
+        Key got = lane < n_waiting ? waiting[warp][lane] : 0;
+        list = merge32(list, sort32(got, lane), lane);
+        if (n_waiting > 32) {
+            got = 32 + lane < n_waiting ? waiting[warp][32 + lane] : 0;
+            list = merge32(list, sort32(got, lane), lane);
+        }
+        n_waiting = 0;
+        last = __shfl_sync(0xffffffffu, list, p.k - 1);
+        if (last != 0) {
+            const int bits = (int)((uint32_t)(last >> 32) ^ 0x80000000u);
+            if (lane == 0) atomicMax(&bar_bits, bits);
+        }
+        __syncwarp();
+    };
+    for (int v = v0; v < v1; v += kThreads * kVectors) {
+        float x[kVectors * E];
+#pragma unroll
+        for (int u = 0; u < kVectors; ++u) {
+            const int at = v + u * kThreads + tid, i = at * E - shift;
+            if (at < v1 && i >= 0 && i + E <= p.vocab) {
+                const uint4 w = __ldcs(reinterpret_cast<const uint4*>(base + (long)i * size));
+                if constexpr (BF16) {
+                    const float2 a = two_bf16(w.x), b = two_bf16(w.y), c = two_bf16(w.z), d = two_bf16(w.w);
+                    x[u * E] = a.x; x[u * E + 1] = a.y; x[u * E + 2] = b.x; x[u * E + 3] = b.y;
+                    x[u * E + 4] = c.x; x[u * E + 5] = c.y; x[u * E + 6] = d.x; x[u * E + 7] = d.y;
+                } else {
+                    x[u * E] = __uint_as_float(w.x); x[u * E + 1] = __uint_as_float(w.y);
+                    x[u * E + 2] = __uint_as_float(w.z); x[u * E + 3] = __uint_as_float(w.w);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                    x[u * E + j] = at < v1 && i + j >= 0 && i + j < p.vocab ? ld_f(base, (size_t)(i + j), BF16 ? DT_BF16 : DT_F32) : -INFINITY;
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kVectors * E; ++j) mx = fmaxf(mx, x[j]);      // (a NaN is dropped)
+        const float m = fmaxf(mine.m, mx);
+        if (m > -INFINITY) {
+            const float d = mine.m - m;
+            if (d < 0.0f) {
+                const float f = mine.m == -INFINITY ? 0.0f : expf(d);
+                mine.e = mine.m == -INFINITY ? 0.0f : f * fmaf(mine.s, d, mine.e);
+                mine.s *= f;
+                mine.m = m;
+            }
+            float s = 0.0f, e = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kVectors * E; ++j) {
+                // 2^-150 and less is 0, and 0 times its finite y adds nothing; -inf and NaN come to y = -1000 or so
+                const float y = fmaxf(x[j] - m, -1000.0f), w = fast_exp2(y * 1.4426950408889634f);
+                s += w;
+                e = fmaf(w, y, e);
+            }
+            mine.s += s;
+            mine.e += e;
+        }
+        if (TOP) {
+            if (first) {
+                // at least k logits are as large as the k-th of the lanes' largest: the first bar
+                first = false;
+                const Key sorted = sort32(key_of(mx, 0), lane);
+                const Key kth = __shfl_sync(0xffffffffu, sorted, p.k - 1);
+                if (lane == 0) atomicMax(&bar_bits, (int)((uint32_t)(kth >> 32) ^ 0x80000000u));
+                __syncwarp();
+            }
+            const int bits = *reinterpret_cast<volatile int*>(&bar_bits);
+            bar = logit_of((Key)((uint32_t)bits ^ 0x80000000u) << 32);
+            if (!(bar > -INFINITY)) bar = -INFINITY;
+            if (__any_sync(0xffffffffu, mx >= bar)) {
+#pragma unroll 1
+                for (int u = 0; u < kVectors; ++u)
+#pragma unroll
+                    for (int j = 0; j < E; ++j) {
+                        float c = -INFINITY;
+#pragma unroll
+                        for (int w = 0; w < kVectors; ++w) c = w == u ? x[w * E + j] : c;
+                        const int at = v + u * kThreads + tid, i = at * E - shift + j;
+                        if (c != c) c = -INFINITY;
+                        const bool looks = at < v1 && i >= 0 && i < p.vocab && c >= bar;
+                        if (!__any_sync(0xffffffffu, looks)) continue;
+                        const Key key = key_of(c, i);
+                        const unsigned pass = __ballot_sync(0xffffffffu, looks && key > last);
+                        if (pass == 0) continue;
+                        if (pass >> lane & 1) waiting[warp][n_waiting + __popc(pass & ((1u << lane) - 1))] = key;
+                        n_waiting += __popc(pass);
+                        if (n_waiting >= 32) settle();
+                    }
+            }
         }
     }
-    s = block_sum(s, scratch);
-    e = block_sum(e, scratch);
-    const float logs = logf(s);
-    if (threadIdx.x == 0) {
+    // -- the warps of a block, then the blocks of a row
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        Sums other;
+        other.m = __shfl_xor_sync(0xffffffffu, mine.m, o);
+        other.s = __shfl_xor_sync(0xffffffffu, mine.s, o);
+        other.e = __shfl_xor_sync(0xffffffffu, mine.e, o);
+        mine = join(mine, other);
+    }
+    if (lane == 0) sums[warp] = mine;
+    if (TOP) {
+        if (n_waiting > 0) settle();
+        lists[warp][lane] = list;
+    }
+    __syncthreads();
+    if (TOP)
+        for (int half = kWarps / 2; half > 0; half >>= 1) {
+            if (warp < half) lists[warp][lane] = merge32(lists[warp][lane], lists[warp + half][lane], lane);
+            __syncthreads();
+        }
+    if (warp == 0) {
+        Sums a = lane < kWarps ? sums[lane] : Sums{-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            Sums other;
+            other.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+            other.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+            other.e = __shfl_xor_sync(0xffffffffu, a.e, o);
+            a = join(a, other);
+        }
+        if (lane == 0) whole = a;
+    }
+    if (splits > 1) {
+        cluster_barrier();
+        if (split == 0 && warp < splits && TOP) list = ld_remote_key(remote_of(&lists[0][lane], warp));
+        if (split == 0 && warp == 0) {
+            Sums a{-INFINITY, 0.0f, 0.0f};
+            if (lane < splits) {
+                const uint32_t at = remote_of(&whole, lane);
+                a = Sums{ld_remote(at), ld_remote(at + 4), ld_remote(at + 8)};
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                Sums other;
+                other.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+                other.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+                other.e = __shfl_xor_sync(0xffffffffu, a.e, o);
+                a = join(a, other);
+            }
+            if (lane == 0) sums[0] = a;
+        }
+        cluster_barrier();          // what other blocks left has been read
+        if (split != 0) return;
+        if (TOP && warp < splits) lists[warp][lane] = list;
+        __syncthreads();
+        if (TOP)
+            for (int half = splits / 2; half > 0; half >>= 1) {
+                if (warp < half) lists[warp][lane] = merge32(lists[warp][lane], lists[warp + half][lane], lane);
+                __syncthreads();
+            }
+        if (tid == 0) whole = sums[0];
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    const Sums a = whole;
+    const float logs = a.m == -INFINITY ? 0.0f : (float)log((double)a.s);
+    if (lane == 0) {
         const int t = p.targets[row];
-        p.logprobs[row] = t < 0 || t >= p.vocab ? __int_as_float(0x7FC00000) : m == -INFINITY ? -INFINITY : logit(p, row, t) - m - logs;
-        p.entropy[row] = m == -INFINITY ? 0.0f : logs - e / s;
+        float x = t < 0 || t >= p.vocab ? __int_as_float(0x7FC00000) : ld_f(p.logits, row * p.vocab + t, BF16 ? DT_BF16 : DT_F32);
+        if (t >= 0 && t < p.vocab && x != x) x = -INFINITY;
+        p.logprobs[row] = x != x ? x : a.m == INFINITY ? a.m - a.m : x == -INFINITY ? x : (x - a.m) - logs;
+        p.entropy[row] = a.m == -INFINITY ? 0.0f : a.m == INFINITY ? a.m - a.m : logs - a.e / a.s;
     }
-    // the k best, one after the other: the greatest (x, -index) below the one before
-    unsigned long long before = ~0ull;
-    for (int k = 0; k < p.k; ++k) {
-        if (threadIdx.x == 0) best = 0;
-        __syncthreads();
-        unsigned long long mine = 0;
-        for (int i = threadIdx.x; i < p.vocab; i += kThreads) {
-            const uint32_t b = __float_as_uint(logit(p, row, i) + 0.0f);
-            const unsigned long long key = (unsigned long long)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t)~i;
-            if (key < before && key > mine) mine = key;
-        }
-        atomicMax(&best, mine);
-        __syncthreads();
-        before = best;
-        if (threadIdx.x == 0) {
-            const int i = (int)~(uint32_t)before;
-            p.ids[row * p.k + k] = i;
-            const float x = logit(p, row, i);
-            p.top[row * p.k + k] = x == -INFINITY ? -INFINITY : x - m - logs;
-        }
-        __syncthreads();
+    if (TOP && lane < p.k) {
+        const Key key = lists[0][lane];
+        const float x = logit_of(key);
+        p.ids[row * p.k + lane] = (int)~(uint32_t)key;
+        p.top[row * p.k + lane] = a.m == INFINITY ? a.m - a.m : x == -INFINITY ? x : (x - a.m) - logs;
     }
 }
 
 }  // namespace
 
+// Blocks that share a row: enough for the device, each with a few turns of its threads.
+static int splits_of(int n, int vocab) {
+    int s = 1;
+    while (s < kMaxSplits && (long)n * s < 4L * sm_count() && vocab / (2 * s) >= 4 * kThreads) s *= 2;
+    return s;
+}
+
 extern "C" int nncpu_token_logprobs(const void* logits, int dt, const int* targets, float* logprobs, float* entropy, float* top, int* ids,
                                     int n, int vocab, int k, cudaStream_t stream) {
     NN_CHECK(n >= 0 && vocab > 0 && vocab < (1 << 30), "token_logprobs: %d rows of %d logits", n, vocab);
-    NN_CHECK(k >= 0 && k <= vocab && k <= 64, "token_logprobs: the best %d of %d (at most 64)", k, vocab);
+    NN_CHECK(k >= 0 && k <= vocab && k <= kMaxTop, "token_logprobs: the best %d of %d (at most %d)", k, vocab, kMaxTop);
+    NN_CHECK((uintptr_t)logits % (dt == DT_BF16 ? 2 : 4) == 0, "token_logprobs: logits do not start on a number's boundary");
     if (n == 0) return 0;
-    Rows p{logits, dt, targets, logprobs, entropy, top, ids, n, vocab, k};
-    rows_kernel<<<(unsigned)n, kThreads, 0, stream>>>(p);
-    NN_LAUNCH_OK("token_logprobs");
+    const Rows p{logits, targets, logprobs, entropy, top, ids, n, vocab, k};
+    const auto kernel = dt == DT_BF16 ? (k ? rows_kernel<true, true> : rows_kernel<true, false>) : (k ? rows_kernel<false, true> : rows_kernel<false, false>);
+    static bool done[4][64];
+    if (first_use_on_this_device(done[(dt == DT_BF16 ? 2 : 0) + (k ? 1 : 0)])) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        NN_CHECK(e == cudaSuccess, "token_logprobs: clusters of %d: %s", kMaxSplits, cudaGetErrorString(e));
+    }
+    const int splits = splits_of(n, vocab);
+    NN_CHECK((long)n * splits < (1L << 31), "token_logprobs: %d rows", n);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(n * splits));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = splits > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p, splits);
+    NN_CHECK(e == cudaSuccess, "token_logprobs: launch failed: %s", cudaGetErrorString(e));
     return 0;
 }

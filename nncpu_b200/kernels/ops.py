@@ -1894,14 +1894,14 @@ _PROMPT_F32 = [_P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _
 
 # -- log probabilities ---------------------------------------------------------------------------------------------------
 
-LOGPROBS_MAX_TOP = 64
+LOGPROBS_MAX_TOP = 32
 _LOGPROBS = [_P, _I, _P, _P, _P, _P, _P, _I, _I, _I]
 
 
 def token_logprobs(logits, targets, logprobs, entropy, top=None, ids=None) -> None:
     """For every row of ``logits`` [n, vocab] (float32 or bfloat16): ``logprobs`` float32 [n], the log probability of token
     targets[r] (int32) under the row's softmax; ``entropy`` float32 [n], in nats; with ``top`` float32 [n, k] and ``ids`` int32 [n, k]
-    (k up to 64) the k most probable tokens, by (log probability descending, id ascending).
+    (k up to 32) the k most probable tokens, by (log probability descending, id ascending).
 
     A NaN counts as -inf; a token of -inf has log probability -inf.  A row with nothing above -inf gives -inf for every token and an
     entropy of 0; one with a logit of +inf gives NaN (and its order).  A target outside the vocabulary gives NaN."""

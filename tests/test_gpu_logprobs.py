@@ -63,7 +63,7 @@ def check(logits, targets, k):
 
 
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("n,vocab,k", [(1, 1, 1), (1, 2, 2), (3, 7, 0), (5, 384, 20), (2, 1025, 64), (9, 4099, 5), (1, 151936, 20), (300, 257, 1),
+@pytest.mark.parametrize("n,vocab,k", [(1, 1, 1), (1, 2, 2), (3, 7, 0), (5, 384, 20), (2, 1025, 32), (3, 33, 33 - 1), (70, 4100, 31), (9, 4099, 5), (1, 151936, 20), (300, 257, 1),
                                        (3, 50257, 10), (8, 151936, 5), (2, 200003, 3), (40, 32768, 2), (2, 400001, 8)])
 def test_rows(n, vocab, k, dt):
     g = torch.Generator().manual_seed(n * vocab)

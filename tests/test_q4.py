@@ -107,7 +107,7 @@ def test_read_refuses(change):
     dict(targets=torch.zeros(3, dtype=torch.int32)), dict(logprobs=torch.zeros(2, dtype=torch.bfloat16)), dict(entropy=torch.zeros(1)),
     dict(top=None), dict(ids=None), dict(top=torch.zeros(2, 11), ids=torch.zeros(2, 11, dtype=torch.int32)),
     dict(top=torch.zeros(2, 0), ids=torch.zeros(2, 0, dtype=torch.int32)), dict(top=torch.zeros(2, 4)), dict(ids=torch.zeros(2, 3)),
-    dict(logits=torch.zeros(2, 200), top=torch.zeros(2, 65), ids=torch.zeros(2, 65, dtype=torch.int32)), dict(entropy=torch.zeros(2, device="meta"))])
+    dict(logits=torch.zeros(2, 200), top=torch.zeros(2, 33), ids=torch.zeros(2, 33, dtype=torch.int32)), dict(entropy=torch.zeros(2, device="meta"))])
 def test_logprobs_refuse(change):
     args = dict(logits=torch.zeros(2, 10), targets=torch.zeros(2, dtype=torch.int32), logprobs=torch.zeros(2), entropy=torch.zeros(2),
                 top=torch.zeros(2, 3), ids=torch.zeros(2, 3, dtype=torch.int32))
