@@ -7,8 +7,8 @@
 // One pass over the logits, which is what bounds it: a thread keeps (maximum, sum, weighted sum) of what it has seen and
 // follows the maximum 16 logits (32 of bfloat16) at a time.  Alternatives ride along: a warp keeps its best 32 as sorted keys
 // (the order of the logit's bits above the complement of the index), one a lane, and a bar that a logit must reach to be
-// looked at: the k-th best of what any warp of the block has seen.  The first bar is the k-th largest of the lanes' first
-// maxima, so that few logits ever pass; those that do gather in shared memory and are sorted into the list 32 at a time.
+// looked at, the k-th best of what any warp of the block has seen or less.  The first bar is the least of what the warps offer, each the
+// ceil(k / warps)-th largest of its lanes' first maxima: at least k logits reach that, and few more.  Those that that do gather in shared memory and are sorted into the list 32 at a time.
 // Where there are few rows several blocks, a cluster, share one, each a stretch of it, and meet in distributed shared memory.
 
 #include <math.h>
@@ -28,10 +28,12 @@ struct Rows {
     int n, vocab, k;
 };
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
 constexpr int kMaxSplits = 16;      // blocks of a cluster
 constexpr int kVectors = 4;         // 16-byte vectors of a thread's turn
+constexpr int kStages = 3;          // turns in flight
+constexpr int kRing = kStages * kVectors * kThreads * 16;
 typedef unsigned long long Key;
 
 __device__ __forceinline__ Key key_of(float x, int i) {
@@ -42,6 +44,9 @@ __device__ __forceinline__ float logit_of(Key key) {
     const uint32_t u = (uint32_t)(key >> 32);
     return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
 }
+
+// A logit's place in the order, as an integer.
+__device__ __forceinline__ int ordered(float x) { return (int)((uint32_t)(key_of(x, 0) >> 32) ^ 0x80000000u); }
 
 // A warp's keys, one a lane, into descending order.
 __device__ __forceinline__ Key step(Key a, int stride, bool larger, int lane) {
@@ -68,15 +73,14 @@ __device__ __forceinline__ Key merge32(Key a, Key b, int lane) {
 struct Sums {
     float m, s, e;      // maximum, sum of w = e^(x - m), sum of w (x - m)
 };
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-    Sums r;
-    r.m = fmaxf(a.m, b.m);
-    if (r.m == -INFINITY) return Sums{-INFINITY, 0.0f, 0.0f};
-    const float da = a.m - r.m, db = b.m - r.m;
-    const float fa = a.m == -INFINITY ? 0.0f : expf(da), fb = b.m == -INFINITY ? 0.0f : expf(db);
-    r.s = a.s * fa + b.s * fb;
-    r.e = (fa == 0.0f ? 0.0f : fa * fmaf(a.s, da, a.e)) + (fb == 0.0f ? 0.0f : fb * fmaf(b.s, db, b.e));
-    return r;
+// Those of a warp's lanes, joined: every lane gets them.
+__device__ __forceinline__ Sums join_lanes(Sums a) {
+    const float m = warp_max(a.m), d = a.m - m;
+    const float f = a.m == -INFINITY ? 0.0f : expf(d);
+    a.e = warp_sum(f == 0.0f ? 0.0f : f * fmaf(a.s, d, a.e));
+    a.s = warp_sum(f * a.s);
+    a.m = m;
+    return a;
 }
 
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -106,13 +110,13 @@ __device__ __forceinline__ Key ld_remote_key(uint32_t at) {
 }
 
 template <bool BF16, bool TOP>
-__global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Rows p, int splits) {
+__global__ void __launch_bounds__(kThreads, 4) rows_kernel(const Rows p, int splits) {
     constexpr int E = BF16 ? 8 : 4;              // logits of a vector
     __shared__ Key waiting[TOP ? kWarps : 1][64];
     __shared__ Key lists[TOP ? kWarps : 1][32];
     __shared__ Sums sums[kWarps];
     __shared__ Sums whole;
-    __shared__ int bar_bits;                     // the bar, as an integer of the same order
+    __shared__ int bar_bits, first_bar;          // the bar, as an integer of the same order; the least of the warps' offers
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const size_t row = blockIdx.x / splits;
     const int split = blockIdx.x % splits;
@@ -123,14 +127,16 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Rows p, int spl
     const int n_vec = (p.vocab + shift + E - 1) / E;
     const int v0 = (int)((long)n_vec * split / splits), v1 = (int)((long)n_vec * (split + 1) / splits);
     if (TOP) {
-        if (tid == 0) bar_bits = 0x80000000;     // below everything
+        if (tid == 0) {
+            bar_bits = 0x80000000;               // below everything
+            first_bar = 0x7FFFFFFF;
+        }
         __syncthreads();
     }
     Sums mine{-INFINITY, 0.0f, 0.0f};
     Key list = 0;                                // this lane's of the warp's best 32
     Key last = 0;                                // the k-th of them
     int n_waiting = 0;
-    float bar = -INFINITY;
     bool first = true;
     auto settle = [&]() {                        // sorts what waits into the list
         __syncwarp();
@@ -142,19 +148,34 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Rows p, int spl
         }
         n_waiting = 0;
         last = __shfl_sync(0xffffffffu, list, p.k - 1);
-        if (last != 0) {
-            const int bits = (int)((uint32_t)(last >> 32) ^ 0x80000000u);
-            if (lane == 0) atomicMax(&bar_bits, bits);
-        }
+        if (last != 0 && lane == 0) atomicMax(&bar_bits, (int)((uint32_t)(last >> 32) ^ 0x80000000u));
         __syncwarp();
     };
+    // Turns ahead lie in shared memory, every thread's own: [kStages][kVectors][kThreads] vectors.  (One that is not the row's alone
+    // is not asked for; its logits are read one by one.)
+    extern __shared__ uint4 ring[];
+    auto ask = [&](int v, int stage) {
+#pragma unroll
+        for (int u = 0; u < kVectors; ++u) {
+            const int at = v + u * kThreads + tid, i = at * E - shift;
+            if (at < v1 && i >= 0 && i + E <= p.vocab)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                 (uint32_t)__cvta_generic_to_shared(ring + (stage * kVectors + u) * kThreads + tid)), "l"(base + (long)i * size) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int stage = 0;
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) ask(v0 + s * kThreads * kVectors, s);
     for (int v = v0; v < v1; v += kThreads * kVectors) {
         float x[kVectors * E];
+        ask(v + (kStages - 1) * kThreads * kVectors, stage == 0 ? kStages - 1 : stage - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
 #pragma unroll
         for (int u = 0; u < kVectors; ++u) {
             const int at = v + u * kThreads + tid, i = at * E - shift;
             if (at < v1 && i >= 0 && i + E <= p.vocab) {
-                const uint4 w = __ldcs(reinterpret_cast<const uint4*>(base + (long)i * size));
+                const uint4 w = ring[(stage * kVectors + u) * kThreads + tid];
                 if constexpr (BF16) {
                     const float2 a = two_bf16(w.x), b = two_bf16(w.y), c = two_bf16(w.z), d = two_bf16(w.w);
                     x[u * E] = a.x; x[u * E + 1] = a.y; x[u * E + 2] = b.x; x[u * E + 3] = b.y;
@@ -169,6 +190,8 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Rows p, int spl
                     x[u * E + j] = at < v1 && i + j >= 0 && i + j < p.vocab ? ld_f(base, (size_t)(i + j), BF16 ? DT_BF16 : DT_F32) : -INFINITY;
             }
         }
+        const uint4* turn = ring + stage * kVectors * kThreads + tid;
+        stage = stage == kStages - 1 ? 0 : stage + 1;
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < kVectors * E; ++j) mx = fmaxf(mx, x[j]);      // (a NaN is dropped)
@@ -194,47 +217,48 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Rows p, int spl
         }
         if (TOP) {
             if (first) {
-                // at least k logits are as large as the k-th of the lanes' largest: the first bar
                 first = false;
-                const Key sorted = sort32(key_of(mx, 0), lane);
-                const Key kth = __shfl_sync(0xffffffffu, sorted, p.k - 1);
-                if (lane == 0) atomicMax(&bar_bits, (int)((uint32_t)(kth >> 32) ^ 0x80000000u));
+                float mine_of_all = mx, offer = warp_max(mx);
+                for (int k = kWarps; k < p.k; k += kWarps) {
+                    const unsigned has = __ballot_sync(0xffffffffu, mine_of_all == offer);
+                    if (lane == __ffs(has) - 1) mine_of_all = -INFINITY;
+                    offer = warp_max(mine_of_all);
+                }
+                if (lane == 0) atomicMin(&first_bar, ordered(offer));
+                __syncthreads();
+                if (lane == 0) atomicMax(&bar_bits, first_bar);
                 __syncwarp();
             }
             const int bits = *reinterpret_cast<volatile int*>(&bar_bits);
-            bar = logit_of((Key)((uint32_t)bits ^ 0x80000000u) << 32);
-            if (!(bar > -INFINITY)) bar = -INFINITY;
-            if (__any_sync(0xffffffffu, mx >= bar)) {
-#pragma unroll 1
-                for (int u = 0; u < kVectors; ++u)
+            const float bar = bits == (int)0x80000000 ? -INFINITY : logit_of((Key)((uint32_t)bits ^ 0x80000000u) << 32);
+            unsigned pass = 0;
+            if (__any_sync(0xffffffffu, mx >= bar))
 #pragma unroll
-                    for (int j = 0; j < E; ++j) {
-                        float c = -INFINITY;
-#pragma unroll
-                        for (int w = 0; w < kVectors; ++w) c = w == u ? x[w * E + j] : c;
-                        const int at = v + u * kThreads + tid, i = at * E - shift + j;
-                        if (c != c) c = -INFINITY;
-                        const bool looks = at < v1 && i >= 0 && i < p.vocab && c >= bar;
-                        if (!__any_sync(0xffffffffu, looks)) continue;
-                        const Key key = key_of(c, i);
-                        const unsigned pass = __ballot_sync(0xffffffffu, looks && key > last);
-                        if (pass == 0) continue;
-                        if (pass >> lane & 1) waiting[warp][n_waiting + __popc(pass & ((1u << lane) - 1))] = key;
-                        n_waiting += __popc(pass);
-                        if (n_waiting >= 32) settle();
-                    }
+                for (int j = 0; j < kVectors * E; ++j) pass |= (x[j] >= bar || bar == -INFINITY ? 1u : 0u) << j;
+            while (__any_sync(0xffffffffu, pass != 0)) {
+                const int j = __ffs(pass) - 1;           // one of each lane's at a time
+                const int at = v + j / E * kThreads + tid, i = at * E - shift + j % E;
+                bool looks = pass != 0 && at < v1 && i >= 0 && i < p.vocab;
+                pass &= pass - 1;
+                Key key = 0;
+                if (looks) {
+                    const int i0 = i - j % E;
+                    float c = i0 >= 0 && i0 + E <= p.vocab ? ld_f(turn + j / E * kThreads, (size_t)(j % E), BF16 ? DT_BF16 : DT_F32)
+                                                           : ld_f(base, (size_t)i, BF16 ? DT_BF16 : DT_F32);
+                    if (c != c) c = -INFINITY;
+                    key = key_of(c, i);
+                    looks = key > last;
+                }
+                const unsigned got = __ballot_sync(0xffffffffu, looks);
+                if (looks) waiting[warp][n_waiting + __popc(got & ((1u << lane) - 1))] = key;
+                n_waiting += __popc(got);
+                if (n_waiting >= 32) settle();
             }
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     // -- the warps of a block, then the blocks of a row
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Sums other;
-        other.m = __shfl_xor_sync(0xffffffffu, mine.m, o);
-        other.s = __shfl_xor_sync(0xffffffffu, mine.s, o);
-        other.e = __shfl_xor_sync(0xffffffffu, mine.e, o);
-        mine = join(mine, other);
-    }
+    mine = join_lanes(mine);
     if (lane == 0) sums[warp] = mine;
     if (TOP) {
         if (n_waiting > 0) settle();
@@ -248,33 +272,22 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Rows p, int spl
         }
     if (warp == 0) {
         Sums a = lane < kWarps ? sums[lane] : Sums{-INFINITY, 0.0f, 0.0f};
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            Sums other;
-            other.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-            other.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-            other.e = __shfl_xor_sync(0xffffffffu, a.e, o);
-            a = join(a, other);
-        }
+        a = join_lanes(a);
         if (lane == 0) whole = a;
     }
     if (splits > 1) {
         cluster_barrier();
-        if (split == 0 && warp < splits && TOP) list = ld_remote_key(remote_of(&lists[0][lane], warp));
+        if (TOP && split == 0) {
+            if (warp < splits) list = ld_remote_key(remote_of(&lists[0][lane], warp));
+            if (warp + kWarps < splits) list = merge32(list, ld_remote_key(remote_of(&lists[0][lane], warp + kWarps)), lane);
+        }
         if (split == 0 && warp == 0) {
             Sums a{-INFINITY, 0.0f, 0.0f};
             if (lane < splits) {
                 const uint32_t at = remote_of(&whole, lane);
                 a = Sums{ld_remote(at), ld_remote(at + 4), ld_remote(at + 8)};
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                Sums other;
-                other.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-                other.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-                other.e = __shfl_xor_sync(0xffffffffu, a.e, o);
-                a = join(a, other);
-            }
+            a = join_lanes(a);
             if (lane == 0) sums[0] = a;
         }
         cluster_barrier();          // what other blocks left has been read
@@ -282,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Rows p, int spl
         if (TOP && warp < splits) lists[warp][lane] = list;
         __syncthreads();
         if (TOP)
-            for (int half = splits / 2; half > 0; half >>= 1) {
+            for (int half = min(splits, kWarps) / 2; half > 0; half >>= 1) {
                 if (warp < half) lists[warp][lane] = merge32(lists[warp][lane], lists[warp + half][lane], lane);
                 __syncthreads();
             }
@@ -309,10 +322,13 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const Rows p, int spl
 
 }  // namespace
 
-// Blocks that share a row: enough for the device, each with a few turns of its threads.
+// Blocks that share a row.  Few rows: as many as give the device's SMs two blocks each (8 rows of 151 936, best 5: 1 block 33 us, 4 16.5,
+// 8 or 16 12.4).  A few hundred: one, because a cluster's own cost is that of some 10 000 logits (300 rows of 50 257, best 20: 1
+// block 30.8 us, 2 31.5, 4 36.4).  Many long rows: two, which end together more nearly (1 001 rows of 151 936: 1 block 102 us, 2 98.8, 4 107).
 static int splits_of(int n, int vocab) {
+    if (n >= 5L * sm_count()) return vocab >= 1 << 16 ? 2 : 1;
     int s = 1;
-    while (s < kMaxSplits && (long)n * s < 4L * sm_count() && vocab / (2 * s) >= 4 * kThreads) s *= 2;
+    while (s < kMaxSplits && 2L * n * s <= 2L * sm_count() && vocab / (2 * s) >= 4 * kThreads) s *= 2;
     return s;
 }
 
@@ -327,6 +343,8 @@ extern "C" int nncpu_token_logprobs(const void* logits, int dt, const int* targe
     static bool done[4][64];
     if (first_use_on_this_device(done[(dt == DT_BF16 ? 2 : 0) + (k ? 1 : 0)])) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        const cudaError_t e2 = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
+        NN_CHECK(e2 == cudaSuccess, "token_logprobs: shared memory: %s", cudaGetErrorString(e2));
         NN_CHECK(e == cudaSuccess, "token_logprobs: clusters of %d: %s", kMaxSplits, cudaGetErrorString(e));
     }
     const int splits = splits_of(n, vocab);
@@ -334,6 +352,7 @@ extern "C" int nncpu_token_logprobs(const void* logits, int dt, const int* targe
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(n * splits));
     cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kRing;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
