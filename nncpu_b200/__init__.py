@@ -10,12 +10,12 @@ from .errors import (BadFormat, Cancelled, ContextFull, ExtensionError, InvalidA
                      UnsupportedModel)
 from .engine import Engine, Model
 from .perf import perf_enable, perf_report, perf_reset, perf_span_ms, perf_totals
-from .sampling import GenerateParams, GenerateResult, SamplerParams, StopReason
+from .sampling import GenerateParams, GenerateResult, SamplerParams, ScoreResult, StopReason, TokenLogprob
 from .session import CancelHandle, Piece, Session, SessionParams
 
 __version__ = "0.1.0"
 
 __all__ = ["BadFormat", "Cancelled", "ContextFull", "ExtensionError", "InvalidArgument", "NncpuError",
            "OutOfMemory", "UnsupportedModel", "Engine", "Model", "GenerateParams", "GenerateResult", "SamplerParams",
-           "StopReason", "CancelHandle", "Piece", "Session", "SessionParams", "perf_enable", "perf_report", "perf_reset",
+           "ScoreResult", "StopReason", "TokenLogprob", "CancelHandle", "Piece", "Session", "SessionParams", "perf_enable", "perf_report", "perf_reset",
            "perf_span_ms", "perf_totals", "__version__"]

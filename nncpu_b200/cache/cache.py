@@ -33,10 +33,16 @@ from ..errors import ContextFull, InvalidArgument, translating_oom
 from .slots import IndexPool
 
 PAGE = 64  # tokens per page; also the unit in which a request's tokens are counted
+Q4_GROUP = 32  # lanes of a head that share a step and a least value in a cache of 4 bits
 
 
 def pages_for(n_tokens: int) -> int:
     return (n_tokens + PAGE - 1) // PAGE
+
+
+def q4_page_bytes(head_dim: int) -> int:
+    """Bytes of a page's keys (or values) of one head in 4 bits: a code a lane and two float16 numbers a group of lanes."""
+    return PAGE * (head_dim // 2 + head_dim // Q4_GROUP * 4)
 
 
 @dataclass(frozen=True)
@@ -67,14 +73,18 @@ class StateRequest:
 class KVGroup:
     """Storage and page bookkeeping of the entries that share one KVRequest."""
 
-    def __init__(self, request: KVRequest, entries: List[int], n_pages: int, dtype, device):
+    def __init__(self, request: KVRequest, entries: List[int], n_pages: int, dtype, device, q4: bool = False):
+        """``q4``: pages are uint8 [entries, n_pages, heads, ``q4_page_bytes``] (the layout is the kernels' business)."""
         self.request = request
         self.entries = list(entries)
         self.n_pages = n_pages
         shape = (len(entries), n_pages, request.n_kv_heads, PAGE)
-        self.k = torch.zeros(shape + (request.head_dim,), dtype=dtype, device=device)
-        self.v = self.k if request.keys_only else torch.zeros(shape + (request.v_head_dim or request.head_dim,),
-                                                              dtype=dtype, device=device)
+        rows = (request.head_dim,), (request.v_head_dim or request.head_dim,)
+        if q4:
+            shape, dtype = shape[:-1], torch.uint8
+            rows = tuple((q4_page_bytes(r[0]),) for r in rows)
+        self.k = torch.zeros(shape + rows[0], dtype=dtype, device=device)
+        self.v = self.k if request.keys_only else torch.zeros(shape + rows[1], dtype=dtype, device=device)
         self.pool = IndexPool(n_pages, "cache page")
         self.tables: Dict[int, List[int]] = {}  # slot -> page ids by page index, -1 = given back
 
@@ -123,14 +133,15 @@ class Cache:
     whose keys and values entry ``i`` reads instead of its own, or None.
 
     ``max_tokens`` is the most tokens the live sequences hold at any time, each
-    sequence's count rounded up to a multiple of ``PAGE``."""
+    sequence's count rounded up to a multiple of ``PAGE``.  ``q4``: keys and values are kept in 4 bits (``dtype`` then
+    says what the model runs in)."""
 
     def __init__(self, requests: Sequence[Tuple[Optional[KVRequest], Optional[StateRequest]]],
                  cache_of: Sequence[Optional[int]], max_tokens: int, dtype: torch.dtype, device,
-                 n_slots: Optional[int] = None, max_seq_len: Optional[int] = None):
+                 n_slots: Optional[int] = None, max_seq_len: Optional[int] = None, q4: bool = False):
         if max_tokens < 1:
             raise InvalidArgument(f"a cache for {max_tokens} tokens")
-        self.dtype, self.device = dtype, torch.device(device)
+        self.dtype, self.device, self.q4 = dtype, torch.device(device), q4
         self.n_pages = pages_for(max_tokens)
         self.max_tokens = self.n_pages * PAGE
         self.max_seq_len = min(max_seq_len or self.max_tokens, self.max_tokens)
@@ -155,13 +166,13 @@ class Cache:
                 by_request.setdefault(kv, []).append(i)
         esize = torch.empty((), dtype=dtype).element_size()
         need = sum(len(e) * self.n_pages * kv.n_kv_heads * PAGE
-                   * (kv.head_dim + (0 if kv.keys_only else kv.v_head_dim or kv.head_dim)) * esize
+                   * (kv.head_dim + (0 if kv.keys_only else kv.v_head_dim or kv.head_dim)) * (5 / 8 if q4 else esize)
                    for kv, e in by_request.items())
         for kv, entries in by_request.items():
             g = len(self.groups)
             with translating_oom(f"a cache of {self.max_tokens} tokens ({need / 2 ** 30:.2f} GiB of keys and values "
                                  f"for {sum(len(e) for e in by_request.values())} layer runs)"):
-                self.groups.append(KVGroup(kv, entries, self.n_pages, dtype, self.device))
+                self.groups.append(KVGroup(kv, entries, self.n_pages, dtype, self.device, q4))
             for k, e in enumerate(entries):
                 self._entry_group[e] = (g, k)
                 self._owns[e] = True
@@ -285,7 +296,8 @@ class Cache:
         return self._owns[entry]
 
     def kv(self, entry: int):
-        """(keys, values) of schedule entry ``entry``: [n_pages, n_kv_heads, PAGE, head_dim]."""
+        """(keys, values) of schedule entry ``entry``: [n_pages, n_kv_heads, PAGE, head_dim], or in 4 bits uint8
+        [n_pages, n_kv_heads, ``q4_page_bytes``]."""
         g, k = self._entry_group[entry]
         return self.groups[g].k[k], self.groups[g].v[k]
 

@@ -23,11 +23,11 @@ from typing import List, Optional
 
 from . import __version__
 from .errors import InvalidArgument, NncpuError
-from .sampling import GenerateParams, SamplerParams
+from .sampling import GenerateParams, SamplerParams, ScoreResult, TokenLogprob
 
 # flag, fewest and most positional arguments (crates/nncpu-cli/src/cli.rs:78-95)
 MODES = {"--help": (0, 0), "-h": (0, 0), "--version": (0, 0), "--gen": (2, 4), "--info": (1, 1),
-         "--random-weights": (3, 3)}
+         "--random-weights": (3, 3), "--perplexity": (2, 2)}
 
 VALUE_OPTIONS = {
     "-m": "model", "--model": "model",
@@ -43,8 +43,10 @@ VALUE_OPTIONS = {
     "-s": "seed", "--seed": "seed",
     "-b": "batch", "--batch": "batch", "--batch_size": "batch",
     "--dtype": "dtype",
+    "--logprobs": "logprobs",
 }
 FLAGS = {"--bf16": ("dtype", "bfloat16"), "--fp32": ("dtype", "float32"), "--kv-f32": ("kv_f32", True),
+         "--kv-q4": ("kv_q4", True),
          "--perf": ("perf", True), "-v": ("verbose", True), "--verbose": ("verbose", True)}
 
 
@@ -66,11 +68,16 @@ class Options:
     batch: int = 1              # -b: copies of the prompt generated together
     dtype: str = "bfloat16"
     kv_f32: bool = False
+    kv_q4: bool = False
+    logprobs: Optional[int] = None
     perf: bool = False
     verbose: bool = False
 
     def sampler(self) -> SamplerParams:
         return SamplerParams(self.temperature, self.top_k, self.top_p, self.min_p)
+
+    def generate_params(self) -> GenerateParams:
+        return GenerateParams(self.n_predict, self.sampler(), self.logprobs)
 
 
 def _number(flag: str, text: str, kind):
@@ -103,7 +110,7 @@ def parse_options(argv: List[str]) -> Options:
                 raise InvalidArgument(f"{a} needs a value")
             i += 1
             name, text = VALUE_OPTIONS[a], argv[i]
-            if name in ("n_predict", "n_ctx", "top_k", "seed", "batch"):
+            if name in ("n_predict", "n_ctx", "top_k", "seed", "batch", "logprobs"):
                 v = _number(a, text, int)
                 if v < 0 and name != "seed":
                     raise InvalidArgument(f"{a}: {v} is negative")
@@ -126,7 +133,9 @@ def parse_options(argv: List[str]) -> Options:
         else:
             raise InvalidArgument(f"unknown option {a!r} (see --help)")
         i += 1
-    o.sampler().check("options")
+    o.generate_params().check("options")
+    if o.kv_f32 and o.kv_q4:
+        raise InvalidArgument("--kv-f32 and --kv-q4 exclude one another")
     return o
 
 
@@ -144,6 +153,7 @@ model:
   --dtype NAME             bfloat16 or float32
   -c, --ctx-size N         context window in tokens (default: up to 4096)
   --kv-f32                 keep the K/V cache in F32 (default: the run's element type)
+  --kv-q4                  keep the K/V cache in 4 bits (3.2 times smaller than bfloat16)
 
 generation:
   -p, --prompt TEXT        answer TEXT and exit; the reply goes to stdout as it is written
@@ -155,6 +165,8 @@ generation:
   --top-k N                sample from the N likeliest tokens; 0 = all (default 40)
   --top-p X                ...that make up probability X (default 0.95)
   --min-p X                ...each at least X times the likeliest (default 0.05)
+  --logprobs N             after the reply, every token's log probability, the entropy of the model's prediction and its N
+                           likeliest tokens (N up to 32), a line of JSON each, on stderr
   -s, --seed N             random seed, for repeatable replies (default: random)
   --perf                   print a table of the time per phase after the reply
   -v, --verbose            show what the library is doing
@@ -162,6 +174,7 @@ generation:
 modes (each runs instead of generation):
   --gen DIR "ID ID ..." [N] [CTX]
                            greedy token-level run: prints every token and the prefill and decode speeds
+  --perplexity DIR FILE    how well the model predicts FILE (token ids, or text if DIR has a tokenizer.json)
   --info DIR               the model folder's configuration, sizes and parameter count
   --random-weights CONFIG.json SEED OUT
                            write OUT/config.json and OUT/model.safetensors with random weights
@@ -216,6 +229,10 @@ def _stats_line(res, verbose: bool, n_predict: int) -> str:
     return f"[{res.n_generated} tokens, {tps:.1f} tok/s{note}]"
 
 
+def _logprob_line(t) -> str:
+    return json.dumps({"token": t.token, "logprob": t.logprob, "entropy": t.entropy, "top": [list(x) for x in t.top]})
+
+
 def run_generate(o: Options, out=sys.stdout, err=sys.stderr) -> int:
     from . import Model, Session, SessionParams
     from .text import load_tokenizer
@@ -228,10 +245,10 @@ def run_generate(o: Options, out=sys.stdout, err=sys.stderr) -> int:
     model = Model.load(o.model, dtype=o.dtype)
     if o.verbose:
         print(f"loaded {model.info()} in {time.perf_counter() - t0:.2f} s", file=err)
-    session = Session(model, SessionParams(n_ctx=o.n_ctx, seed=o.seed, kv_f32=o.kv_f32, max_batch=o.batch,
+    session = Session(model, SessionParams(n_ctx=o.n_ctx, seed=o.seed, kv_f32=o.kv_f32, kv_q4=o.kv_q4, max_batch=o.batch,
                                            system_prompt=o.system_prompt), tokenizer=tok)
     _perf_begin(o)
-    params = GenerateParams(o.n_predict, o.sampler())
+    params = o.generate_params()
     if tok is not None:
         # one chat turn on the session's own sequence, streamed in whole characters
         def on_text(p):
@@ -249,6 +266,9 @@ def run_generate(o: Options, out=sys.stdout, err=sys.stderr) -> int:
         res = session.generate([_token_list(o.tokens)] * o.batch, params, on_piece)
     out.write("\n")
     out.flush()
+    for r in res:
+        for t in r.logprobs or ():
+            print(_logprob_line(t), file=err)
     if o.perf or o.verbose:
         r = res[0]
         n = sum(x.n_generated for x in res)
@@ -289,7 +309,7 @@ def chat_loop(session, o: Options, lines, out=sys.stdout, err=sys.stderr, intera
     the session's cancel handle while a reply is written.  A conversation that has filled the context starts
     afresh and the message is tried again (crates/nncpu-cli/src/chat.rs:138-166,302-484)."""
     from .errors import ContextFull
-    params = GenerateParams(o.n_predict, o.sampler())
+    params = o.generate_params()
     cancel = session.cancel_handle()
 
     def turn(message):
@@ -355,7 +375,7 @@ def run_chat(o: Options, stdin=None, out=sys.stdout, err=sys.stderr) -> int:
         raise InvalidArgument("no model: pass -m DIR")
     tok = load_tokenizer(o.model)
     model = Model.load(o.model, dtype=o.dtype)
-    session = Session(model, SessionParams(n_ctx=o.n_ctx, seed=o.seed, kv_f32=o.kv_f32, max_batch=1,
+    session = Session(model, SessionParams(n_ctx=o.n_ctx, seed=o.seed, kv_f32=o.kv_f32, kv_q4=o.kv_q4, max_batch=1,
                                            system_prompt=o.system_prompt), tokenizer=tok)
     info = model.info()
     print(f"{o.model} ({info['architecture']}, {info['layers']} layers, {info['dtype']}) - "
@@ -372,7 +392,7 @@ def run_gen(o: Options, out=sys.stdout) -> int:
     n = int(o.args[2]) if len(o.args) > 2 else 32
     ctx = int(o.args[3]) if len(o.args) > 3 else max(256, len(ids) + n + 1)
     model = Model.load(folder, dtype=o.dtype)
-    session = Session(model, SessionParams(n_ctx=ctx, seed=1, kv_f32=o.kv_f32, max_batch=1))
+    session = Session(model, SessionParams(n_ctx=ctx, seed=1, kv_f32=o.kv_f32, kv_q4=o.kv_q4, max_batch=1))
     _perf_begin(o)
     res = session.generate([ids], GenerateParams(n, SamplerParams.greedy()))[0]
     out.write(" ".join(str(t) for t in res.tokens) + "\n")
@@ -380,6 +400,40 @@ def run_gen(o: Options, out=sys.stdout) -> int:
     out.write(f"decode: {res.n_generated} tokens, {res.decode * 1e3:.1f} ms ({res.n_generated / max(res.decode, 1e-9):.1f} tok/s)\n")
     out.write(f"stop: {res.stop.value}\n")
     _perf_end(o, "gen", res.n_prompt + res.n_generated, out)
+    return 0
+
+
+def run_perplexity(o: Options, out=sys.stdout, err=sys.stderr) -> int:
+    """How well the model predicts a file: token ids, or text where the folder has a tokenizer.  A file longer than the
+    context is scored in stretches of the context's length, each by itself (crates/nncpu-cli/src/devtools.rs:711-767)."""
+    from . import Model, Session, SessionParams
+    from .text import load_tokenizer
+    folder, path = o.args[0], Path(o.args[1])
+    try:
+        text = path.read_text()
+    except (OSError, UnicodeDecodeError) as e:
+        raise InvalidArgument(f"{path}: {e}") from None
+    words = text.replace(",", " ").split()
+    ids = [int(t) for t in words] if all(t.isdigit() for t in words) else load_tokenizer(folder).encode(text)
+    if len(ids) < 2:
+        raise InvalidArgument(f"{path}: {len(ids)} tokens, a prediction takes two")
+    model = Model.load(folder, dtype=o.dtype)
+    session = Session(model, SessionParams(n_ctx=o.n_ctx, seed=1, kv_f32=o.kv_f32, kv_q4=o.kv_q4, max_batch=1))
+    _perf_begin(o)
+    n, total, k = 0, 0.0, o.logprobs or 0
+    t0 = time.perf_counter()
+    for at in range(0, len(ids), session.n_ctx):
+        part = ids[at:at + session.n_ctx]
+        r = session.score([part], k)[0]
+        n, total = n + len(r.tokens), total + r.logprob
+        if o.logprobs is not None:
+            for t in r.tokens:
+                print(_logprob_line(t), file=err)
+    dt = time.perf_counter() - t0
+    mean = ScoreResult([TokenLogprob(0, total / n, 0.0)])
+    out.write(f"{n} predictions of {len(ids)} tokens: {total / n:.6f} nats a token, perplexity {mean.perplexity:.4f} "
+              f"({len(ids) / max(dt, 1e-9):.1f} tok/s)\n")
+    _perf_end(o, "perplexity", len(ids), out)
     return 0
 
 
@@ -436,6 +490,8 @@ def main(argv: Optional[List[str]] = None) -> int:
             return run_gen(o)
         if o.mode == "chat":
             return run_chat(o)
+        if o.mode == "perplexity":
+            return run_perplexity(o)
         if o.mode == "info":
             return run_info(o)
         if o.mode == "random-weights":

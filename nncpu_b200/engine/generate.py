@@ -40,6 +40,7 @@ from typing import Callable, List, Optional, Sequence
 
 from ..cache import PAGE, pages_for
 from ..errors import ContextFull, InvalidArgument
+from ..sampling.logprobs import Logprobs
 from ..sampling.params import GenerateParams, GenerateResult, StopReason
 
 
@@ -72,7 +73,8 @@ def generate(engine, chooser, prompts: Sequence[Sequence[int]], params: Generate
     called for every generated token and may return False to stop that
     sequence; ``on_finish(index)`` is called once when a sequence has stopped.
     ``run_ahead`` False keeps every step behind the host's decisions (the
-    tokens are the same either way).  Results come in the order of the prompts."""
+    tokens are the same either way).  Results come in the order of the prompts.  With ``params.logprobs`` every step's logits are
+    asked about the chosen tokens right after the choice; the answers are fetched once, when the batch is done."""
     n_ctx = n_ctx or engine.max_seq_len
     stops = frozenset(int(t) for t in stop_token_ids)
     if not prompts:
@@ -125,10 +127,18 @@ def _run_batch(engine, chooser, members, params, stops, on_token, cancelled, n_c
                  and (getattr(chooser, "chooses_on_device", False) or getattr(chooser, "greedy_on_device", False))
                  and all(hasattr(engine, a) for a in ("choice_buffer", "fetch_choices", "step_again")))
 
-    def settle(rows, chosen):
-        """Takes one chosen token per sequence of ``rows``; returns the sequences that go on."""
+    # what the steps' logits say about the tokens, row by row, and which of the rows belong to a sequence's tokens
+    logprobs = None if params.logprobs is None else Logprobs(params.logprobs, engine.vocab_size)
+    kept = {idx: [] for idx, _ in members}
+
+    def score(logits, tokens) -> int:
+        return 0 if logprobs is None else logprobs.add(logits, tokens)
+
+    def settle(rows, chosen, first, at=None):
+        """Takes one chosen token per sequence of ``rows``; returns the sequences that go on.  ``first``: the number of the
+        step's first row of log probabilities, ``at`` the rows' places in the step (None: in order)."""
         still = []
-        for (idx, slot, toks, r), tok in zip(rows, chosen):
+        for k, ((idx, slot, toks, r), tok) in enumerate(zip(rows, chosen)):
             tok = int(tok)
             toks.append(tok)
             if tok in stops:
@@ -136,6 +146,7 @@ def _run_batch(engine, chooser, members, params, stops, on_token, cancelled, n_c
             else:
                 r.n_generated += 1
                 r.tokens.append(tok)
+                kept[idx].append(first + (k if at is None else at[k]))
                 if on_token is not None and on_token(idx, tok) is False:
                     r.stop = StopReason.CALLBACK
                 elif len(toks) >= n_ctx:
@@ -177,6 +188,7 @@ def _run_batch(engine, chooser, members, params, stops, on_token, cancelled, n_c
                 # sequence with this very token, launch the next step on top of them.
                 if not getattr(chooser, "greedy_on_device", False):
                     chooser.enqueue(logits, [idx for idx, _, _, _ in live], buffer)
+                row = score(logits, buffer)
                 event, ids = engine.fetch_choices(len(live))
                 if all(len(toks) + 2 <= n_ctx and (params.max_tokens <= 0 or r.n_generated + 2 <= params.max_tokens)
                        for _, _, toks, r in live):
@@ -185,11 +197,12 @@ def _run_batch(engine, chooser, members, params, stops, on_token, cancelled, n_c
                 chosen = ids[:len(live)].tolist()
             else:
                 chosen = chooser.choose(logits, [idx for idx, _, _, _ in live])
+                row = score(logits, chosen)
             check_status()      # the device has been waited for: did every kernel of the step finish its work?
             if prefill is None:  # the first choice waits for the prompt step to finish
                 t1 = time.perf_counter()
                 prefill = t1 - t0
-            still = settle(live, chosen)
+            still = settle(live, chosen, row)
             if ahead is not None and len(still) == len(live):
                 live, logits = still, ahead     # nobody stopped: the step run ahead is the step in flight
                 continue
@@ -201,10 +214,11 @@ def _run_batch(engine, chooser, members, params, stops, on_token, cancelled, n_c
                 rows = [k for k, m in enumerate(live) if m[0] in going_on]
                 if not getattr(chooser, "greedy_on_device", False):
                     chooser.enqueue(ahead, [m[0] for m in live], engine.choice_buffer(len(live)))
+                row = score(ahead, engine.choice_buffer(len(live))) if logprobs is not None else 0
                 event, ids = engine.fetch_choices(len(live))
                 event.synchronize()
                 check_status()
-                still = settle(still, [int(ids[k]) for k in rows])
+                still = settle(still, [int(ids[k]) for k in rows], row, rows)
             live = still
             if live:
                 logits = engine.step([s for _, s, _, _ in live], [[t[-1]] for _, _, t, _ in live])
@@ -212,6 +226,10 @@ def _run_batch(engine, chooser, members, params, stops, on_token, cancelled, n_c
         for r in done_results:
             r.prefill = prefill if prefill is not None else t2 - t0
             r.decode = t2 - t1
+        if logprobs is not None:
+            found = logprobs.read()
+            for (idx, _), r in zip(members, done_results):
+                r.logprobs = [found[k] for k in kept[idx]]
         for (idx, _), r in zip(members, done_results):
             results[idx] = r
     finally:

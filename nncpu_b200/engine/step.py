@@ -17,8 +17,9 @@ import numpy as np
 import torch
 
 from .. import perf
-from ..cache import Cache, pages_for
-from ..errors import InvalidArgument, translating_oom
+from ..cache import Cache, PAGE, pages_for
+from ..cache.cache import Q4_GROUP
+from ..errors import InvalidArgument, UnsupportedModel, translating_oom
 from ..kernels import ops
 from ..parts import EntryCache
 from ..parts.runtime import Arena
@@ -173,10 +174,13 @@ class Engine:
     model's forward over the shapes of the largest expected step (``max_step_tokens`` tokens, by default the
     cache's capacity up to 8 192): a step asks the allocator for nothing.  A step that turns out larger (more
     tokens, or many rows of logits wanted) is served by the allocator once, and the arena is as large from then on
-    (the reference sizes its scratch once, crates/nncpu/src/model/kv.rs:295-332)."""
+    (the reference sizes its scratch once, crates/nncpu/src/model/kv.rs:295-332).
+
+    ``kv_dtype``: what keys and values are kept in, a torch type or ``"q4"`` (4 bits a lane, and two float16 numbers for every 32
+    lanes: ``ops.qk_norm_rope_append_q4``), for models whose mixers all take that; None: the run's own type."""
 
     def __init__(self, model, max_tokens: int, n_slots: Optional[int] = None, max_seq_len: Optional[int] = None,
-                 kv_dtype: Optional[torch.dtype] = None, use_graphs: bool = True,
+                 kv_dtype=None, use_graphs: bool = True,
                  max_step_tokens: Optional[int] = None):
         from .decode_graph import PROMPT_GRAPH_MAX, DecodeGraphs
         self._prompt_graph_max = PROMPT_GRAPH_MAX
@@ -193,8 +197,16 @@ class Engine:
         # A table of learned position vectors is the exception: a sequence cannot outgrow it.
         if model.pos_table is not None:
             max_seq_len = min(max_seq_len or model.pos_table.shape[0], model.pos_table.shape[0])
-        self.cache = Cache(requests, cache_of, max_tokens, kv_dtype or rt.dtype, rt.device, n_slots=n_slots,
-                           max_seq_len=max_seq_len)
+        q4 = isinstance(kv_dtype, str)
+        if q4:
+            if kv_dtype != "q4":
+                raise InvalidArgument(f"a cache of {kv_dtype!r}: a torch type or 'q4'")
+            wrong = sorted({m.spec.kind for b in model.blocks for m in b.mixers() if not m.takes_q4()})
+            if wrong:
+                raise UnsupportedModel(f"{model.spec.architecture}: a cache of 4 bits holds grouped-query attention with heads of whole "
+                                       f"groups of {Q4_GROUP} lanes, keys and values apart (mixers here that are not: {', '.join(wrong)})")
+        self.cache = Cache(requests, cache_of, max_tokens, rt.dtype if q4 or kv_dtype is None else kv_dtype, rt.device, n_slots=n_slots,
+                           max_seq_len=max_seq_len, q4=q4)
         self.vocab_size = model.spec.vocab_size
         self.arena = Arena(rt.device)
         self.max_step_tokens = min(max_step_tokens or 8192, self.cache.max_tokens)
@@ -234,6 +246,25 @@ class Engine:
 
     def free_slot(self, slot: int) -> None:
         self.cache.free_slot(slot)
+
+    def cached(self, slot: int, user: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+        """What the cache holds of the sequence in ``slot``, as numbers: keys and values, float32 [length, n_kv_heads, head_dim] on the
+        device, of cache user ``user`` (the mixers that keep or read keys and values, in the order of the schedule).  Positions that a window has given back
+        are zeros."""
+        n, g = self.cache.length(slot), self.cache.group_of(user)
+        if g is None:
+            raise InvalidArgument(f"cache user {user} keeps no keys and values")
+        k, v = self.cache.kv(user)
+        table = torch.tensor(self.cache.block_table(g, [slot]), dtype=torch.int32, device=self.cache.device)
+        pos = torch.arange(n, dtype=torch.int32, device=self.cache.device)
+        if not self.cache.q4:
+            page = table[0, pos.long() // PAGE].long()
+            there = (page >= 0)[:, None, None]
+            return tuple(torch.where(there, t[page.clamp(min=0), :, pos.long() % PAGE].float(), 0.0) for t in (k, v))
+        heads = k.shape[1]
+        out = [torch.empty(n, heads * self.cache.groups[g].request.head_dim, device=self.cache.device) for _ in range(2)]
+        ops.q4_read(k, v, table, torch.zeros_like(pos), pos, *out)
+        return tuple(t.view(n, heads, -1) for t in out)
 
     # -- the step ----------------------------------------------------------------
 

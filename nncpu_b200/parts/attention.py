@@ -31,6 +31,9 @@ inside the attention kernel.
 the projection, so the value is the convolved key; the last n - 1 projections of a sequence are its state, 32-bit, in the
 cache's state area.  Convolution, per-head norm, rotation (neighbouring lanes) and append are one kernel in a prompt step
 (``ops.qk_conv_norm_append``) and the attention kernel's own first steps in a decode step; both leave the state advanced.
+A cache of 4 bits (``takes_q4`` says for which options): norm, rotation and append are one kernel that cuts keys and values to 4
+bits, decode steps attend straight from the codes and prompts take them out once (``_forward_q4``).
+
 ``score_cap`` c: a scaled score z becomes c tanh(z / c), 32-bit, inside every attention kernel.  ``head_gate``: one gate
 logit per head, whose rows ride in the projection's product; the attention kernels apply the sigmoid where they divide by
 the softmax's sum.
@@ -117,6 +120,10 @@ class Attention(Mixer):
             return None
         return StateRequest((ops.conv_state_floats(self.spec.conv, self.q_size + self.kv_size),), torch.float32)
 
+    def takes_q4(self) -> bool:
+        s = self.spec
+        return (not (self.apart or self.convolved or s.values_are_keys or self.v_dim != s.head_dim) and ops.q4_supported(s.head_dim))
+
     def _proj_names(self):
         if self.shared_kv:
             return ["q_proj"]
@@ -194,12 +201,46 @@ class Attention(Mixer):
     def weight_bytes(self):
         return sum(t.numel() * t.element_size() for t in (self.w_qkv, self.w_o))
 
+    def _forward_q4(self, ctx, x, cache, attn, eps):
+        """Projections, append and attention with keys and values in 4 bits."""
+        s, rt = self.spec, self.rt
+        n = x.shape[0]
+        qkv = rt.empty(n, self.q_size + self.kv_size + self.v_size + self.gate_size, dtype=torch.float32)
+        with rt.phase("attn_qkv", self.w_qkv, n):
+            rt.linear(x, self.w_qkv, self.b_qkv, qkv)
+        q = rt.empty(n, self.q_size)
+        with rt.phase("attn_rope"):
+            cos_sin = None if self.position is None else self.position.tables(ctx)
+            ops.qk_norm_rope_append_q4(qkv, self.q_gamma, self.k_gamma, eps, cos_sin, ctx.tok_seq, ctx.tok_pos, cache.block_table,
+                                       cache.k_pages, cache.v_pages, q, s.n_heads, 0 if self.shared_kv else s.n_kv_heads, s.head_dim,
+                                       self.q_temp)
+        options = dict(window=self.span, slope_base=s.slope_base, sinks=self.sinks, keep=s.keep_first, cap=s.score_cap,
+                       head_gate=(qkv, self.gate_col) if s.head_gate else None)
+        sizes = (s.n_heads, s.n_kv_heads, s.head_dim)
+        with self._core_phase(ctx, cache):
+            if ctx.is_decode:
+                longest = self._longest_span(ctx) + 128 if self.span else ctx.max_kv_len
+                floats = ops.attention_q4_scratch_floats(n, *sizes, rt.dtype, longest)
+                scratch = rt.empty(floats, dtype=torch.float32) if floats else None
+                ops.attention_q4(q, cache.k_pages, cache.v_pages, cache.block_table, ctx.tok_seq, ctx.tok_pos, attn, *sizes, s.scale,
+                                 longest=longest, scratch=scratch, **options)
+            else:
+                need = ops.attention_q4_prompt_scratch_bytes(n, ctx.n_seqs, *sizes, rt.dtype, ctx.max_kv_len, s.slope_base, s.score_cap)
+                scratch = rt.empty(need, dtype=torch.uint8) if need else None
+                ops.attention_q4_prompt(q, cache.k_pages, cache.v_pages, cache.block_table, ctx.cu_seqlens, ctx.tok_seq, ctx.tok_pos, attn,
+                                        ctx.n_seqs, *sizes, s.scale, ctx.max_kv_len, rt.workspace.status, scratch=scratch, **options)
+        if s.out_gate:
+            with rt.phase("attn_gate"):
+                ops.sigmoid_gate(attn, qkv, self.gate_col)
+
     def forward(self, ctx, x, residual, cache):
         s, rt = self.spec, self.rt
         n = x.shape[0]
         eps = s.qk_norm.eps if s.qk_norm else 0.0
         attn = rt.empty(n, self.out_size)
-        if self._fused_qkv(x, cache):
+        if cache.k_pages.dtype == torch.uint8:
+            self._forward_q4(ctx, x, cache, attn, eps)
+        elif self._fused_qkv(x, cache):
             # a prompt: norm, rotation and the cache append happen in the projection's epilogue, on its
             # float32 accumulators; its threads are tokens, so the rotation table is laid out by pair
             q = rt.empty(n, self.q_size)
@@ -269,7 +310,8 @@ class Attention(Mixer):
             return perf._NULL
         s = self.spec
         keys = ctx.span_sum(s.window, s.chunk, s.keep_first)
-        return self.rt.phase("attn_core", nbytes=1.0 * keys * s.n_kv_heads * (s.head_dim + self.v_dim) * cache.k_pages.element_size(),
+        lane = 5 / 8 if cache.k_pages.dtype == torch.uint8 else cache.k_pages.element_size()
+        return self.rt.phase("attn_core", nbytes=1.0 * keys * s.n_kv_heads * (s.head_dim + self.v_dim) * lane,
                              flops=2.0 * keys * (self.q_size + self.out_size))
 
     def _decode_from_projections(self, ctx, cache) -> bool:

@@ -144,7 +144,7 @@ class PositionEncoding(Part):
 @dataclass
 class EntryCache:
     """What one schedule entry sees of the cache during a step."""
-    k_pages: Optional[torch.Tensor]      # [n_pages, n_kv_heads, PAGE, head_dim] or None
+    k_pages: Optional[torch.Tensor]      # [n_pages, n_kv_heads, PAGE, head_dim] (in 4 bits: uint8 pages) or None
     v_pages: Optional[torch.Tensor]
     block_table: Optional[torch.Tensor]  # int32 [n_seqs, width]: page ids of the step's sequences
     owns_kv: bool                        # False: the pages belong to another entry; read, do not append
@@ -159,6 +159,10 @@ class Mixer(Part):
 
     def state_request(self) -> Optional[StateRequest]:
         return None
+
+    def takes_q4(self) -> bool:
+        """Whether this mixer can work on a cache of 4 bits (one without keys and values has nothing there)."""
+        return self.kv_request() is None
 
     def forward(self, ctx, x: torch.Tensor, residual: torch.Tensor, cache: EntryCache) -> None:
         raise NotImplementedError
@@ -175,6 +179,13 @@ class Block(Part):
     def entry_norm_request(self, ctx, residual: torch.Tensor) -> Optional[NormRequest]:
         """The request of the norm this block begins with, for the block before it to fulfil (None: none)."""
         return None
+
+    def mixers(self) -> List["Mixer"]:
+        """The mixers this block is made of."""
+        parts = []
+        for v in vars(self).values():
+            parts += v if isinstance(v, (list, tuple)) else [v]
+        return [p for i, p in enumerate(parts) if isinstance(p, Mixer) and not any(p is q for q in parts[:i])]
 
     def cache_requests(self) -> List[tuple]:
         """One (KVRequest or None, StateRequest or None) pair per mixer of the block, in the order in which

@@ -30,8 +30,13 @@ from .cache import PAGE
 from .engine.generate import generate as _generate, generate_on_slot as _generate_on_slot
 from .engine.step import Engine
 from .errors import ContextFull, InvalidArgument, NncpuError
-from .sampling import GenerateParams, GenerateResult, Sampler, SamplerParams
+from .sampling import GenerateParams, GenerateResult, Sampler, SamplerParams, ScoreResult
+from .sampling.logprobs import Logprobs
+from .sampling.params import check_alternatives
 from .text import TextStream, chat_turn, end_token_ids
+
+
+SCORE_TOKENS = 256     # tokens of a text that one step of ``Session.score`` brings
 
 
 @dataclass(frozen=True)
@@ -40,6 +45,8 @@ class SessionParams:
     (crates/nncpu/src/session/engine.rs:113-117); ``seed`` 0 = random
     (crates/nncpu/src/session/engine.rs:125); ``kv_f32`` keeps the cache in
     float32 whatever the run's element type (the reference's ``--kv-f32``);
+    ``kv_q4`` keeps it in 4 bits (3.2 times smaller than bfloat16; for models whose
+    attention takes that, ``score`` says what it costs);
     ``max_batch``: sequences generated together (in either precision a
     sequence's logits depend on the others by rounding alone: the kernels of
     a step follow from its size); ``system_prompt`` opens the
@@ -54,6 +61,7 @@ class SessionParams:
     system_prompt: str = ""
     reply_open: str = ""
     run_ahead: bool = True      # launch each decode step on the device's own choices before the host reads them
+    kv_q4: bool = False
 
 
 @dataclass(frozen=True)
@@ -93,6 +101,8 @@ class Session:
         session's own sequence."""
         if params.n_ctx < 0 or params.max_batch < 1:
             raise InvalidArgument(f"n_ctx {params.n_ctx}, max_batch {params.max_batch}")
+        if params.kv_f32 and params.kv_q4:
+            raise InvalidArgument("a cache in float32 (kv_f32) and in 4 bits (kv_q4)")
         self.model = model
         self.params = params
         self.tokenizer = tokenizer
@@ -100,7 +110,7 @@ class Session:
         per_seq = (self.n_ctx + PAGE - 1) // PAGE * PAGE
         self.engine = engine if engine is not None else Engine(
             model, max_tokens=per_seq * (params.max_batch + 1), max_seq_len=self.n_ctx,
-            kv_dtype=torch.float32 if params.kv_f32 else None)
+            kv_dtype=torch.float32 if params.kv_f32 else "q4" if params.kv_q4 else None)
         self.seed = params.seed if params.seed != 0 else int.from_bytes(os.urandom(8), "little") | 1
         self._cancel = CancelHandle()
         self._own_slot: Optional[int] = None
@@ -119,9 +129,7 @@ class Session:
         ``max_batch`` run as later batches on the slots the earlier ones gave
         back.  ``on_piece(Piece)`` may return False to stop that sequence.
         ``stop_token_ids`` defaults to the configuration's end-of-sequence ids."""
-        params.sampler.check("generate")
-        if params.max_tokens < 0:
-            raise InvalidArgument(f"generate: max_tokens {params.max_tokens}")
+        params.check("generate")
         stops = self._stops(stop_token_ids)
         sampler = self._make_sampler(params.sampler, self.seed + 1000003 * self._n_generate_calls, self.model.spec.vocab_size)
         self._n_generate_calls += 1
@@ -132,6 +140,36 @@ class Session:
                          max_batch=self.params.max_batch, n_ctx=self.n_ctx,
                          n_pages=self.engine.n_pages - (self.n_ctx + PAGE - 1) // PAGE, on_finish=on_finish,
                          run_ahead=self.params.run_ahead)
+
+    def score(self, texts: Sequence[Sequence[int]], alternatives: int = 0) -> List[ScoreResult]:
+        """How likely every text (token ids) is: for each of its tokens from the second on the log probability given those
+        before it, the entropy of the prediction and the ``alternatives`` likeliest tokens (up to 32).  A text is run through the model and
+        this session's cache as generation would run it, ``SCORE_TOKENS`` tokens a step (their logits are what takes memory:
+        151 936 tokens of vocabulary make 150 MB of them), on a slot of its own that is given back
+        (the reference's --perplexity: crates/nncpu-cli/src/devtools.rs:711-767)."""
+        check_alternatives(alternatives, "score")
+        for i, text in enumerate(texts):
+            if len(text) == 0:
+                raise InvalidArgument(f"score: text {i} is empty")
+            if len(text) > self.n_ctx:
+                raise ContextFull(f"text {i} of {len(text)} tokens does not fit the {self.n_ctx}-token context")
+        results = []
+        for text in texts:
+            text = [int(t) for t in text]
+            rows = Logprobs(alternatives, self.model.spec.vocab_size)
+            slot = self.engine.alloc_slot()
+            try:
+                for at in range(0, len(text), SCORE_TOKENS):
+                    part = text[at:at + SCORE_TOKENS]
+                    given = text[at + 1:at + 1 + len(part)]          # a token's logits predict the one after it
+                    logits = self.engine.step([slot], [part], want=[list(range(len(given)))])
+                    if given:
+                        rows.add(logits, given)
+                results.append(ScoreResult(rows.read()))
+                self.engine.check_status()
+            finally:
+                self.engine.free_slot(slot)
+        return results
 
     def _stops(self, stop_token_ids):
         """The configuration's end-of-sequence ids and, with a tokenizer, the end markers its vocabulary
@@ -232,9 +270,7 @@ class Session:
         earlier calls is kept, only what is new is evaluated, and the generated
         tokens (a stop token included) join the sequence; the last of them
         waits to be evaluated by the next call."""
-        params.sampler.check("generate")
-        if params.max_tokens < 0:
-            raise InvalidArgument(f"generate: max_tokens {params.max_tokens}")
+        params.check("generate")
         context = self._own_tokens + [int(t) for t in tokens]
         if not context:
             raise InvalidArgument("there is nothing to continue: the context and the new tokens are both empty")
