@@ -10,6 +10,7 @@
 #include <math.h>
 
 #define NN_LIB attention_q4
+#define NN_LAUNCH_OVERLAP
 #include "common.cuh"
 #include "cache_q4.cuh"
 
@@ -71,8 +72,9 @@ __device__ __forceinline__ float closing_factor(const AttnQ4& p, int t, int h, f
 // Rounded below 32 bits are: a weight p, and p d, both to 11 bits.
 //
 // A block is two warps, each of which takes one half of every page: it brings its 32 keys' codes and scales (5 KB for D = 128) to its
-// own ring in shared memory by 16-byte cp.async and shares nothing with the other until a pair's pages are done, when
-// the first adds what the second leaves in shared memory.
+// own ring in shared memory by 16-byte cp.async (with the copy engine's untiled copies, asked for by one lane, 64 sequences of up to
+// 8 000 keys took 115 us instead of 98) and shares nothing with the other until a pair's pages are done, when the first adds
+// what the second leaves in shared memory.
 //
 // The pages of all (token, key/value head) pairs lie in one row, of which every block takes an equal share, wherever that
 // begins and ends: unequal sequences cost nothing, and there is one wave of blocks.  A pair that lies within one block is finished by it; of
@@ -87,10 +89,11 @@ struct Stream {
     int heads;              // query heads of a pair (a part of those that share a key/value head where these are many)
     int chunks;             // such parts of a key/value head
     int pairs;              // n_kv * chunks: pairs of a token
-    int min_pages;          // pages that a block takes at least
+    int min_places;         // places of the row that a block takes at least
     int blocks;             // blocks of the launch
     float scale2;           // scale * log2(e)
     ScoreCap cap;
+    int2* parts;            // [n, pairs]: the first block that has a part of a pair, and the last
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -169,62 +172,71 @@ __device__ __forceinline__ int pages_of(const AttnQ4& p, int t) {
     return PageWalk(first_visible_key(pos, p.window), pos, p.keep).n;
 }
 
-// How the row of pages is cut: its length, the blocks that share it, and where a block's share begins.
+// How the row of pairs is cut.  A pair is kPairCost places and then its pages, one place each: what a block does once for a pair (queries
+// in, parts out) takes about as long as that many pages, so that blocks with several short pairs end with the others.
+constexpr unsigned kPairCost = 3;
 struct Row {
-    long pages;
-    int blocks;
-    __device__ __forceinline__ long start(int b) const { return pages * b / blocks; }
-    __device__ __forceinline__ int block_of(long page) const { return (int)(((page + 1) * blocks - 1) / pages); }
+    unsigned places, blocks, each, more;         // a block has `each` places, the first `more` blocks one more
+    __device__ __forceinline__ unsigned start(unsigned b) const { return each * b + min(b, more); }
+    __device__ __forceinline__ int block_of(unsigned place) const {
+        const unsigned at = more * (each + 1);
+        return place < at ? place / (each + 1) : more + (place - at) / each;
+    }
 };
-// (Every warp by itself, 32 tokens at a time.)
-__device__ __forceinline__ Row row_of(const AttnQ4& p, const Stream& st, int lane) {
-    int sum = 0;
-    for (int t = lane; t < p.n; t += 32) sum += pages_of(p, t);
-    long total = sum;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+// (Every warp by itself, 32 tokens at a time; `mine`: the pages of token `lane`, which are asked for once.)
+__device__ __forceinline__ Row row_of(const AttnQ4& p, const Stream& st, int lane, int mine) {
+    unsigned sum = mine > 0 ? mine + kPairCost : 0;
+    for (int t = lane + 32; t < p.n; t += 32) {
+        const int n = pages_of(p, t);
+        sum += n > 0 ? n + kPairCost : 0;
+    }
     Row row;
-    row.pages = total * st.pairs;
-    const long b = (row.pages + st.min_pages - 1) / st.min_pages;
-    row.blocks = (int)(b < st.blocks ? b : st.blocks);
+    row.places = __reduce_add_sync(0xffffffffu, sum) * st.pairs;
+    row.blocks = min((row.places + st.min_places - 1) / st.min_places, (unsigned)st.blocks);
+    row.each = row.blocks > 0 ? row.places / row.blocks : 0;
+    row.more = row.places - row.each * row.blocks;
     return row;
 }
 
-// A place in the row of pages: page i of the n that pair y of token t walks through.
+// Where a block is: page i of the n that pair y of token t walks through, and how many places are left to it.
 struct Place {
-    int t, y, i, n;
+    int t, y, i, n, left;
     // to the next pair with pages
     __device__ __forceinline__ void next_pair(const AttnQ4& p, const Stream& st) {
         i = 0;
+        left -= kPairCost;
         if (++y == st.pairs) {
             y = 0;
             do { ++t; } while (t < p.n && (n = pages_of(p, t)) == 0);
         }
     }
 };
-__device__ __forceinline__ Place place_of(const AttnQ4& p, const Stream& st, long page, int lane) {
-    long before = 0;
+__device__ __forceinline__ Place place_of(const AttnQ4& p, const Stream& st, unsigned place, int left, int lane, int mine) {
+    unsigned before = 0;
     for (int t0 = 0;; t0 += 32) {
-        const int n = t0 + lane < p.n ? pages_of(p, t0 + lane) : 0;
-        int upto = n;
+        const int n = t0 == 0 ? mine : t0 + lane < p.n ? pages_of(p, t0 + lane) : 0;
+        const unsigned places = n > 0 ? n + kPairCost : 0;
+        unsigned upto = places;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += v;
         }
-        const unsigned beyond = __ballot_sync(0xffffffffu, before + (long)upto * st.pairs > page);
+        const unsigned beyond = __ballot_sync(0xffffffffu, before + upto * st.pairs > place);
         if (beyond != 0 || t0 + 32 >= p.n) {
             const int l = beyond != 0 ? __ffs(beyond) - 1 : 31;
-            const int nl = __shfl_sync(0xffffffffu, n, l), at = __shfl_sync(0xffffffffu, upto, l) - nl;
-            const long rest = page - before - (long)at * st.pairs;
+            const unsigned of_pair = __shfl_sync(0xffffffffu, places, l);
+            const unsigned rest = place - before - (__shfl_sync(0xffffffffu, upto, l) - of_pair) * st.pairs;
             Place w;
             w.t = t0 + l;
-            w.n = nl;
-            w.y = (int)(rest / max(nl, 1));
-            w.i = (int)(rest - (long)w.y * nl);
+            w.n = __shfl_sync(0xffffffffu, n, l);
+            w.y = of_pair > 0 ? rest / of_pair : 0;
+            w.i = (int)(rest - w.y * of_pair) - (int)kPairCost;
+            w.left = left + min(w.i, 0);          // (the places before the pair's first page)
+            w.i = max(w.i, 0);
             return w;
         }
-        before += (long)__shfl_sync(0xffffffffu, upto, 31) * st.pairs;
+        before += __shfl_sync(0xffffffffu, upto, 31) * st.pairs;
     }
 }
 
@@ -233,6 +245,17 @@ __device__ __forceinline__ Place place_of(const AttnQ4& p, const Stream& st, lon
 // float16, and so is p d.  Greater steps (they are at most 8 736: numbers lie within +-65 504) leave less.
 constexpr float kLag = 4.0f;
 __device__ __forceinline__ float headroom(float d_max) { return d_max <= 1.0f ? 11.0f : 11.0f - ceilf(log2f(d_max)); }
+
+// Rows of no sequence are zeros, and in one part.
+template <int D>
+__device__ __forceinline__ void zero_rows(const AttnQ4& p, const Stream& st) {
+    for (int t = blockIdx.x; t < p.n; t += gridDim.x) {
+        if (pages_of(p, t) > 0) continue;
+        for (int i = threadIdx.x; i < p.n_heads * D / 8; i += 32 * kStreamWarps)
+            reinterpret_cast<uint4*>(p.out)[(size_t)t * p.n_heads * D / 8 + i] = make_uint4(0, 0, 0, 0);
+        for (int i = threadIdx.x; i < st.pairs; i += 32 * kStreamWarps) st.parts[(size_t)t * st.pairs + i] = make_int2(0, 0);
+    }
+}
 
 template <int NG, int NT>
 __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_kernel(const AttnQ4 p, const Stream st) {
@@ -245,18 +268,31 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
     uint8_t* ring = stream_smem + warp * kStreamStages * kStage;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
     float* meet = reinterpret_cast<float*>(stream_smem + kStreamWarps * kStreamStages * kStage);   // [COLS][D + 4]: lanes, reference, sum
-
-    // rows of no sequence are zeros
-    for (int t = blockIdx.x; t < p.n; t += gridDim.x)
-        if (pages_of(p, t) == 0)
-            for (int i = threadIdx.x; i < p.n_heads * D; i += 32 * kStreamWarps)
-                reinterpret_cast<__nv_bfloat16*>(p.out)[(size_t)t * p.n_heads * D + i] = __float2bfloat16_rn(0.0f);
-    const Row row = row_of(p, st, lane);
-    if ((int)blockIdx.x >= row.blocks) return;
-    const long first_page = row.start(blockIdx.x);
-    const int n_mine = (int)(row.start(blockIdx.x + 1) - first_page);
-    Place here = place_of(p, st, first_page, lane), ahead = here;
-    int fetched = 0;
+    wait_for_previous_kernels();
+    let_next_kernel_start();
+    const int my_pages = lane < p.n ? pages_of(p, lane) : 0;
+    const Row row = row_of(p, st, lane, my_pages);
+    if ((int)blockIdx.x >= row.blocks) {
+        zero_rows<D>(p, st);
+        return;
+    }
+    const unsigned first_place = row.start(blockIdx.x);
+    Place here = place_of(p, st, first_place, (int)(row.start(blockIdx.x + 1) - first_place), lane, my_pages), ahead = here;
+    // the queries of a pair, as they lie: head r of the column tile, lanes 32 g + 8 c to + 7
+    uint4 raw[NT][NG];
+    auto ask_queries = [&]() {
+        const int kvh = here.y / st.chunks, part = here.y - kvh * st.chunks, group = p.n_heads / p.n_kv;
+        const int nh = here.left > 0 ? min(st.heads, group - part * st.heads) : 0;
+        const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q) + ((size_t)here.t * p.n_heads + kvh * group + part * st.heads) * D + 8 * c;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                raw[nt][g] = make_uint4(0, 0, 0, 0);
+                if (8 * nt + r < nh) raw[nt][g] = *reinterpret_cast<const uint4*>(q + (8 * nt + r) * D + 32 * g);
+            }
+    };
+    ask_queries();
     unsigned there = 0;                     // bit s: stage s holds a page (and not one that is missing)
     int ids = -1, id_at = 0, id_end = 0;    // lane l holds the page l of the next 32 of the pair that is being fetched; the next one, and how many
     const uint8_t *kc = nullptr, *vc = nullptr, *ks = nullptr, *vs = nullptr;   // this lane's first 16 bytes of a page: codes and scales
@@ -264,7 +300,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
 
     // asks for this warp's keys of the next page (nothing for a page that is not there)
     auto fetch = [&](int stage) {
-        if (fetched < n_mine) {
+        if (ahead.left > 0) {
             if (id_at == id_end) {
                 const int pos = p.tok_pos[ahead.t];
                 const PageWalk walk(first_visible_key(pos, p.window), pos, p.keep);
@@ -295,7 +331,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
             } else {
                 there &= ~(1u << stage);
             }
-            ++fetched;
+            --ahead.left;
             if (++ahead.i == ahead.n) ahead.next_pair(p, st);
         }
         cp_async_commit();
@@ -305,10 +341,12 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
     for (int s = 0; s < kStreamStages - 1; ++s) fetch(s);
 
     int stage = 0;
-    for (int done = 0; done < n_mine;) {
+    while (here.left > 0) {
         // -- a pair, or the part of it that lies here
-        const int t = here.t, take = min(here.n - here.i, n_mine - done);
-        const int kvh = here.y / st.chunks, h0 = kvh * (p.n_heads / p.n_kv) + here.y % st.chunks * st.heads;
+        const int t = here.t, y = here.y, from = here.i, take = min(here.n - from, here.left);
+        const int n_pages = here.n;
+        const bool whole = take == n_pages;
+        const int kvh = y / st.chunks, h0 = kvh * (p.n_heads / p.n_kv) + (y - kvh * st.chunks) * st.heads;
         const int nh = min(st.heads, (kvh + 1) * (p.n_heads / p.n_kv) - h0);
         const int pos = p.tok_pos[t], first = first_visible_key(pos, p.window);
         const PageWalk walk(first, pos, p.keep);
@@ -318,14 +356,10 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
         float col[NT][2];              // what scores of heads 2 c and 2 c + 1 are multiplied by
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            uint4 w[NG];
+            const uint4 (&w)[NG] = raw[nt];
             float top = 0.0f;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                w[g] = make_uint4(0, 0, 0, 0);
-                if (8 * nt + r < nh)
-                    w[g] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + ((size_t)t * p.n_heads + h0 + 8 * nt + r) * D +
-                                                           32 * g + 8 * c);
                 const float2 a = two_bf16(w[g].x), b = two_bf16(w[g].y), e = two_bf16(w[g].z), f = two_bf16(w[g].w);
                 top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))),
                                        fmaxf(fmaxf(fabsf(e.x), fabsf(e.y)), fmaxf(fabsf(f.x), fabsf(f.y)))));
@@ -378,7 +412,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
             od[nt][0] = od[nt][1] = od[nt][2] = od[nt][3] = 0.0f;
             m[nt][0] = m[nt][1] = 0.0f;
         }
-        int pi = walk.page(here.i);
+        int pi = walk.page(from);
         for (int i = 0; i < take; ++i) {
             cp_async_wait<kStreamStages - 2>();
             __syncwarp();
@@ -387,7 +421,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
             fetch(stage == 0 ? kStreamStages - 1 : stage - 1);
             stage = stage == kStreamStages - 1 ? 0 : stage + 1;
             const int key0 = pi * kPage + 16 * kTiles * warp;
-            pi = here.i + i + 1 == walk.n_kept ? walk.lo : pi + 1;
+            pi = from + i + 1 == walk.n_kept ? walk.lo : pi + 1;
             if (missing || key0 > pos || (key0 + 16 * kTiles - 1 < first && key0 >= p.keep)) continue;      // none of these keys is seen
             const bool full = key0 >= first && key0 + 16 * kTiles - 1 <= pos;
             if (!full) {
@@ -544,98 +578,105 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
                 }
             }
         }
-        // -- the warps' parts meet: thread (r, c) holds lanes 32 g + 4 r to + 3 of heads 2 c and 2 c + 1
+        // -- on to the next pair: its queries come while this one's parts meet
+        here.i += take;
+        here.left -= take;
+        const int left = here.left;
+        if (here.i == here.n) here.next_pair(p, st);
+        ask_queries();
+        if (from == 0 && threadIdx.x == 0)      // the first block with a part of the pair, and the last
+            st.parts[(size_t)t * st.pairs + y] =
+                make_int2(blockIdx.x, whole ? (int)blockIdx.x : row.block_of(row.start(blockIdx.x + 1) - (left + take) + n_pages - 1));
+        // -- the warps' parts meet: thread (r, c) holds lanes 32 g + 4 r to + 3 of heads 2 c and 2 c + 1.  Each warp leaves the other one's
+        // head and finishes its own.
         __syncthreads();                 // (the last pair's part has been read)
-        const bool whole = take == here.n;
-        const int slot = 2 * blockIdx.x + (here.i > 0 ? 0 : 1);      // (a pair that began in an earlier block is this one's first)
+        const int slot = 2 * blockIdx.x + (from > 0 ? 0 : 1);      // (a pair that began in an earlier block is this one's first)
 #pragma unroll
         for (int pass = 0; pass < 2; ++pass) {
             if (pass == 1) __syncthreads();
-            if (warp == 1 - pass)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int h = 8 * nt + 2 * c + e;
-                        float* other = meet + h * (D + 4);
-                        const float sum = __shfl_sync(0xffffffffu, od[nt][e + 2], c), ref = fresh ? -INFINITY : m[nt][e];
-                        float f0 = 1.0f, f1 = 0.0f, top = ref, total = sum;
-                        if (pass == 1) {
-                            top = fmaxf(ref, other[D]);
-                            f0 = ref == -INFINITY ? 0.0f : exp2f(ref - top);
-                            f1 = other[D] == -INFINITY ? 0.0f : exp2f(other[D] - top);
-                            total = fmaf(other[D + 1], f1, sum * f0);
-                            if (whole && h < nh) f0 *= closing_factor(p, t, h0 + h, top / kLog2e, total), f1 *= closing_factor(p, t, h0 + h, top / kLog2e, total);
-                        }
-#pragma unroll
-                        for (int g = 0; g < NG; ++g) {
-                            const float b = fmaf(8.0f, __shfl_sync(0xffffffffu, od[nt][e], 8 * g + c), __shfl_sync(0xffffffffu, od[nt][e], 8 * g + 4 + c));
-                            const int d = 32 * g + 4 * r;
-                            float4 v = make_float4(o[nt][2 * g][e] + b, o[nt][2 * g][e + 2] + b, o[nt][2 * g + 1][e] + b, o[nt][2 * g + 1][e + 2] + b);
-                            if (pass == 0) {
-                                *reinterpret_cast<float4*>(other + d) = v;
-                                continue;
-                            }
-                            const float4 w = *reinterpret_cast<const float4*>(other + d);
-                            v = make_float4(fmaf(w.x, f1, v.x * f0), fmaf(w.y, f1, v.y * f0), fmaf(w.z, f1, v.z * f0), fmaf(w.w, f1, v.w * f0));
-                            if (h >= nh) continue;
-                            if (whole) {
-                                __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
-                                uint2 packed = make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
-                                __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + ((size_t)t * p.n_heads + h0 + h) * D + d;
-                                *reinterpret_cast<uint2*>(out) = packed;
-                            } else {
-                                *reinterpret_cast<float4*>(p.part + ((size_t)slot * COLS + h) * (D + 4) + d) = v;
-                            }
-                        }
-                        if (r == 0 && pass == 0) {
-                            other[D] = top;
-                            other[D + 1] = total;
-                        }
-                        if (r == 0 && pass == 1 && !whole && h < nh) {
-                            float* part = p.part + ((size_t)slot * COLS + h) * (D + 4);
-                            part[D] = top;
-                            part[D + 1] = total;
+                for (int e = 0; e < 2; ++e) {
+                    if ((e == warp) != (pass == 1)) continue;
+                    const int h = 8 * nt + 2 * c + e;
+                    float* other = meet + h * (D + 4);
+                    const float sum = __shfl_sync(0xffffffffu, od[nt][e + 2], c), ref = fresh ? -INFINITY : m[nt][e];
+                    float f0 = 1.0f, f1 = 0.0f, top = ref, total = sum;
+                    if (pass == 1) {
+                        top = fmaxf(ref, other[D]);
+                        f0 = ref == -INFINITY ? 0.0f : exp2f(ref - top);
+                        f1 = other[D] == -INFINITY ? 0.0f : exp2f(other[D] - top);
+                        total = fmaf(other[D + 1], f1, sum * f0);
+                        if (whole && h < nh) {
+                            const float f = closing_factor(p, t, h0 + h, top / kLog2e, total);
+                            f0 *= f;
+                            f1 *= f;
                         }
                     }
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        const float b = fmaf(8.0f, __shfl_sync(0xffffffffu, od[nt][e], 8 * g + c), __shfl_sync(0xffffffffu, od[nt][e], 8 * g + 4 + c));
+                        const int d = 32 * g + 4 * r;
+                        float4 v = make_float4(o[nt][2 * g][e] + b, o[nt][2 * g][e + 2] + b, o[nt][2 * g + 1][e] + b, o[nt][2 * g + 1][e + 2] + b);
+                        if (pass == 0) {
+                            *reinterpret_cast<float4*>(other + d) = v;
+                            continue;
+                        }
+                        const float4 w = *reinterpret_cast<const float4*>(other + d);
+                        v = make_float4(fmaf(w.x, f1, v.x * f0), fmaf(w.y, f1, v.y * f0), fmaf(w.z, f1, v.z * f0), fmaf(w.w, f1, v.w * f0));
+                        if (h >= nh) continue;
+                        if (whole) {
+                            const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+                            const uint2 packed = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+                            *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + ((size_t)t * p.n_heads + h0 + h) * D + d) = packed;
+                        } else {
+                            *reinterpret_cast<float4*>(p.part + ((size_t)slot * COLS + h) * (D + 4) + d) = v;
+                        }
+                    }
+                    if (r == 0 && pass == 0) {
+                        other[D] = top;
+                        other[D + 1] = total;
+                    }
+                    if (r == 0 && pass == 1 && !whole && h < nh) {
+                        float* part = p.part + ((size_t)slot * COLS + h) * (D + 4);
+                        part[D] = top;
+                        part[D + 1] = total;
+                    }
+                }
         }
-        done += take;
-        here.i += take;
-        if (here.i == here.n) here.next_pair(p, st);
     }
     cp_async_wait<0>();
+    zero_rows<D>(p, st);
 }
 
-// The parts of a pair that lies in several blocks, in the order of its keys.  grid = (n, pairs), 128 threads.
+// The parts of a pair that lies in several blocks, in the order of its keys.  grid = (n, pairs, heads of a pair), a thread a lane.
 __global__ void __launch_bounds__(128) stream_merge_kernel(const AttnQ4 p, const Stream st, int cols) {
-    const int t = blockIdx.x, y = blockIdx.y, lane = threadIdx.x & 31;
-    const int n = pages_of(p, t);
-    if (n == 0) return;
-    const Row row = row_of(p, st, lane);
-    int before = 0;
-    for (int i = lane; i < t; i += 32) before += pages_of(p, i);
-    long at = before;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) at += __shfl_xor_sync(0xffffffffu, at, o);
-    at = at * st.pairs + (long)y * n;
-    const int b0 = row.block_of(at), b1 = row.block_of(at + n - 1);
-    if (b0 == b1) return;                // that block has finished it
+    const int t = blockIdx.x, y = blockIdx.y, h = blockIdx.z, D = p.D, d = threadIdx.x;
+    wait_for_previous_kernels();
+    let_next_kernel_start();
+    const int2 b = st.parts[(size_t)t * st.pairs + y];
     const int kvh = y / st.chunks, h0 = kvh * (p.n_heads / p.n_kv) + y % st.chunks * st.heads;
-    const int nh = min(st.heads, (kvh + 1) * (p.n_heads / p.n_kv) - h0), D = p.D;
-    for (int x = threadIdx.x; x < nh * D; x += 128) {
-        const int h = x / D, d = x % D;
-        float mx = -INFINITY, sum = 0.0f, out = 0.0f;
-        for (int b = b0; b <= b1; ++b)
-            mx = fmaxf(mx, p.part[((size_t)(2 * b + (b == b0 ? 1 : 0)) * cols + h) * (D + 4) + D]);
-        for (int b = b0; b <= b1; ++b) {
-            const float* from = p.part + ((size_t)(2 * b + (b == b0 ? 1 : 0)) * cols + h) * (D + 4);
-            const float f = from[D] == -INFINITY ? 0.0f : exp2f(from[D] - mx);
-            sum = fmaf(from[D + 1], f, sum);
-            out = fmaf(from[d], f, out);
-        }
-        const float f = closing_factor(p, t, h0 + h, mx / kLog2e, sum);
-        reinterpret_cast<__nv_bfloat16*>(p.out)[((size_t)t * p.n_heads + h0 + h) * D + d] = __float2bfloat16_rn(out * f);
+    if (b.x == b.y || h0 + h >= (kvh + 1) * (p.n_heads / p.n_kv)) return;       // that block has finished it; no such head
+    // the first part is its block's last, the others are their blocks' first
+    const size_t step = (size_t)2 * cols * (D + 4);
+    const float* first = p.part + ((size_t)(2 * b.x + 1) * cols + h) * (D + 4);
+    const float* rest = p.part + ((size_t)(2 * b.x + 2) * cols + h) * (D + 4);
+    const int n = b.y - b.x;
+    float top = first[D];
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) top = fmaxf(top, rest[i * step + D]);
+    float f = first[D] == -INFINITY ? 0.0f : exp2f(first[D] - top);
+    float sum = first[D + 1] * f, out = first[d] * f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        const float* from = rest + i * step;
+        f = from[D] == -INFINITY ? 0.0f : exp2f(from[D] - top);
+        sum = fmaf(from[D + 1], f, sum);
+        out = fmaf(from[d], f, out);
     }
+    f = closing_factor(p, t, h0 + h, top / kLog2e, sum);
+    reinterpret_cast<__nv_bfloat16*>(p.out)[((size_t)t * p.n_heads + h0 + h) * D + d] = __float2bfloat16_rn(out * f);
 }
 
 // Pages of a token's walk that split s takes: [first, end).
@@ -806,7 +847,7 @@ static bool sizes_ok(int n, int n_heads, int n_kv, int D) {
 static bool streams(int dt, int D) { return dt == DT_BF16 && D <= 128; }
 
 // Blocks of a token's pages' row, all of which run at once, and how the heads of a key/value head are dealt with.
-constexpr int kStreamMinPages = 4;
+constexpr int kStreamMinPlaces = 4;
 static int stream_tiles(int n_heads, int n_kv) { return n_heads / n_kv > 8 ? 2 : 1; }
 static int stream_smem(int D, int tiles) {
     return kStreamWarps * kStreamStages * 40 * D + 8 * tiles * (D + 4) * (int)sizeof(float);
@@ -848,7 +889,8 @@ extern "C" long nncpu_attention_q4_scratch(int n, int n_heads, int n_kv, int D, 
     if (n <= 0 || !sizes_ok(n, n_heads, n_kv, D)) return 0;
     if (streams(dt, D)) {
         const int tiles = stream_tiles(n_heads, n_kv);
-        return 2L * stream_blocks(D, tiles) * 8 * tiles * (D + 4);
+        const int group = n_heads / n_kv, chunks = (group + 8 * tiles - 1) / (8 * tiles);
+        return 2L * stream_blocks(D, tiles) * 8 * tiles * (D + 4) + 2L * n * n_kv * chunks;
     }
     const int s = any_splits(n, n_heads, n_kv, longest);
     return s > 1 ? (long)n * n_heads * s * (D + 2) : 0;
@@ -873,12 +915,29 @@ extern "C" int nncpu_attention_q4(const void* q, int dt, const uint8_t* k_pages,
         NN_CHECK((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)part % 16 == 0,
                  "attention_q4: bfloat16 queries, output and scratch start on 16-byte boundaries");
         const int tiles = stream_tiles(n_heads, n_kv), chunks = (group + 8 * tiles - 1) / (8 * tiles);
+        NN_CHECK((long)n * n_kv * chunks * (bt_stride + 3L) < (1L << 31), "attention_q4: %d tokens of up to %d pages", n, bt_stride);
         NN_CHECK(n_kv <= 65535 / chunks, "attention_q4: %d key/value heads in %d parts", n_kv, chunks);
-        Stream st{(group + chunks - 1) / chunks, chunks, n_kv * chunks, kStreamMinPages, stream_blocks(D, tiles), scale * kLog2e, score_cap(scale, cap)};
-        stream_kernel_of(D, tiles)<<<st.blocks, 32 * kStreamWarps, stream_smem(D, tiles), stream>>>(p, st);
-        NN_LAUNCH_OK("attention_q4");
-        stream_merge_kernel<<<dim3((unsigned)n, (unsigned)st.pairs), 128, 0, stream>>>(p, st, 8 * tiles);
-        NN_LAUNCH_OK("attention_q4 (merge)");
+        Stream st{(group + chunks - 1) / chunks, chunks, n_kv * chunks, kStreamMinPlaces, stream_blocks(D, tiles), scale * kLog2e, score_cap(scale, cap), nullptr};
+        st.parts = reinterpret_cast<int2*>(part + 2L * st.blocks * 8 * tiles * (D + 4));
+        // All blocks of the first kernel have to run at once, six to an SM, so it is not launched to start under the end of the one
+        // before: beside blocks of that one an SM may find room for five, and the sixth, begun when those are done, doubles the time
+        // (64 sequences of up to 8 000 keys: 84 us instead of 71).  The second one is.
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[1];
+        cfg.gridDim = dim3((unsigned)st.blocks);
+        cfg.blockDim = dim3(32 * kStreamWarps);
+        cfg.dynamicSmemBytes = stream_smem(D, tiles);
+        cfg.stream = stream;
+        cfg.attrs = attr;
+        cfg.numAttrs = 0;
+        cudaError_t e = cudaLaunchKernelEx(&cfg, stream_kernel_of(D, tiles), p, st);
+        NN_CHECK(e == cudaSuccess, "attention_q4: launch failed: %s", cudaGetErrorString(e));
+        cfg.gridDim = dim3((unsigned)n, (unsigned)st.pairs, (unsigned)st.heads);
+        cfg.blockDim = dim3(D);
+        cfg.dynamicSmemBytes = 0;
+        cfg.numAttrs = overlap_attribute(attr);
+        e = cudaLaunchKernelEx(&cfg, stream_merge_kernel, p, st, 8 * tiles);
+        NN_CHECK(e == cudaSuccess, "attention_q4 (merge): launch failed: %s", cudaGetErrorString(e));
         return 0;
     }
     const int chunks = (group + kAnyHeads - 1) / kAnyHeads;

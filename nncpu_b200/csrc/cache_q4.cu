@@ -151,33 +151,149 @@ __global__ void __launch_bounds__(256) append_kernel(const Append a) {
     }
 }
 
-// The number of lane `i` of position `at` in a page.
-template <bool VALUES>
-__device__ __forceinline__ float page_number(const uint8_t* base, int at, int i, int D) {
-    const int NG = D / kGroup, g = i >> 5;
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(base);
-    const float2 dm = __half22float2(reinterpret_cast<const __half2*>(base + q4_scales_at(D))[at * NG + g]);
-    const uint32_t code = VALUES ? words[q4_value_word(at, (i & 31) >> 2, g, NG)] >> (16 * (at & 1) + 4 * (i & 3))
-                                 : words[q4_key_word(at, (i & 31) >> 3, g, NG)] >> (4 * (i & 7));
-    return q4_number(code & 15, dm);
+// ---------------------------------------------------------------------------
+// Heads of 32, 64 and 128 lanes, rotated whole or not at all, in float32 rows of whole 16-byte pieces: T = D / 4 threads a head, each
+// with four neighbouring lanes, so that a rotation's partner is T / 2 threads away, a group is eight threads, and a thread's four
+// codes are the half of a word that it stores.  A block takes a token and as many heads as it has rounds for, which share the token's
+// angles.  grid = (n, blocks a token), 256 threads.
+// ---------------------------------------------------------------------------
+template <int D, typename F>
+__device__ __forceinline__ void norm_rotate4(F (&x)[4], const float4* gamma, const float2 (&cs)[4], bool rotated, F eps, int j) {
+    constexpr int T = D / 4;
+    if (gamma != nullptr) {
+        F s = (x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]);
+#pragma unroll
+        for (int o = T / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        F r;
+        if constexpr (sizeof(F) == 8) r = rsqrt(s / F(D) + eps);
+        else r = 1.0f / sqrtf(s / F(D) + eps);
+        x[0] *= r * F(gamma->x); x[1] *= r * F(gamma->y); x[2] *= r * F(gamma->z); x[3] *= r * F(gamma->w);
+    }
+    if (rotated) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const F other = __shfl_xor_sync(0xffffffffu, x[e], T / 2);
+            x[e] = j >= T / 2 ? x[e] * F(cs[e].x) + other * F(cs[e].y) : x[e] * F(cs[e].x) - other * F(cs[e].y);
+        }
+    }
 }
 
-// What the cache holds of given tokens: a warp per (token, head), keys by grid.y 0, values by 1.
+template <int D>
+__global__ void __launch_bounds__(256) append_fast_kernel(const Append a) {
+    constexpr int T = D / 4, NG = D / 32, kHeads = 256 / T;
+    const int t = blockIdx.x, j = threadIdx.x % T, per_tok = a.n_heads + 2 * a.n_kv;
+    wait_for_previous_kernels();
+    let_next_kernel_start();
+    const int seq = a.tok_seq[t], pos = a.tok_pos[t];
+    const bool rotated = a.cs != nullptr;
+    float2 cs[4] = {};
+    if (rotated) {
+        const float4* at = reinterpret_cast<const float4*>(a.cs + (size_t)t * (D / 2) + j % (T / 2) * 4);
+        const float4 u = at[0], v = at[1];
+        cs[0] = make_float2(u.x, u.y); cs[1] = make_float2(u.z, u.w); cs[2] = make_float2(v.x, v.y); cs[3] = make_float2(v.z, v.w);
+    }
+    float4 q_gamma = {}, k_gamma = {};
+    if (a.q_gamma != nullptr) q_gamma = ld_f4(a.q_gamma, 4 * j, a.g_dt);
+    if (a.k_gamma != nullptr) k_gamma = ld_f4(a.k_gamma, 4 * j, a.g_dt);
+    float times = 1.0f;
+    if (a.temp_coef != 0.0f) times = 1.0f + a.temp_coef * logf(floorf((float)(pos + 1) / (float)a.temp_every) + 1.0f);
+    const int page = a.n_kv > 0 ? page_of(a.block_table, a.bt_stride, a.n_pages, seq, pos) : -1;
+    const int at = page < 0 ? 0 : pos % kPage;
+    const float* row = reinterpret_cast<const float*>(a.qkv) + (size_t)t * a.ld;
+    // (all threads of a warp go round together: a round's last heads may not be there)
+    for (int h0 = blockIdx.y * kHeads; h0 < per_tok; h0 += gridDim.y * kHeads) {
+        const int h = h0 + threadIdx.x / T;
+        const bool there = h < per_tok;
+        float4 v = make_float4(0, 0, 0, 0);
+        if (there) v = *reinterpret_cast<const float4*>(row + (size_t)h * D + 4 * j);
+        // a warp's heads are of one kind (all of q, all of k, ...) or take every branch that one of them takes
+        const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv;
+        if (__any_sync(0xffffffffu, there && is_q)) {
+            float x[4] = {v.x, v.y, v.z, v.w};
+            norm_rotate4<D, float>(x, a.q_gamma != nullptr ? &q_gamma : nullptr, cs, rotated, (float)a.eps, j);
+            if (there && is_q) {
+                const size_t to = ((size_t)t * a.n_heads + h) * D + 4 * j;
+                if (a.q_dt == DT_F32) {
+                    *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.q_out) + to) = make_float4(x[0] * times, x[1] * times, x[2] * times, x[3] * times);
+                } else {
+                    const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0] * times, x[1] * times), hi = __floats2bfloat162_rn(x[2] * times, x[3] * times);
+                    uint2 u;
+                    u.x = *reinterpret_cast<const uint32_t*>(&lo);
+                    u.y = *reinterpret_cast<const uint32_t*>(&hi);
+                    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.q_out) + to) = u;
+                }
+            }
+        }
+        if (!__any_sync(0xffffffffu, there && !is_q && page >= 0)) continue;
+        float x[4] = {v.x, v.y, v.z, v.w};
+        if (__any_sync(0xffffffffu, there && !is_q && !is_v)) {
+            // in 64 bits, see append_kernel
+            double y[4] = {v.x, v.y, v.z, v.w};
+            norm_rotate4<D, double>(y, a.k_gamma != nullptr ? &k_gamma : nullptr, cs, rotated, a.eps, j);
+            if (!is_v)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = (float)y[e];
+        }
+        bool bad = false;
+        float lo = kHalfMax, hi = -kHalfMax;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] = q4_in_range(x[e]);
+            bad |= x[e] != x[e];
+            lo = fminf(lo, x[e]);
+            hi = fmaxf(hi, x[e]);
+        }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const unsigned any_bad = __ballot_sync(0xffffffffu, bad);
+        if (any_bad >> (threadIdx.x & 24) & 255) lo = hi = __int_as_float(0x7FC00000);
+        const Q4Scale s = q4_scale(lo, hi);
+        const uint32_t codes = q4_code(x[0], s) | q4_code(x[1], s) << 4 | q4_code(x[2], s) << 8 | q4_code(x[3], s) << 12;
+        if (!there || is_q || page < 0) continue;
+        const int kvh = h - a.n_heads - (is_v ? a.n_kv : 0), g = j >> 3, quad = j & 7;
+        uint8_t* base = (is_v ? a.v_pages : a.k_pages) + ((size_t)page * a.n_kv + kvh) * q4_page_bytes(D);
+        const int half = is_v ? 2 * q4_value_word(at, quad, g, NG) + (at & 1) : 2 * q4_key_word(at, quad >> 1, g, NG) + (quad & 1);
+        reinterpret_cast<uint16_t*>(base)[half] = (uint16_t)codes;
+        if (quad == 0) reinterpret_cast<__half2*>(base + q4_scales_at(D))[at * NG + g] = __halves2half2(s.d, s.m);
+    }
+}
+
+// What the cache holds of given tokens: a thread takes four neighbouring lanes of a key and of a value.
 __global__ void __launch_bounds__(256) read_kernel(const uint8_t* k_pages, const uint8_t* v_pages, int n_pages, const int* block_table,
                                                    int bt_stride, const int* tok_seq, const int* tok_pos, void* k_out, void* v_out,
                                                    int out_dt, int n, int n_kv, int D) {
-    const long item = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (item >= (long)n * n_kv) return;
-    const int t = (int)(item / n_kv), h = (int)(item % n_kv);
-    const int pos = tok_pos[t];
-    const int page = page_of(block_table, bt_stride, n_pages, tok_seq[t], pos);
-    const bool values = blockIdx.y == 1;
-    void* out = values ? v_out : k_out;
-    const uint8_t* base = (values ? v_pages : k_pages) + ((size_t)max(page, 0) * n_kv + h) * q4_page_bytes(D);
-    for (int i = lane; i < D; i += 32) {
-        const float v = page < 0 ? 0.0f : values ? page_number<true>(base, pos % kPage, i, D) : page_number<false>(base, pos % kPage, i, D);
-        st_f(out, ((size_t)t * n_kv + h) * D + i, out_dt, v);
+    wait_for_previous_kernels();
+    let_next_kernel_start();
+    const int per_tok = n_kv * D / 4, NG = D / kGroup;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (long)n * per_tok) return;
+    const int t = (int)(i / per_tok), rest = (int)(i - (long)t * per_tok), h = rest / (D / 4), lane = (rest - h * (D / 4)) * 4, g = lane >> 5;
+    const int pos = tok_pos[t], page = page_of(block_table, bt_stride, n_pages, tok_seq[t], pos), at = page < 0 ? 0 : pos % kPage;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (page >= 0) {
+            const uint8_t* base = (which ? v_pages : k_pages) + ((size_t)page * n_kv + h) * q4_page_bytes(D);
+            const int half = which ? 2 * q4_value_word(at, (lane & 31) >> 2, g, NG) + (at & 1)
+                                   : 2 * q4_key_word(at, (lane & 31) >> 3, g, NG) + (lane >> 2 & 1);
+            const uint32_t codes = reinterpret_cast<const uint16_t*>(base)[half];
+            const float2 dm = __half22float2(reinterpret_cast<const __half2*>(base + q4_scales_at(D))[at * NG + g]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = q4_number(codes >> (4 * e) & 15, dm);
+        }
+        void* out = which ? v_out : k_out;
+        if (out_dt == DT_F32) {
+            reinterpret_cast<float4*>(out)[i] = make_float4(x[0], x[1], x[2], x[3]);
+        } else {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
+            uint2 u;
+            u.x = *reinterpret_cast<const uint32_t*>(&lo);
+            u.y = *reinterpret_cast<const uint32_t*>(&hi);
+            reinterpret_cast<uint2*>(out)[i] = u;
+        }
     }
 }
 
@@ -288,6 +404,23 @@ extern "C" int nncpu_qk_norm_rope_append_q4(const void* qkv, int qkv_dt, int ld,
     if (n == 0) return 0;
     Append a{qkv, qkv_dt, ld, q_gamma, k_gamma, g_dt, eps, reinterpret_cast<const float2*>(cos_sin), half, tok_seq, tok_pos, block_table,
              bt_stride, k_pages, v_pages, n_pages, q_out, q_dt, n, n_heads, n_kv, D, temp_coef, temp_every};
+    if ((D == 32 || D == 64 || D == 128) && qkv_dt == DT_F32 && ld % 4 == 0 && (cos_sin == nullptr || half == D / 2) && (uintptr_t)qkv % 16 == 0 &&
+        (uintptr_t)q_out % 16 == 0 && (uintptr_t)cos_sin % 16 == 0 && (uintptr_t)q_gamma % 16 == 0 && (uintptr_t)k_gamma % 16 == 0) {
+        const int rounds = (n_heads + 2 * n_kv + 1024 / D - 1) / (1024 / D);      // a block's rounds, were it alone with a token
+        // as many blocks as eight on each SM ask for
+        long per = (8L * sm_count() + n - 1) / n;
+        per = per < rounds ? per : rounds;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)n, (unsigned)per);
+        cfg.blockDim = dim3(256);
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        cfg.attrs = attr;
+        cfg.numAttrs = overlap_attribute(attr);
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, D == 32 ? append_fast_kernel<32> : D == 64 ? append_fast_kernel<64> : append_fast_kernel<128>, a);
+        NN_CHECK(e == cudaSuccess, "qk_norm_rope_append_q4: launch failed: %s", cudaGetErrorString(e));
+        return 0;
+    }
     const long items = (long)n * (n_heads + 2 * n_kv);
     const dim3 grid((unsigned)((items + 7) / 8));
     switch (D / 32) {
@@ -310,10 +443,19 @@ extern "C" int nncpu_q4_read(const uint8_t* k_pages, const uint8_t* v_pages, int
     NN_CHECK(q4_lanes_ok(D), "q4_read: heads of %d lanes (whole groups of 32, at most 256)", D);
     NN_CHECK(n >= 0 && n_kv > 0 && bt_stride > 0 && n_pages > 0, "q4_read: %d tokens, %d heads, %d pages", n, n_kv, n_pages);
     if (n == 0) return 0;
-    const long items = (long)n * n_kv;
-    read_kernel<<<dim3((unsigned)((items + 7) / 8), 2), 256, 0, stream>>>(k_pages, v_pages, n_pages, block_table, bt_stride, tok_seq, tok_pos,
-                                                                         k_out, v_out, out_dt, n, n_kv, D);
-    NN_LAUNCH_OK("q4_read");
+    NN_CHECK((uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0, "q4_read: outputs start on 16-byte boundaries");
+    const long items = (long)n * n_kv * D / 4;
+    NN_CHECK(items / 256 < (1L << 31), "q4_read: %d tokens", n);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((items + 255) / 256));
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    cfg.attrs = attr;
+    cfg.numAttrs = overlap_attribute(attr);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, read_kernel, k_pages, v_pages, n_pages, block_table, bt_stride, tok_seq, tok_pos, k_out, v_out,
+                                             out_dt, n, n_kv, D);
+    NN_CHECK(e == cudaSuccess, "q4_read: launch failed: %s", cudaGetErrorString(e));
     return 0;
 }
 

@@ -122,7 +122,7 @@ def launch_overlap(on: bool) -> None:
     On by default; off, every kernel waits for the one before it to be over, and the results are the same bits.  Where a product
     asks for its first weights themselves, the kernel of this library right before it in the stream must not be the one that
     writes them."""
-    for name in ("linear_skinny", "gemm_sm100", "generic", "attention_tc", "linear_f32", "attention_f32"):
+    for name in ("linear_skinny", "gemm_sm100", "generic", "attention_tc", "linear_f32", "attention_f32", "cache_q4", "attention_q4"):
         getattr(library.load(name), f"nncpu_launch_overlap_{name}")(ctypes.c_int(1 if on else 0))
 
 
