@@ -166,7 +166,7 @@ __device__ __forceinline__ void norm_rotate4(F (&x)[4], const float4* gamma, con
         for (int o = T / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         F r;
         if constexpr (sizeof(F) == 8) r = rsqrt(s / F(D) + eps);
-        else r = 1.0f / sqrtf(s / F(D) + eps);
+        else r = rsqrtf(s * (1.0f / D) + eps);
         x[0] *= r * F(gamma->x); x[1] *= r * F(gamma->y); x[2] *= r * F(gamma->z); x[3] *= r * F(gamma->w);
     }
     if (rotated) {
@@ -200,12 +200,19 @@ __global__ void __launch_bounds__(256) append_fast_kernel(const Append a) {
     const int page = a.n_kv > 0 ? page_of(a.block_table, a.bt_stride, a.n_pages, seq, pos) : -1;
     const int at = page < 0 ? 0 : pos % kPage;
     const float* row = reinterpret_cast<const float*>(a.qkv) + (size_t)t * a.ld;
-    // (all threads of a warp go round together: a round's last heads may not be there)
-    for (int h0 = blockIdx.y * kHeads; h0 < per_tok; h0 += gridDim.y * kHeads) {
+    // The heads of two rounds ahead are asked for before a round's are worked on.  (All threads of a warp go round together: a round's
+    // last heads may not be there.)
+    const int stride = gridDim.y * kHeads, first = blockIdx.y * kHeads + threadIdx.x / T;
+    auto ask = [&](int h) { return h < per_tok ? *reinterpret_cast<const float4*>(row + (size_t)h * D + 4 * j) : make_float4(0, 0, 0, 0); };
+    float4 v = ask(first), v1 = ask(first + stride), v2 = ask(first + 2 * stride);
+    for (int h0 = blockIdx.y * kHeads; h0 < per_tok; h0 += stride) {
         const int h = h0 + threadIdx.x / T;
         const bool there = h < per_tok;
-        float4 v = make_float4(0, 0, 0, 0);
-        if (there) v = *reinterpret_cast<const float4*>(row + (size_t)h * D + 4 * j);
+        if (h0 > blockIdx.y * kHeads) {
+            v = v1;
+            v1 = v2;
+            v2 = ask(h + 2 * stride);
+        }
         // a warp's heads are of one kind (all of q, all of k, ...) or take every branch that one of them takes
         const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv;
         if (__any_sync(0xffffffffu, there && is_q)) {
@@ -261,40 +268,49 @@ __global__ void __launch_bounds__(256) append_fast_kernel(const Append a) {
     }
 }
 
-// What the cache holds of given tokens: a thread takes four neighbouring lanes of a key and of a value.
+// What the cache holds of given tokens: a thread takes eight neighbouring lanes of a key and of a value.
+__device__ __forceinline__ void put8(void* out, long i, int dt, const float (&x)[8]) {
+    if (dt == DT_F32) {
+        reinterpret_cast<float4*>(out)[2 * i] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(out)[2 * i + 1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        uint32_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const __nv_bfloat162 two = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+            u[e] = *reinterpret_cast<const uint32_t*>(&two);
+        }
+        reinterpret_cast<uint4*>(out)[i] = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+}
 __global__ void __launch_bounds__(256) read_kernel(const uint8_t* k_pages, const uint8_t* v_pages, int n_pages, const int* block_table,
                                                    int bt_stride, const int* tok_seq, const int* tok_pos, void* k_out, void* v_out,
                                                    int out_dt, int n, int n_kv, int D) {
     wait_for_previous_kernels();
     let_next_kernel_start();
-    const int per_tok = n_kv * D / 4, NG = D / kGroup;
+    const int per_tok = n_kv * D / 8, NG = D / kGroup;
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
     if (i >= (long)n * per_tok) return;
-    const int t = (int)(i / per_tok), rest = (int)(i - (long)t * per_tok), h = rest / (D / 4), lane = (rest - h * (D / 4)) * 4, g = lane >> 5;
-    const int pos = tok_pos[t], page = page_of(block_table, bt_stride, n_pages, tok_seq[t], pos), at = page < 0 ? 0 : pos % kPage;
+    const int t = (int)(i / per_tok), rest = (int)(i - (long)t * per_tok), h = rest / (D / 8), lane = (rest - h * (D / 8)) * 8;
+    const int g = lane >> 5, c = (lane & 31) >> 3, pos = tok_pos[t];
+    const int page = page_of(block_table, bt_stride, n_pages, tok_seq[t], pos), at = page < 0 ? 0 : pos % kPage;
+    float k[8] = {}, v[8] = {};
+    if (page >= 0) {
+        const size_t base = ((size_t)page * n_kv + h) * q4_page_bytes(D);
+        const uint8_t *kb = k_pages + base, *vb = v_pages + base;
+        const uint32_t kw = reinterpret_cast<const uint32_t*>(kb)[q4_key_word(at, c, g, NG)];
+        const uint16_t* vh = reinterpret_cast<const uint16_t*>(vb) + (at & 1);
+        const uint32_t v0 = vh[2 * q4_value_word(at, 2 * c, g, NG)], v1 = vh[2 * q4_value_word(at, 2 * c + 1, g, NG)];
+        const float2 ks = __half22float2(reinterpret_cast<const __half2*>(kb + q4_scales_at(D))[at * NG + g]);
+        const float2 vs = __half22float2(reinterpret_cast<const __half2*>(vb + q4_scales_at(D))[at * NG + g]);
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (page >= 0) {
-            const uint8_t* base = (which ? v_pages : k_pages) + ((size_t)page * n_kv + h) * q4_page_bytes(D);
-            const int half = which ? 2 * q4_value_word(at, (lane & 31) >> 2, g, NG) + (at & 1)
-                                   : 2 * q4_key_word(at, (lane & 31) >> 3, g, NG) + (lane >> 2 & 1);
-            const uint32_t codes = reinterpret_cast<const uint16_t*>(base)[half];
-            const float2 dm = __half22float2(reinterpret_cast<const __half2*>(base + q4_scales_at(D))[at * NG + g]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = q4_number(codes >> (4 * e) & 15, dm);
-        }
-        void* out = which ? v_out : k_out;
-        if (out_dt == DT_F32) {
-            reinterpret_cast<float4*>(out)[i] = make_float4(x[0], x[1], x[2], x[3]);
-        } else {
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
-            uint2 u;
-            u.x = *reinterpret_cast<const uint32_t*>(&lo);
-            u.y = *reinterpret_cast<const uint32_t*>(&hi);
-            reinterpret_cast<uint2*>(out)[i] = u;
+        for (int e = 0; e < 8; ++e) {
+            k[e] = q4_number(kw >> (4 * e) & 15, ks);
+            v[e] = q4_number((e < 4 ? v0 : v1) >> (4 * (e & 3)) & 15, vs);
         }
     }
+    put8(k_out, i, out_dt, k);
+    put8(v_out, i, out_dt, v);
 }
 
 // The pages that a step's tokens see, as numbers in pages of their own: float16 or float32 rows of `lanes` >= D lanes, zeros behind a
@@ -444,7 +460,7 @@ extern "C" int nncpu_q4_read(const uint8_t* k_pages, const uint8_t* v_pages, int
     NN_CHECK(n >= 0 && n_kv > 0 && bt_stride > 0 && n_pages > 0, "q4_read: %d tokens, %d heads, %d pages", n, n_kv, n_pages);
     if (n == 0) return 0;
     NN_CHECK((uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0, "q4_read: outputs start on 16-byte boundaries");
-    const long items = (long)n * n_kv * D / 4;
+    const long items = (long)n * n_kv * D / 8;
     NN_CHECK(items / 256 < (1L << 31), "q4_read: %d tokens", n);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((items + 255) / 256));
