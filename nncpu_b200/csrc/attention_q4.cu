@@ -88,12 +88,15 @@ constexpr int kTiles = 2;                   // tensor-core tiles of 16 keys that
 struct Stream {
     int heads;              // query heads of a pair (a part of those that share a key/value head where these are many)
     int chunks;             // such parts of a key/value head
-    int pairs;              // n_kv * chunks: pairs of a token
+    int pairs;              // n_kv * chunks: pairs of a tile
+    int tile;               // tokens of a tile: 1, or (cu not null) several neighbours of the step's one sequence
+    int tiles;              // tiles of the step
+    const int* cu;          // or null: the first token of the step's one sequence, and the first behind it
     int min_places;         // places of the row that a block takes at least
     int blocks;             // blocks of the launch
     float scale2;           // scale * log2(e)
     ScoreCap cap;
-    int2* parts;            // [n, pairs]: the first block that has a part of a pair, and the last
+    int2* parts;            // [tiles, pairs]: the first block that has a part of a pair, and the last
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -165,11 +168,32 @@ __device__ __forceinline__ void lds_words(uint32_t (&w)[N], const uint8_t* p) {
     }
 }
 
-// The pages that a token sees (none for a row of no sequence).
-__device__ __forceinline__ int pages_of(const AttnQ4& p, int t) {
-    const int pos = p.tok_pos[t];
-    if (p.tok_seq[t] < 0 || pos < 0) return 0;
-    return PageWalk(first_visible_key(pos, p.window), pos, p.keep).n;
+// A tile: its first token, how many it has (0: it is of no sequence), the positions of the first and the last, the first key that one of
+// them sees.
+struct Tile {
+    int t0, count, pos, last, first;
+};
+template <bool TILED>
+__device__ __forceinline__ Tile tile_of(const AttnQ4& p, const Stream& st, int i) {
+    Tile w{i, 1, 0, 0, 0};
+    if (TILED && st.cu != nullptr) {
+        w.t0 = st.cu[0] + i * st.tile;
+        w.count = max(0, min(st.tile, st.cu[1] - w.t0));
+    }
+    if (w.count > 0) {
+        w.pos = p.tok_pos[w.t0];
+        const int seq = p.tok_seq[w.t0];        // (both asked for at once)
+        if (min(w.pos, seq) < 0) w.count = 0;
+    }
+    w.last = w.pos + w.count - 1;
+    w.first = first_visible_key(w.pos, p.window);
+    return w;
+}
+// The pages that a tile sees.
+template <bool TILED>
+__device__ __forceinline__ int pages_of(const AttnQ4& p, const Stream& st, int i) {
+    const Tile w = tile_of<TILED>(p, st, i);
+    return w.count > 0 ? PageWalk(w.first, w.last, p.keep).n : 0;
 }
 
 // How the row of pairs is cut.  A pair is kPairCost places and then its pages, one place each: what a block does once for a pair (queries
@@ -183,11 +207,12 @@ struct Row {
         return place < at ? place / (each + 1) : more + (place - at) / each;
     }
 };
-// (Every warp by itself, 32 tokens at a time; `mine`: the pages of token `lane`, which are asked for once.)
+// (Every warp by itself, 32 tokens at a time; `mine`: the pages of tile `lane`, which are asked for once.)
+template <bool TILED>
 __device__ __forceinline__ Row row_of(const AttnQ4& p, const Stream& st, int lane, int mine) {
     unsigned sum = mine > 0 ? mine + kPairCost : 0;
-    for (int t = lane + 32; t < p.n; t += 32) {
-        const int n = pages_of(p, t);
+    for (int t = lane + 32; t < st.tiles; t += 32) {
+        const int n = pages_of<TILED>(p, st, t);
         sum += n > 0 ? n + kPairCost : 0;
     }
     Row row;
@@ -198,23 +223,25 @@ __device__ __forceinline__ Row row_of(const AttnQ4& p, const Stream& st, int lan
     return row;
 }
 
-// Where a block is: page i of the n that pair y of token t walks through, and how many places are left to it.
+// Where a block is: page i of the n that pair y of tile t walks through, and how many places are left to it.
 struct Place {
     int t, y, i, n, left;
     // to the next pair with pages
+    template <bool TILED>
     __device__ __forceinline__ void next_pair(const AttnQ4& p, const Stream& st) {
         i = 0;
         left -= kPairCost;
         if (++y == st.pairs) {
             y = 0;
-            do { ++t; } while (t < p.n && (n = pages_of(p, t)) == 0);
+            do { ++t; } while (t < st.tiles && (n = pages_of<TILED>(p, st, t)) == 0);
         }
     }
 };
+template <bool TILED>
 __device__ __forceinline__ Place place_of(const AttnQ4& p, const Stream& st, unsigned place, int left, int lane, int mine) {
     unsigned before = 0;
     for (int t0 = 0;; t0 += 32) {
-        const int n = t0 == 0 ? mine : t0 + lane < p.n ? pages_of(p, t0 + lane) : 0;
+        const int n = t0 == 0 ? mine : t0 + lane < st.tiles ? pages_of<TILED>(p, st, t0 + lane) : 0;
         const unsigned places = n > 0 ? n + kPairCost : 0;
         unsigned upto = places;
 #pragma unroll
@@ -223,7 +250,7 @@ __device__ __forceinline__ Place place_of(const AttnQ4& p, const Stream& st, uns
             if (lane >= o) upto += v;
         }
         const unsigned beyond = __ballot_sync(0xffffffffu, before + upto * st.pairs > place);
-        if (beyond != 0 || t0 + 32 >= p.n) {
+        if (beyond != 0 || t0 + 32 >= st.tiles) {
             const int l = beyond != 0 ? __ffs(beyond) - 1 : 31;
             const unsigned of_pair = __shfl_sync(0xffffffffu, places, l);
             const unsigned rest = place - before - (__shfl_sync(0xffffffffu, upto, l) - of_pair) * st.pairs;
@@ -246,12 +273,12 @@ __device__ __forceinline__ Place place_of(const AttnQ4& p, const Stream& st, uns
 constexpr float kLag = 4.0f;
 __device__ __forceinline__ float headroom(float d_max) { return d_max <= 1.0f ? 11.0f : 11.0f - ceilf(log2f(d_max)); }
 
-// Rows of no sequence are zeros, and in one part.
-template <int D>
+// Tiles of no sequence are in one part, and (token by token) zeros.
+template <int D, bool TILED>
 __device__ __forceinline__ void zero_rows(const AttnQ4& p, const Stream& st) {
-    for (int t = blockIdx.x; t < p.n; t += gridDim.x) {
-        if (pages_of(p, t) > 0) continue;
-        for (int i = threadIdx.x; i < p.n_heads * D / 8; i += 32 * kStreamWarps)
+    for (int t = blockIdx.x; t < st.tiles; t += gridDim.x) {
+        if (pages_of<TILED>(p, st, t) > 0) continue;
+        for (int i = threadIdx.x; st.cu == nullptr && i < p.n_heads * D / 8; i += 32 * kStreamWarps)
             reinterpret_cast<uint4*>(p.out)[(size_t)t * p.n_heads * D / 8 + i] = make_uint4(0, 0, 0, 0);
         for (int i = threadIdx.x; i < st.pairs; i += 32 * kStreamWarps) st.parts[(size_t)t * st.pairs + i] = make_int2(0, 0);
     }
@@ -260,6 +287,7 @@ __device__ __forceinline__ void zero_rows(const AttnQ4& p, const Stream& st) {
 template <int NG, int NT>
 __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_kernel(const AttnQ4 p, const Stream st) {
     constexpr int D = 32 * NG, COLS = 8 * NT;
+    constexpr bool TILED = NT == 2;       // a tile may have several tokens
     constexpr int kCodes = 256 * NG, kScales = 64 * NG;          // bytes of a tile's 16 keys
     constexpr int kVCodes = kTiles * kCodes, kKScales = 2 * kVCodes, kVScales = kKScales + kTiles * kScales, kStage = 2 * kTiles * (kCodes + kScales);
     constexpr unsigned kPageBytes = 40 * D;
@@ -270,27 +298,30 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
     float* meet = reinterpret_cast<float*>(stream_smem + kStreamWarps * kStreamStages * kStage);   // [COLS][D + 4]: lanes, reference, sum
     wait_for_previous_kernels();
     let_next_kernel_start();
-    const int my_pages = lane < p.n ? pages_of(p, lane) : 0;
-    const Row row = row_of(p, st, lane, my_pages);
+    const int my_pages = lane < st.tiles ? pages_of<TILED>(p, st, lane) : 0;
+    const Row row = row_of<TILED>(p, st, lane, my_pages);
     if ((int)blockIdx.x >= row.blocks) {
-        zero_rows<D>(p, st);
+        zero_rows<D, TILED>(p, st);
         return;
     }
     const unsigned first_place = row.start(blockIdx.x);
-    Place here = place_of(p, st, first_place, (int)(row.start(blockIdx.x + 1) - first_place), lane, my_pages), ahead = here;
-    // the queries of a pair, as they lie: head r of the column tile, lanes 32 g + 8 c to + 7
+    Place here = place_of<TILED>(p, st, first_place, (int)(row.start(blockIdx.x + 1) - first_place), lane, my_pages), ahead = here;
+    // The columns of a pair are its tile's tokens times its heads.  Their queries, as they lie: column r of each eight, lanes 32 g + 8 c to + 7.
+    const int group = p.n_heads / p.n_kv;
     uint4 raw[NT][NG];
     auto ask_queries = [&]() {
-        const int kvh = here.y / st.chunks, part = here.y - kvh * st.chunks, group = p.n_heads / p.n_kv;
-        const int nh = here.left > 0 ? min(st.heads, group - part * st.heads) : 0;
-        const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q) + ((size_t)here.t * p.n_heads + kvh * group + part * st.heads) * D + 8 * c;
+        const int kvh = here.y / st.chunks, part = here.y - kvh * st.chunks, heads = min(st.heads, group - part * st.heads);
+        const Tile w = here.left > 0 ? tile_of<TILED>(p, st, here.t) : Tile{0, 0, 0, 0, 0};
+        const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q) + ((size_t)w.t0 * p.n_heads + kvh * group + part * st.heads) * D + 8 * c;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+            const int at = !TILED || st.tile == 1 ? 0 : (8 * nt + r) / heads, h = 8 * nt + r - at * heads;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 raw[nt][g] = make_uint4(0, 0, 0, 0);
-                if (8 * nt + r < nh) raw[nt][g] = *reinterpret_cast<const uint4*>(q + (8 * nt + r) * D + 32 * g);
+                if (at < w.count && h < heads) raw[nt][g] = *reinterpret_cast<const uint4*>(q + ((size_t)at * p.n_heads + h) * D + 32 * g);
             }
+        }
     };
     ask_queries();
     unsigned there = 0;                     // bit s: stage s holds a page (and not one that is missing)
@@ -302,12 +333,12 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
     auto fetch = [&](int stage) {
         if (ahead.left > 0) {
             if (id_at == id_end) {
-                const int pos = p.tok_pos[ahead.t];
-                const PageWalk walk(first_visible_key(pos, p.window), pos, p.keep);
+                const Tile w = tile_of<TILED>(p, st, ahead.t);
+                const PageWalk walk(w.first, w.last, p.keep);
                 id_at = 0;
                 id_end = min(32, ahead.n - ahead.i);
                 const int pi = walk.page(min(ahead.i + lane, ahead.n - 1));
-                ids = pi < p.bt_stride ? p.block_table[(size_t)p.tok_seq[ahead.t] * p.bt_stride + pi] : -1;
+                ids = pi < p.bt_stride ? p.block_table[(size_t)p.tok_seq[w.t0] * p.bt_stride + pi] : -1;
                 if (ids >= p.n_pages) ids = -1;
                 const size_t head = (size_t)(ahead.y / st.chunks) * kPageBytes + lane * 16;
                 kc = p.k_pages + head + warp * kTiles * kCodes;
@@ -332,7 +363,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
                 there &= ~(1u << stage);
             }
             --ahead.left;
-            if (++ahead.i == ahead.n) ahead.next_pair(p, st);
+            if (++ahead.i == ahead.n) ahead.template next_pair<TILED>(p, st);
         }
         cp_async_commit();
     };
@@ -346,10 +377,17 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
         const int t = here.t, y = here.y, from = here.i, take = min(here.n - from, here.left);
         const int n_pages = here.n;
         const bool whole = take == n_pages;
-        const int kvh = y / st.chunks, h0 = kvh * (p.n_heads / p.n_kv) + (y - kvh * st.chunks) * st.heads;
-        const int nh = min(st.heads, (kvh + 1) * (p.n_heads / p.n_kv) - h0);
-        const int pos = p.tok_pos[t], first = first_visible_key(pos, p.window);
-        const PageWalk walk(first, pos, p.keep);
+        const int kvh = y / st.chunks, h0 = kvh * group + (y - kvh * st.chunks) * st.heads, heads = min(st.heads, (kvh + 1) * group - h0);
+        const Tile tile = tile_of<TILED>(p, st, t);
+        const int count = TILED ? tile.count : 1, t0 = TILED ? tile.t0 : t, nh = heads * count;      // tokens, and columns
+        const int pos = tile.pos, last = TILED ? tile.last : pos, first = tile.first, first_last = TILED ? first_visible_key(last, p.window) : first;
+        const PageWalk walk(first, last, p.keep);
+        // this thread's columns 2 c and 2 c + 1 of each eight: which token of the tile
+        int tok[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) tok[nt][e] = !TILED || st.tile == 1 ? 0 : min((8 * nt + 2 * c + e) / heads, count - 1);
         // Queries as the right-hand operand: head r of the column tile, the lanes of word (c, g), in the order of the codes' pairs.
         uint32_t qb[NT][NG][4];
         uint32_t qhi[NT], qlo[NT];     // the right-hand operand of (d_c, m_c): (-off, sum of q) of group c and head r, in two parts
@@ -403,7 +441,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
         float od[NT][4];
         float m[NT][2];                       // the weights' reference (0 until a key has been seen)
         float d_max = 1.0f, room = 11.0f;     // greatest step that the references leave room for, and how much that is
-        bool fresh = true;                    // no key has been seen
+        unsigned seen = 0;                    // bit 2 nt + e: this thread's column e of the eight has seen a key
+        bool all_seen = false;                // every column of the warp has
         const uint32_t ones = r == 0 ? 0x3C003C00u : 0u;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -422,12 +461,12 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
             stage = stage == kStreamStages - 1 ? 0 : stage + 1;
             const int key0 = pi * kPage + 16 * kTiles * warp;
             pi = from + i + 1 == walk.n_kept ? walk.lo : pi + 1;
-            if (missing || key0 > pos || (key0 + 16 * kTiles - 1 < first && key0 >= p.keep)) continue;      // none of these keys is seen
-            const bool full = key0 >= first && key0 + 16 * kTiles - 1 <= pos;
+            if (missing || key0 > last || (key0 + 16 * kTiles - 1 < first && key0 >= p.keep)) continue;      // none of these keys is seen
+            const bool full = key0 >= first_last && key0 + 16 * kTiles - 1 <= pos;                          // all of them by all
             if (!full) {
                 // what is not seen may hold anything, NaN too: its weight will be zero, and so must its numbers be
                 const int key = key0 + lane;
-                if (key > pos || (key < first && key >= p.keep))
+                if (key > last || (key < first && key >= p.keep))
 #pragma unroll
                     for (int g = 0; g < NG; ++g) *reinterpret_cast<uint32_t*>(at + kVScales + lane * 4 * NG + g * 4) = 0;
                 __syncwarp();
@@ -486,7 +525,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
             }
             if (r & 1) step = 0.0f;
             // -- weights: first what 2 is raised to
-            bool moves = fresh | (step > d_max);
+            bool moves = step > d_max;
             if (full && p.slope_base == 0.0f && st.cap.out == 0.0f) {
 #pragma unroll
                 for (int kt = 0; kt < kTiles; ++kt)
@@ -504,21 +543,31 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int key = key0 + 16 * kt + r + 8 * (e >> 1);
+                            const int key = key0 + 16 * kt + r + 8 * (e >> 1), at_pos = TILED ? pos + tok[nt][e & 1] : pos;
                             float v = z[kt][nt][e] * col[nt][e & 1];
                             if (st.cap.out > 0.0f) v = capped_score(v, st.cap);
-                            if (p.slope_base != 0.0f) v -= slope_of(p, h0 + 8 * nt + 2 * c + (e & 1)) * kLog2e * (float)(pos - key);
+                            if (p.slope_base != 0.0f)
+                                v -= slope_of(p, h0 + 8 * nt + 2 * c + (e & 1) - tok[nt][e & 1] * heads) * kLog2e * (float)(at_pos - key);
                             v -= m[nt][e & 1];
-                            if (key > pos || (key < first && key >= p.keep)) v = -INFINITY;
+                            if (key > at_pos || (key < first_visible_key(at_pos, p.window) && key >= p.keep)) v = -INFINITY;
                             z[kt][nt][e] = v;
                             moves |= v > room + kLag;
                         }
             }
+            if (!TILED) moves |= !all_seen;      // (every column sees the same keys: the first are the first of all)
+            if (TILED && !all_seen)
+#pragma unroll
+                for (int kt = 0; kt < kTiles; ++kt)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) moves |= !(seen >> (2 * nt + (e & 1)) & 1) && z[kt][nt][e] > -INFINITY;
             if (__any_sync(0xffffffffu, moves)) {
                 float d = step;
 #pragma unroll
                 for (int x = 1; x < 32; x <<= 1) d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, x));
                 d_max = fmaxf(d_max, d);
+                const bool was_seen = all_seen;
                 const float less = room - headroom(d_max);
                 room -= less;
 #pragma unroll
@@ -531,9 +580,11 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
                         // by how much the reference rises (the first time it may fall)
-                        float rise = fresh ? mx - room : fmaxf(less, mx - room);
-                        if (mx == -INFINITY) rise = fresh ? 0.0f : less;
-                        const float corr = fresh ? 1.0f : fast_exp2(0.0f - rise);
+                        const bool unseen = TILED ? !(seen >> (2 * nt + e) & 1) : !was_seen;
+                        float rise = unseen ? mx - room : fmaxf(less, mx - room);
+                        if (mx == -INFINITY) rise = unseen ? 0.0f : less;
+                        else if (TILED) seen |= 1u << (2 * nt + e);
+                        const float corr = unseen ? 1.0f : fast_exp2(0.0f - rise);
                         m[nt][e] += rise;
                         od[nt][e] *= corr;
                         od[nt][e + 2] *= corr;
@@ -548,7 +599,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
                             o[nt][k][e + 2] *= corr;
                         }
                     }
-                fresh = false;
+                all_seen = !TILED || __all_sync(0xffffffffu, seen == (1u << (2 * NT)) - 1);
             }
             // -- values
 #pragma unroll
@@ -582,7 +633,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
         here.i += take;
         here.left -= take;
         const int left = here.left;
-        if (here.i == here.n) here.next_pair(p, st);
+        if (here.i == here.n) here.template next_pair<TILED>(p, st);
         ask_queries();
         if (from == 0 && threadIdx.x == 0)      // the first block with a part of the pair, and the last
             st.parts[(size_t)t * st.pairs + y] =
@@ -601,7 +652,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
                     if ((e == warp) != (pass == 1)) continue;
                     const int h = 8 * nt + 2 * c + e;
                     float* other = meet + h * (D + 4);
-                    const float sum = __shfl_sync(0xffffffffu, od[nt][e + 2], c), ref = fresh ? -INFINITY : m[nt][e];
+                    const float sum = __shfl_sync(0xffffffffu, od[nt][e + 2], c), ref = (TILED ? seen >> (2 * nt + e) & 1 : all_seen) ? m[nt][e] : -INFINITY;
                     float f0 = 1.0f, f1 = 0.0f, top = ref, total = sum;
                     if (pass == 1) {
                         top = fmaxf(ref, other[D]);
@@ -609,7 +660,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
                         f1 = other[D] == -INFINITY ? 0.0f : exp2f(other[D] - top);
                         total = fmaf(other[D + 1], f1, sum * f0);
                         if (whole && h < nh) {
-                            const float f = closing_factor(p, t, h0 + h, top / kLog2e, total);
+                            const float f = closing_factor(p, t0 + tok[nt][e], h0 + h - tok[nt][e] * heads, top / kLog2e, total);
                             f0 *= f;
                             f1 *= f;
                         }
@@ -629,7 +680,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
                         if (whole) {
                             const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
                             const uint2 packed = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-                            *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + ((size_t)t * p.n_heads + h0 + h) * D + d) = packed;
+                            *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + ((size_t)(t0 + tok[nt][e]) * p.n_heads + h0 + h - tok[nt][e] * heads) * D + d) = packed;
                         } else {
                             *reinterpret_cast<float4*>(p.part + ((size_t)slot * COLS + h) * (D + 4) + d) = v;
                         }
@@ -647,17 +698,20 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
         }
     }
     cp_async_wait<0>();
-    zero_rows<D>(p, st);
+    zero_rows<D, TILED>(p, st);
 }
 
-// The parts of a pair that lies in several blocks, in the order of its keys.  grid = (n, pairs, heads of a pair), a thread a lane.
+// The parts of a pair that lies in several blocks, in the order of its keys.  grid = (tiles, pairs, columns of a pair), a thread a lane.
 __global__ void __launch_bounds__(128) stream_merge_kernel(const AttnQ4 p, const Stream st, int cols) {
-    const int t = blockIdx.x, y = blockIdx.y, h = blockIdx.z, D = p.D, d = threadIdx.x;
+    const int y = blockIdx.y, h = blockIdx.z, D = p.D, d = threadIdx.x;
     wait_for_previous_kernels();
     let_next_kernel_start();
-    const int2 b = st.parts[(size_t)t * st.pairs + y];
-    const int kvh = y / st.chunks, h0 = kvh * (p.n_heads / p.n_kv) + y % st.chunks * st.heads;
-    if (b.x == b.y || h0 + h >= (kvh + 1) * (p.n_heads / p.n_kv)) return;       // that block has finished it; no such head
+    const int2 b = st.parts[(size_t)blockIdx.x * st.pairs + y];
+    if (b.x == b.y) return;              // that block has finished it
+    const Tile tile = st.cu == nullptr ? Tile{(int)blockIdx.x, 1, 0, 0, 0} : tile_of<true>(p, st, blockIdx.x);
+    const int group = p.n_heads / p.n_kv, kvh = y / st.chunks, h0 = kvh * group + y % st.chunks * st.heads;
+    const int heads = min(st.heads, (kvh + 1) * group - h0), tok = h / heads, head = h0 + h - tok * heads;
+    if (tok >= tile.count) return;       // no such column
     // the first part is its block's last, the others are their blocks' first
     const size_t step = (size_t)2 * cols * (D + 4);
     const float* first = p.part + ((size_t)(2 * b.x + 1) * cols + h) * (D + 4);
@@ -675,8 +729,8 @@ __global__ void __launch_bounds__(128) stream_merge_kernel(const AttnQ4 p, const
         sum = fmaf(from[D + 1], f, sum);
         out = fmaf(from[d], f, out);
     }
-    f = closing_factor(p, t, h0 + h, top / kLog2e, sum);
-    reinterpret_cast<__nv_bfloat16*>(p.out)[((size_t)t * p.n_heads + h0 + h) * D + d] = __float2bfloat16_rn(out * f);
+    f = closing_factor(p, tile.t0 + tok, head, top / kLog2e, sum);
+    reinterpret_cast<__nv_bfloat16*>(p.out)[((size_t)(tile.t0 + tok) * p.n_heads + head) * D + d] = __float2bfloat16_rn(out * f);
 }
 
 // Pages of a token's walk that split s takes: [first, end).
@@ -888,19 +942,22 @@ static int stream_blocks(int D, int tiles) {
 extern "C" long nncpu_attention_q4_scratch(int n, int n_heads, int n_kv, int D, int dt, int longest) {
     if (n <= 0 || !sizes_ok(n, n_heads, n_kv, D)) return 0;
     if (streams(dt, D)) {
-        const int tiles = stream_tiles(n_heads, n_kv);
-        const int group = n_heads / n_kv, chunks = (group + 8 * tiles - 1) / (8 * tiles);
-        return 2L * stream_blocks(D, tiles) * 8 * tiles * (D + 4) + 2L * n * n_kv * chunks;
+        // (enough for one column tile and for two, and for parts token by token)
+        const int group = n_heads / n_kv, chunks = (group + 7) / 8;
+        const long one = 8L * stream_blocks(D, 1), two = 16L * stream_blocks(D, 2);
+        return 2L * (one > two ? one : two) * (D + 4) + 2L * n * n_kv * chunks;
     }
     const int s = any_splits(n, n_heads, n_kv, longest);
     return s > 1 ? (long)n * n_heads * s * (D + 2) : 0;
 }
 
+// one_seq (bfloat16, at most 128 lanes): the tokens are those of ONE sequence, at consecutive positions, from one_seq[0] to before
+// one_seq[1] of the n; several of them then go through the pages together.
 extern "C" int nncpu_attention_q4(const void* q, int dt, const uint8_t* k_pages, const uint8_t* v_pages, int n_pages,
                                   const int* block_table, int bt_stride, const int* tok_seq, const int* tok_pos, void* out, float* part,
                                   long part_floats, int n, int n_heads, int n_kv, int D, float scale, int window, int keep,
                                   float slope_base, const float* sinks, float cap, const float* head_gate, int gate_ld, int longest,
-                                  cudaStream_t stream) {
+                                  const int* one_seq, cudaStream_t stream) {
     NN_CHECK(sizes_ok(n, n_heads, n_kv, D), "attention_q4: %d tokens, %d heads over %d of %d lanes (whole groups of 32, at most 256)", n, n_heads, n_kv, D);
     NN_CHECK(cap >= 0.0f && keep >= 0 && (keep == 0 || window > 0) && (head_gate == nullptr || gate_ld >= n_heads),
              "attention_q4: cap %f, %d kept keys, gate rows of %d", cap, keep, gate_ld);
@@ -914,10 +971,14 @@ extern "C" int nncpu_attention_q4(const void* q, int dt, const uint8_t* k_pages,
     if (streams(dt, D)) {
         NN_CHECK((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)part % 16 == 0,
                  "attention_q4: bfloat16 queries, output and scratch start on 16-byte boundaries");
-        const int tiles = stream_tiles(n_heads, n_kv), chunks = (group + 8 * tiles - 1) / (8 * tiles);
-        NN_CHECK((long)n * n_kv * chunks * (bt_stride + 3L) < (1L << 31), "attention_q4: %d tokens of up to %d pages", n, bt_stride);
+        // several tokens of one sequence: in two column tiles, as many as have columns there
+        const int tiles = one_seq != nullptr && n > 1 ? 2 : stream_tiles(n_heads, n_kv), chunks = (group + 8 * tiles - 1) / (8 * tiles);
+        const int heads = (group + chunks - 1) / chunks, tile = one_seq != nullptr && n > 1 ? 16 / heads : 1;
+        const int n_tiles = (n + tile - 1) / tile;
+        NN_CHECK((long)n_tiles * n_kv * chunks * (bt_stride + 3L) < (1L << 31), "attention_q4: %d tokens of up to %d pages", n, bt_stride);
         NN_CHECK(n_kv <= 65535 / chunks, "attention_q4: %d key/value heads in %d parts", n_kv, chunks);
-        Stream st{(group + chunks - 1) / chunks, chunks, n_kv * chunks, kStreamMinPlaces, stream_blocks(D, tiles), scale * kLog2e, score_cap(scale, cap), nullptr};
+        Stream st{heads, chunks, n_kv * chunks, tile, n_tiles, one_seq, kStreamMinPlaces, stream_blocks(D, tiles), scale * kLog2e,
+                  score_cap(scale, cap), nullptr};
         st.parts = reinterpret_cast<int2*>(part + 2L * st.blocks * 8 * tiles * (D + 4));
         // All blocks of the first kernel have to run at once, six to an SM, so it is not launched to start under the end of the one
         // before: beside blocks of that one an SM may find room for five, and the sixth, begun when those are done, doubles the time
@@ -932,7 +993,7 @@ extern "C" int nncpu_attention_q4(const void* q, int dt, const uint8_t* k_pages,
         cfg.numAttrs = 0;
         cudaError_t e = cudaLaunchKernelEx(&cfg, stream_kernel_of(D, tiles), p, st);
         NN_CHECK(e == cudaSuccess, "attention_q4: launch failed: %s", cudaGetErrorString(e));
-        cfg.gridDim = dim3((unsigned)n, (unsigned)st.pairs, (unsigned)st.heads);
+        cfg.gridDim = dim3((unsigned)n_tiles, (unsigned)st.pairs, (unsigned)(st.heads * tile));
         cfg.blockDim = dim3(D);
         cfg.dynamicSmemBytes = 0;
         cfg.numAttrs = overlap_attribute(attr);

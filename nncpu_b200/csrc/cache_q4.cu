@@ -315,10 +315,8 @@ __global__ void __launch_bounds__(256) read_kernel(const uint8_t* k_pages, const
 
 // The pages that a step's tokens see, as numbers in pages of their own: float16 or float32 rows of `lanes` >= D lanes, zeros behind a
 // head's own and in rows behind the sequence's end (whatever the cache holds there).  Page i of sequence b goes to page b * width + i,
-// and the table for the attention kernels is written too.  grid = (width, n_kv, n_seqs).
-//
-// A page's codes and scales come to shared memory as they lie; then a thread writes 16 neighbouring bytes of a row of keys (a word's
-// eight lanes), or 8 of one of values (four lanes), neighbouring threads of a row next to each other.
+// and the table for the attention kernels is written too.  A block takes a page of keys or of values of one head, a thread eight
+// neighbouring lanes of a row at a time: grid = (width, 2 n_kv, n_seqs).
 struct Expand {
     const uint8_t* k_pages;
     const uint8_t* v_pages;
@@ -333,64 +331,57 @@ struct Expand {
     int n_kv, D, lanes, window, keep;
 };
 
-__device__ __forceinline__ float q4_as_half_can(float v) { return q4_in_range(v); }      // (d c + m may pass the range by a rounding)
-
-template <typename T>
-__device__ __forceinline__ void put4(T* row, float a, float b, float c, float d);
-template <>
-__device__ __forceinline__ void put4<float>(float* row, float a, float b, float c, float d) {
-    *reinterpret_cast<float4*>(row) = make_float4(a, b, c, d);
+__device__ __forceinline__ void put8_row(float* row, const float (&x)[8]) {
+    reinterpret_cast<float4*>(row)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(row)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
-template <>
-__device__ __forceinline__ void put4<__half>(__half* row, float a, float b, float c, float d) {
-    const __half2 lo = __floats2half2_rn(q4_as_half_can(a), q4_as_half_can(b)), hi = __floats2half2_rn(q4_as_half_can(c), q4_as_half_can(d));
-    uint2 u;
-    u.x = *reinterpret_cast<const uint32_t*>(&lo);
-    u.y = *reinterpret_cast<const uint32_t*>(&hi);
-    *reinterpret_cast<uint2*>(row) = u;
+__device__ __forceinline__ void put8_row(__half* row, const float (&x)[8]) {
+    uint32_t u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {       // (d c + m may pass the range by a rounding)
+        const __half2 two = __floats2half2_rn(q4_in_range(x[2 * e]), q4_in_range(x[2 * e + 1]));
+        u[e] = *reinterpret_cast<const uint32_t*>(&two);
+    }
+    *reinterpret_cast<uint4*>(row) = make_uint4(u[0], u[1], u[2], u[3]);
 }
 
 constexpr int kExpandThreads = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const Expand p) {
-    __shared__ __align__(16) uint8_t page[40 * 256];
     wait_for_previous_kernels();       // (before anything is read: the kernel after this one reads the step's metadata before it waits)
     let_next_kernel_start();
-    const int pi = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
-    const int row = b * gridDim.x + pi;
-    if (h == 0 && tid == 0) p.table[row] = row;
+    const int pi = blockIdx.x, b = blockIdx.z, row = b * gridDim.x + pi;
+    const bool values = blockIdx.y >= p.n_kv;
+    const int h = values ? blockIdx.y - p.n_kv : blockIdx.y;
+    if (blockIdx.y == 0 && threadIdx.x == 0) p.table[row] = row;
     const int t0 = p.cu_seqlens[b], t1 = p.cu_seqlens[b + 1];
     if (t1 <= t0) return;
     const int first = first_visible_key(p.tok_pos[t0], p.window), last = p.tok_pos[t1 - 1];
     if (pi * kPage > last || (pi * kPage + kPage - 1 < first && pi * kPage >= p.keep)) return;      // no token sees the page
     int id = pi < p.bt_stride ? p.block_table[(size_t)b * p.bt_stride + pi] : -1;
     if (id >= p.n_pages) id = -1;
-    const int D = p.D, NG = D / kGroup, rows = id < 0 ? 0 : min(kPage, last + 1 - pi * kPage);
-    for (int which = 0; which < 2; ++which) {
-        const bool values = which == 1;
-        T* out = reinterpret_cast<T*>(values ? p.v_out : p.k_out) + ((size_t)row * p.n_kv + h) * kPage * p.lanes;
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(page);
-        const __half2* scales = reinterpret_cast<const __half2*>(page + q4_scales_at(D));
-        if (rows > 0) {
-            const uint4* src = reinterpret_cast<const uint4*>((values ? p.v_pages : p.k_pages) + ((size_t)id * p.n_kv + h) * q4_page_bytes(D));
-            __syncthreads();
-            for (int i = tid; i < (int)q4_page_bytes(D) / 16; i += kExpandThreads) reinterpret_cast<uint4*>(page)[i] = src[i];
-            __syncthreads();
-        }
-        // four lanes at a time
-        for (int i = tid; i < kPage * p.lanes / 4; i += kExpandThreads) {
-            const int at = i / (p.lanes / 4), lane = i % (p.lanes / 4) * 4, g = lane >> 5;
-            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (at < rows && lane < D) {
-                const uint32_t u = values ? words[q4_value_word(at, (lane & 31) >> 2, g, NG)] >> (16 * (at & 1))
-                                          : words[q4_key_word(at, (lane & 31) >> 3, g, NG)] >> (4 * (lane & 4));
-                const float2 dm = __half22float2(scales[at * NG + g]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = q4_number(u >> (4 * j) & 15, dm);
+    const int D = p.D, NG = D / kGroup, rows = id < 0 ? 0 : min(kPage, last + 1 - pi * kPage), per_row = p.lanes / 8;
+    const uint8_t* base = (values ? p.v_pages : p.k_pages) + ((size_t)max(id, 0) * p.n_kv + h) * q4_page_bytes(D);
+    const __half2* scales = reinterpret_cast<const __half2*>(base + q4_scales_at(D));
+    T* out = reinterpret_cast<T*>(values ? p.v_out : p.k_out) + ((size_t)row * p.n_kv + h) * kPage * p.lanes;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kPage * per_row; i += kExpandThreads) {
+        const int at = i / per_row, lane = (i - at * per_row) * 8, g = lane >> 5, c = (lane & 31) >> 3;
+        float x[8] = {};
+        if (at < rows && lane < D) {
+            uint32_t u;
+            if (values) {
+                const uint16_t* half = reinterpret_cast<const uint16_t*>(base) + (at & 1);
+                u = half[2 * q4_value_word(at, 2 * c, g, NG)] | (uint32_t)half[2 * q4_value_word(at, 2 * c + 1, g, NG)] << 16;
+            } else {
+                u = reinterpret_cast<const uint32_t*>(base)[q4_key_word(at, c, g, NG)];
             }
-            put4<T>(out + (size_t)at * p.lanes + lane, x[0], x[1], x[2], x[3]);
+            const float2 dm = __half22float2(scales[at * NG + g]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = q4_number(u >> (4 * e) & 15, dm);
         }
+        put8_row(out + (size_t)at * p.lanes + lane, x);
     }
 }
 
@@ -481,7 +472,7 @@ extern "C" int nncpu_q4_expand(const uint8_t* k_pages, const uint8_t* v_pages, i
                                int keep, int half, void* k_out, void* v_out, int* table, const void* q, void* q_out, int n_tok, int n_heads,
                                cudaStream_t stream) {
     NN_CHECK(q4_lanes_ok(D) && lanes >= D && lanes % 8 == 0, "q4_expand: heads of %d lanes in rows of %d", D, lanes);
-    NN_CHECK(n_seqs > 0 && n_seqs <= 65535 && width > 0 && n_kv > 0 && n_kv <= 65535 && n_pages > 0 && bt_stride > 0,
+    NN_CHECK(n_seqs > 0 && n_seqs <= 65535 && width > 0 && n_kv > 0 && n_kv <= 32767 && n_pages > 0 && bt_stride > 0,
              "q4_expand: %d sequences of %d pages, %d heads", n_seqs, width, n_kv);
     if (q != nullptr && n_tok > 0) {
         const long pieces = (long)n_tok * n_heads * lanes / 8;
@@ -490,7 +481,7 @@ extern "C" int nncpu_q4_expand(const uint8_t* k_pages, const uint8_t* v_pages, i
     }
     const Expand p{k_pages, v_pages, n_pages, block_table, bt_stride, cu_seqlens, tok_pos, k_out, v_out, table, n_kv, D, lanes, window, keep};
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)width, (unsigned)n_kv, (unsigned)n_seqs);
+    cfg.gridDim = dim3((unsigned)width, (unsigned)(2 * n_kv), (unsigned)n_seqs);
     cfg.blockDim = dim3(kExpandThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

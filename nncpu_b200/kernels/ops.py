@@ -1597,7 +1597,7 @@ def _launch(libname: str, fn: str, types, *args) -> None:
         found = _typed[fn] = (f, lib)
     if _dry:
         return
-    dev = torch._C._cuda_getDevice()
+    dev = _cuda_device()
     stream = _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
     _last_fn = ""
     if found[0](*args, stream) != 0:
@@ -1606,29 +1606,36 @@ def _launch(libname: str, fn: str, types, *args) -> None:
     _last_fn = fn
 
 
-def _at(t):
-    """A tensor's address (a shape-only one's: none)."""
-    return None if t is None or (t.is_meta and _dry) else t.data_ptr()
+_cuda_device = torch._C._cuda_getDevice
 
 
-def _one_place(fn: str, *tensors) -> None:
-    """Every tensor on the current device (whose stream the kernels are launched on), in rows without gaps."""
+def _addresses(fn: str, *tensors):
+    """Where the tensors lie (None: nowhere; in a pass over shapes alone nothing does): on the current device, whose stream the kernels
+    are launched on, in rows without gaps."""
     if _dry:
-        return
-    dev = tensors[0].get_device()
-    same = contiguous = True
+        return (None,) * len(tensors)
+    dev, out = tensors[0].get_device(), []
     for t in tensors:
-        if t is not None:
-            same = same and t.get_device() == dev
-            contiguous = contiguous and t.is_contiguous()
-    if not same:
-        raise InvalidArgument(f"{fn}: tensors on several devices ({', '.join(sorted({str(t.device) for t in tensors if t is not None}))})")
-    if not contiguous:
+        if t is None:
+            out.append(None)
+            continue
+        if t.get_device() != dev or not t.is_contiguous():
+            _misplaced(fn, [t for t in tensors if t is not None])
+        out.append(t.data_ptr())
+    if dev < 0 or dev != _cuda_device():
+        _misplaced(fn, [t for t in tensors if t is not None])
+    return out
+
+
+def _misplaced(fn: str, tensors) -> None:
+    devices = sorted({str(t.device) for t in tensors})
+    if len(devices) > 1:
+        raise InvalidArgument(f"{fn}: tensors on several devices ({', '.join(devices)})")
+    if not all(t.is_contiguous() for t in tensors):
         raise InvalidArgument(f"{fn}: kernels take contiguous tensors")
-    if dev < 0:
+    if not tensors[0].is_cuda:
         raise ExtensionError("the kernels run on the GPU: a tensor on the CPU was passed, and there is no CPU path")
-    if dev != torch._C._cuda_getDevice():
-        raise InvalidArgument(f"{fn}: tensors on cuda:{dev}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    raise InvalidArgument(f"{fn}: tensors on {devices[0]}, the current device is cuda:{_cuda_device()}")
 
 
 def _int32(fn: str, **tensors) -> None:
@@ -1701,14 +1708,13 @@ def qk_norm_rope_append_q4(qkv, q_gamma, k_gamma, eps: float, cos_sin, tok_seq, 
         _need(False, fn, f"{n_heads} heads over {n_kv} of {head_dim} lanes of {tok_seq.numel()} tokens in rows of {list(rows)}, "
               f"queries to {list(q_out.shape)}")
     g = q_gamma if q_gamma is not None else k_gamma
-    if n_kv:
-        _one_place("qk_norm_rope_append_q4", qkv, q_gamma, k_gamma, cos_sin, tok_seq, tok_pos, block_table, k_pages, v_pages, q_out)
-        cache = (_at(block_table), block_table.shape[1], _at(k_pages), _at(v_pages), k_pages.shape[0])
-    else:
-        _one_place("qk_norm_rope_append_q4", qkv, q_gamma, k_gamma, cos_sin, tok_seq, tok_pos, q_out)
-        cache = (None, 0, None, None, 0)
-    _launch("cache_q4", "nncpu_qk_norm_rope_append_q4", _APPEND_Q4, _at(qkv), _code(qkv), rows[1], _at(q_gamma), _at(k_gamma), _code(g),
-            eps, _at(cos_sin), half, _at(tok_seq), _at(tok_pos), *cache, _at(q_out), _code(q_out), n, n_heads, n_kv, head_dim, coef, every)
+    width, n_pages = (block_table.shape[1], k_pages.shape[0]) if n_kv else (0, 0)
+    if not n_kv:
+        block_table = k_pages = v_pages = None
+    qkv_at, qg_at, kg_at, cs_at, seq_at, pos_at, table_at, k_at, v_at, q_at = _addresses(
+        "qk_norm_rope_append_q4", qkv, q_gamma, k_gamma, cos_sin, tok_seq, tok_pos, block_table, k_pages, v_pages, q_out)
+    _launch("cache_q4", "nncpu_qk_norm_rope_append_q4", _APPEND_Q4, qkv_at, _code(qkv), rows[1], qg_at, kg_at, _code(g), eps, cs_at, half, seq_at,
+            pos_at, table_at, width, k_at, v_at, n_pages, q_at, _code(q_out), n, n_heads, n_kv, head_dim, coef, every)
 
 
 _READ_Q4 = [_P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I]
@@ -1725,9 +1731,9 @@ def q4_read(k_pages, v_pages, block_table, tok_seq, tok_pos, k_out, v_out) -> No
         _q4_pages("q4_read", k_pages, v_pages, n_kv, head_dim)
         _q4_places("q4_read", n, block_table, tok_seq, tok_pos)
         _need(False, "q4_read", f"keys to {k_out.dtype} {list(k_out.shape)}, values to {v_out.dtype} {list(v_out.shape)}")
-    _one_place("q4_read", k_pages, v_pages, block_table, tok_seq, tok_pos, k_out, v_out)
-    _launch("cache_q4", "nncpu_q4_read", _READ_Q4, _at(k_pages), _at(v_pages), pages[0], _at(block_table), block_table.shape[1], _at(tok_seq),
-            _at(tok_pos), _at(k_out), _at(v_out), _code(k_out), n, n_kv, head_dim)
+    k_at, v_at, table_at, seq_at, pos_at, k_to, v_to = _addresses("q4_read", k_pages, v_pages, block_table, tok_seq, tok_pos, k_out, v_out)
+    _launch("cache_q4", "nncpu_q4_read", _READ_Q4, k_at, v_at, pages[0], table_at, block_table.shape[1], seq_at, pos_at, k_to, v_to, _code(k_out), n,
+            n_kv, head_dim)
 
 
 def _attention_q4_check(fn: str, q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads: int, n_kv: int, head_dim: int,
@@ -1746,14 +1752,15 @@ def _attention_q4_check(fn: str, q, k_pages, v_pages, block_table, tok_seq, tok_
     return n
 
 
-def _q4_gate(head_gate, n: int, n_heads: int):
+def _q4_gate(fn: str, head_gate, n: int, n_heads: int):
     """As ``_head_gate``, as plain numbers."""
     if head_gate is None:
         return None, 0
     rows, col = head_gate
-    _need(rows.dtype == torch.float32 and rows.dim() == 2 and rows.is_contiguous() and rows.shape[0] == n and 0 <= col <= rows.shape[1] - n_heads,
-          "attention_q4", f"gate logits are float32 rows [{n}, at least {col + n_heads}]")
-    return (None if _dry else rows.data_ptr() + 4 * col), rows.shape[1]
+    _need(rows.dtype == torch.float32 and rows.dim() == 2 and rows.shape[0] == n and 0 <= col <= rows.shape[1] - n_heads, fn,
+          f"gate logits are float32 rows [{n}, at least {col + n_heads}]")
+    at, = _addresses(fn, rows)
+    return (None if at is None else at + 4 * col), rows.shape[1]
 
 
 def _q4_longest(block_table, longest: int, window: int, keep: int) -> int:
@@ -1775,7 +1782,7 @@ def attention_q4_scratch_floats(n_tok: int, n_heads: int, n_kv: int, head_dim: i
     return _attention_q4_scratch(torch._C._cuda_getDevice(), n_tok, n_heads, n_kv, head_dim, _DT[dtype], longest)
 
 
-_ATTENTION_Q4 = [_P, _I, _P, _P, _I, _P, _I, _P, _P, _P, _P, _L, _I, _I, _I, _I, _F, _I, _I, _F, _P, _F, _P, _I, _I]
+_ATTENTION_Q4 = [_P, _I, _P, _P, _I, _P, _I, _P, _P, _P, _P, _L, _I, _I, _I, _I, _F, _I, _I, _F, _P, _F, _P, _I, _I, _P]
 
 
 def attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads: int, n_kv: int, head_dim: int, scale: float,
@@ -1788,35 +1795,42 @@ def attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_head
     is not there (an id outside the pages) holds no keys."""
     n = _attention_q4_check("attention_q4", q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads, n_kv, head_dim, window,
                             keep, cap, sinks)
-    _one_place("attention_q4", q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, sinks)
     longest = _q4_longest(block_table, longest, window, keep)
     code = _code(q)
+    q_at, k_at, v_at, table_at, seq_at, pos_at, out_at, sinks_at, scratch_at = _addresses(
+        "attention_q4", q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, sinks, scratch)
     if scratch is None and not _dry:
-        need = _attention_q4_scratch(q.get_device(), n, n_heads, n_kv, head_dim, code, longest)
-        scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
-    _need(scratch is None or (scratch.dtype is torch.float32 and scratch.is_contiguous()), "attention_q4", "scratch is contiguous float32")
-    _launch("attention_q4", "nncpu_attention_q4", _ATTENTION_Q4, _at(q), code, _at(k_pages), _at(v_pages), k_pages.shape[0], _at(block_table),
-            block_table.shape[1], _at(tok_seq), _at(tok_pos), _at(out), _at(scratch), 0 if scratch is None else scratch.numel(), n, n_heads,
-            n_kv, head_dim, scale, window, keep, slope_base, _at(sinks), cap, *_q4_gate(head_gate, n, n_heads), longest)
+        need = _attention_q4_scratch(_cuda_device(), n, n_heads, n_kv, head_dim, code, longest)
+        if need:
+            scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+            scratch_at = scratch.data_ptr()
+    elif scratch is not None and scratch.dtype is not torch.float32:
+        raise InvalidArgument("attention_q4: scratch is float32")
+    gate_at, gate_ld = _q4_gate("attention_q4", head_gate, n, n_heads)
+    _launch("attention_q4", "nncpu_attention_q4", _ATTENTION_Q4, q_at, code, k_at, v_at, k_pages.shape[0], table_at, block_table.shape[1], seq_at,
+            pos_at, out_at, scratch_at, 0 if scratch is None else scratch.numel(), n, n_heads, n_kv, head_dim, scale, window, keep, slope_base,
+            sinks_at, cap, gate_at, gate_ld, longest, None)
 
 
-# Prompts take their sequences' keys and values out of the codes once, for all query tiles and heads, and attend to those: float16 for
-# the tcgen05 kernel, float32 for the 32-bit one.  So many positions at a time (of whole sequences, one at least).
+# A portion of one sequence attends straight from the codes, as many of its tokens at a time as have columns on the tensor cores, while
+# its tokens are at most so many.  Longer ones, and several sequences, have their keys and values taken out of the codes once, for
+# all query tiles and heads: float16 for the tcgen05 kernel, float32 for the 32-bit one; so many positions at a time (of whole sequences,
+# one at least).
+Q4_FEW_TOKENS = 64
 Q4_EXPAND_POSITIONS = 16384
 Q4_EXPAND_POSITIONS_F32 = 65536
 
 
 @functools.lru_cache(maxsize=4096)
 def _q4_prompt_plan(n: int, n_seqs: int, n_heads: int, n_kv: int, head_dim: int, bf16: bool, longest: int, slope_and_cap: bool):
-    """How a prompt attends: (lanes of the rows that the keys are taken out to, or 0: token by token; pages of a sequence; sequences
-    at a time; bytes of keys; of keys, values and table; of all)."""
+    """How a prompt attends: (lanes of the rows that the keys are taken out to, or 0: straight from the codes; pages of a sequence;
+    sequences at a time; bytes of keys; of keys, values and table; of all)."""
     width = (longest + 63) // 64
     lanes = 0
-    if n <= n_seqs:
+    if n <= n_seqs or (bf16 and n_seqs == 1 and n <= Q4_FEW_TOKENS and head_dim <= 128):
         pass
     elif bf16:
-        lanes = 64 if head_dim <= 64 else 128 if head_dim <= 128 and not slope_and_cap else 0
-        lanes = 0 if slope_and_cap else lanes
+        lanes = 0 if slope_and_cap else 64 if head_dim <= 64 else 128 if head_dim <= 128 else 0
     elif head_dim <= 128 and n_heads // n_kv <= 32 and n_seqs * width * 64 <= Q4_EXPAND_POSITIONS_F32:
         lanes = head_dim
     if lanes == 0:
@@ -1844,49 +1858,56 @@ def attention_q4_prompt(q, k_pages, v_pages, block_table, cu_seqlens, tok_seq, t
     """``attention_q4`` for prompts and portions of them: any number of tokens a sequence, at consecutive positions (``cu_seqlens``
     int32 [n_seqs + 1]: each sequence's first token).  ``longest``: at least as many keys as any token sees.  ``status``: an int32 word on
     the device that receives a code if a bounded wait runs out, as in ``attention_prefill_tc``.  ``scratch``: uint8,
-    ``attention_q4_prompt_scratch_bytes`` elements (None: taken from the allocator).  Here a page that is not there counts as zeros."""
+    ``attention_q4_prompt_scratch_bytes`` elements (None: taken from the allocator).  What is left in the rows of no sequence is not said;
+    a page that is not there may count as zeros."""
     fn = "attention_q4_prompt"
     n = _attention_q4_check(fn, q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads, n_kv, head_dim, window, keep, cap, sinks)
     if not (cu_seqlens.dtype is torch.int32 and cu_seqlens.dim() == 1 and 0 < n_seqs < cu_seqlens.shape[0] and longest > 0
             and block_table.shape[0] >= n_seqs and status.dtype is torch.int32 and status.numel() > 0):
         _int32(fn, cu_seqlens=cu_seqlens, status=status)
         _need(False, fn, f"{n_seqs} sequences, places {list(cu_seqlens.shape)}, tables {list(block_table.shape)}, {longest} keys")
-    _one_place(fn, q, k_pages, v_pages, block_table, cu_seqlens, tok_seq, tok_pos, out, sinks, status, scratch)
-    longest = min(longest, block_table.shape[1] * 64)
-    bf16 = _code(q) == 1
+    table_width = block_table.shape[1]
+    longest = min(longest, table_width * 64)
+    code = _code(q)
+    bf16 = code == 1
     lanes, width, at_once, kv_bytes, table_end, need = _q4_prompt_plan(n, n_seqs, n_heads, n_kv, head_dim, bf16, longest,
                                                                        slope_base != 0.0 and cap != 0.0)
-    if lanes == 0:
-        if scratch is not None:
-            scratch = scratch.view(torch.float32)
-        attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads, n_kv, head_dim, scale, window, slope_base, sinks, keep,
-                     cap, head_gate, longest, scratch)
-        return
-    if scratch is None:
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _need(scratch.dtype is torch.uint8 and scratch.dim() == 1 and scratch.numel() >= need and _aligned(scratch), fn,
-          f"scratch of {scratch.numel()} bytes ({need} are needed, from a 16-byte boundary)")
+    q_at, k_at, v_at, table_at, cu_at, seq_at, pos_at, out_at, sinks_at, status_at, base = _addresses(
+        fn, q, k_pages, v_pages, block_table, cu_seqlens, tok_seq, tok_pos, out, sinks, status, scratch)
+    if not _dry:
+        if lanes == 0:
+            need = 4 * _attention_q4_scratch(_cuda_device(), n, n_heads, n_kv, head_dim, code, longest)
+        if scratch is None and need:
+            scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+            base = scratch.data_ptr()
+        if need and not (scratch.dtype is torch.uint8 and scratch.numel() >= need and base % 16 == 0):
+            raise InvalidArgument(f"{fn}: scratch of {need} bytes, from a 16-byte boundary")
+    gate_at, gate_ld = _q4_gate(fn, head_gate, n, n_heads)
     if n == 0:
         return
-    base = _at(scratch) or 0
-    k_at, v_at, table_at = base, base + kv_bytes, base + 2 * kv_bytes
+    if lanes == 0:
+        _launch("attention_q4", "nncpu_attention_q4", _ATTENTION_Q4, q_at, code, k_at, v_at, k_pages.shape[0], table_at, table_width, seq_at, pos_at,
+                out_at, base, need // 4, n, n_heads, n_kv, head_dim, scale, window, keep, slope_base, sinks_at, cap, gate_at, gate_ld, longest,
+                cu_at if bf16 and n_seqs == 1 and head_dim <= 128 else None)
+        return
+    if _dry:
+        table_at = cu_at = base = 0
+    k_to, v_to, table_to, q_to = base, base + kv_bytes, base + 2 * kv_bytes, base + table_end
     longer = bf16 and lanes != head_dim
-    gate, gate_ld = _q4_gate(head_gate, n, n_heads)
-    width_in = block_table.shape[1]
     for b in range(0, n_seqs, at_once):
         count = min(at_once, n_seqs - b)
-        table_in, cu = (_at(block_table) or 0) + 4 * b * width_in, (_at(cu_seqlens) or 0) + 4 * b
-        _launch("cache_q4", "nncpu_q4_expand", _EXPAND_Q4, _at(k_pages), _at(v_pages), k_pages.shape[0], table_in, width_in, cu, _at(tok_pos),
-                count, width, n_kv, head_dim, lanes, window, keep, bf16, k_at, v_at, table_at, _at(q) if longer and b == 0 else None,
-                base + table_end if longer else None, n, n_heads)
+        cu = cu_at + 4 * b
+        _launch("cache_q4", "nncpu_q4_expand", _EXPAND_Q4, k_at, v_at, k_pages.shape[0], table_at + 4 * b * table_width, table_width, cu, pos_at,
+                count, width, n_kv, head_dim, lanes, window, keep, bf16, k_to, v_to, table_to, q_at if longer and b == 0 else None,
+                q_to if longer else None, n, n_heads)
         if bf16:
-            _launch("attention_tc", "nncpu_attention_prefill_tc_half", _PREFILL_HALF, base + table_end if longer else _at(q), k_at, v_at,
-                    count * width, table_at, width, cu, _at(tok_pos), _at(out), n, count, n_heads, n_kv, lanes, head_dim, scale, window, keep,
-                    slope_base, _at(sinks), cap, gate, gate_ld, longest, _at(status))
+            _launch("attention_tc", "nncpu_attention_prefill_tc_half", _PREFILL_HALF, q_to if longer else q_at, k_to, v_to, count * width,
+                    table_to, width, cu, pos_at, out_at, n, count, n_heads, n_kv, lanes, head_dim, scale, window, keep, slope_base, sinks_at,
+                    cap, gate_at, gate_ld, longest, status_at)
         else:
-            _launch("attention_f32", "nncpu_attention_f32", _PROMPT_F32, _at(q), k_at, v_at, table_at, width, _at(tok_seq), _at(tok_pos),
-                    _at(out), None, n, n_heads, n_kv, head_dim, head_dim, head_dim, scale, window, keep, slope_base, _at(sinks), cap, gate,
-                    gate_ld, 0, 0, n_seqs, torch.cuda.get_device_properties(q.device).multi_processor_count if not _dry else 148)
+            _launch("attention_f32", "nncpu_attention_f32", _PROMPT_F32, q_at, k_to, v_to, table_to, width, seq_at, pos_at, out_at, None, n,
+                    n_heads, n_kv, head_dim, head_dim, head_dim, scale, window, keep, slope_base, sinks_at, cap, gate_at, gate_ld, 0, 0, n_seqs,
+                    148 if _dry else torch.cuda.get_device_properties(q.device).multi_processor_count)
 
 
 _PROMPT_F32 = [_P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _F, _P, _F, _P, _I, _I, _I, _I, _I]
@@ -1917,6 +1938,5 @@ def token_logprobs(logits, targets, logprobs, entropy, top=None, ids=None) -> No
         _need((top is None) == (ids is None), fn, "top and ids come together")
         _need(top is None or 0 < k <= min(LOGPROBS_MAX_TOP, vocab), fn, f"the best {k} of {vocab} (1 to {LOGPROBS_MAX_TOP})")
         _need(False, fn, f"{n} rows: targets int32, logprobs and entropy float32 [{n}], top float32 and ids int32 [{n}, {k}]")
-    _one_place("token_logprobs", logits, targets, logprobs, entropy, top, ids)
-    _launch("token_logprobs", "nncpu_token_logprobs", _LOGPROBS, _at(logits), _code(logits), _at(targets), _at(logprobs), _at(entropy), _at(top),
-            _at(ids), n, vocab, k)
+    at, targets_at, logprobs_at, entropy_at, top_at, ids_at = _addresses("token_logprobs", logits, targets, logprobs, entropy, top, ids)
+    _launch("token_logprobs", "nncpu_token_logprobs", _LOGPROBS, at, _code(logits), targets_at, logprobs_at, entropy_at, top_at, ids_at, n, vocab, k)
