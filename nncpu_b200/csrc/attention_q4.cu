@@ -78,7 +78,9 @@ __device__ __forceinline__ float closing_factor(const AttnQ4& p, int t, int h, f
 //
 // The pages of all (token, key/value head) pairs lie in one row, of which every block takes an equal share, wherever that
 // begins and ends: unequal sequences cost nothing, and there is one wave of blocks.  A pair that lies within one block is finished by it; of
-// the others every block leaves its part (its first and its last pair at most) in scratch for stream_merge_kernel.
+// the others every block leaves its part (its first and its last pair at most) in scratch for stream_merge_kernel.  Where there are few
+// pairs of not too many pages (CLUSTER), a cluster of blocks shares each of them instead, and its parts meet in distributed
+// shared memory: one launch, and no way through global memory.
 // ---------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kStreamWarps = 2;
@@ -96,6 +98,7 @@ struct Stream {
     int blocks;             // blocks of the launch
     float scale2;           // scale * log2(e)
     ScoreCap cap;
+    int cluster;            // CLUSTER: blocks that share a pair
     int2* parts;            // [tiles, pairs]: the first block that has a part of a pair, and the last
 };
 
@@ -113,6 +116,17 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
     uint32_t d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t local, uint32_t rank) {
+    uint32_t remote;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+    return v;
 }
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
@@ -284,7 +298,7 @@ __device__ __forceinline__ void zero_rows(const AttnQ4& p, const Stream& st) {
     }
 }
 
-template <int NG, int NT>
+template <int NG, int NT, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_kernel(const AttnQ4 p, const Stream st) {
     constexpr int D = 32 * NG, COLS = 8 * NT;
     constexpr bool TILED = NT == 2;       // a tile may have several tokens
@@ -298,14 +312,26 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
     float* meet = reinterpret_cast<float*>(stream_smem + kStreamWarps * kStreamStages * kStage);   // [COLS][D + 4]: lanes, reference, sum
     wait_for_previous_kernels();
     let_next_kernel_start();
-    const int my_pages = lane < st.tiles ? pages_of<TILED>(p, st, lane) : 0;
-    const Row row = row_of<TILED>(p, st, lane, my_pages);
-    if ((int)blockIdx.x >= row.blocks) {
-        zero_rows<D, TILED>(p, st);
-        return;
+    const int my_pages = CLUSTER ? 0 : lane < st.tiles ? pages_of<TILED>(p, st, lane) : 0;
+    Row row{};
+    Place here;
+    if (CLUSTER) {
+        const int pair = blockIdx.x / st.cluster, rank = blockIdx.x - pair * st.cluster;
+        here.t = pair / st.pairs;
+        here.y = pair - here.t * st.pairs;
+        here.n = pages_of<TILED>(p, st, here.t);
+        here.i = here.n * rank / st.cluster;
+        here.left = here.n * (rank + 1) / st.cluster - here.i;
+    } else {
+        row = row_of<TILED>(p, st, lane, my_pages);
+        if ((int)blockIdx.x >= row.blocks) {
+            zero_rows<D, TILED>(p, st);
+            return;
+        }
+        const unsigned first_place = row.start(blockIdx.x);
+        here = place_of<TILED>(p, st, first_place, (int)(row.start(blockIdx.x + 1) - first_place), lane, my_pages);
     }
-    const unsigned first_place = row.start(blockIdx.x);
-    Place here = place_of<TILED>(p, st, first_place, (int)(row.start(blockIdx.x + 1) - first_place), lane, my_pages), ahead = here;
+    Place ahead = here;
     // The columns of a pair are its tile's tokens times its heads.  Their queries, as they lie: column r of each eight, lanes 32 g + 8 c to + 7.
     const int group = p.n_heads / p.n_kv;
     uint4 raw[NT][NG];
@@ -363,7 +389,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
                 there &= ~(1u << stage);
             }
             --ahead.left;
-            if (++ahead.i == ahead.n) ahead.template next_pair<TILED>(p, st);
+            if (++ahead.i == ahead.n && !CLUSTER) ahead.template next_pair<TILED>(p, st);
         }
         cp_async_commit();
     };
@@ -376,7 +402,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
         // -- a pair, or the part of it that lies here
         const int t = here.t, y = here.y, from = here.i, take = min(here.n - from, here.left);
         const int n_pages = here.n;
-        const bool whole = take == n_pages;
+        const bool whole = !CLUSTER && take == n_pages;
         const int kvh = y / st.chunks, h0 = kvh * group + (y - kvh * st.chunks) * st.heads, heads = min(st.heads, (kvh + 1) * group - h0);
         const Tile tile = tile_of<TILED>(p, st, t);
         const int count = TILED ? tile.count : 1, t0 = TILED ? tile.t0 : t, nh = heads * count;      // tokens, and columns
@@ -633,9 +659,11 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
         here.i += take;
         here.left -= take;
         const int left = here.left;
-        if (here.i == here.n) here.template next_pair<TILED>(p, st);
-        ask_queries();
-        if (from == 0 && threadIdx.x == 0)      // the first block with a part of the pair, and the last
+        if (!CLUSTER) {
+            if (here.i == here.n) here.template next_pair<TILED>(p, st);
+            ask_queries();
+        }
+        if (!CLUSTER && from == 0 && threadIdx.x == 0)      // the first block with a part of the pair, and the last
             st.parts[(size_t)t * st.pairs + y] =
                 make_int2(blockIdx.x, whole ? (int)blockIdx.x : row.block_of(row.start(blockIdx.x + 1) - (left + take) + n_pages - 1));
         // -- the warps' parts meet: thread (r, c) holds lanes 32 g + 4 r to + 3 of heads 2 c and 2 c + 1.  Each warp leaves the other one's
@@ -677,7 +705,9 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
                         const float4 w = *reinterpret_cast<const float4*>(other + d);
                         v = make_float4(fmaf(w.x, f1, v.x * f0), fmaf(w.y, f1, v.y * f0), fmaf(w.z, f1, v.z * f0), fmaf(w.w, f1, v.w * f0));
                         if (h >= nh) continue;
-                        if (whole) {
+                        if (CLUSTER) {
+                            *reinterpret_cast<float4*>(other + d) = v;       // (this thread alone has read it)
+                        } else if (whole) {
                             const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
                             const uint2 packed = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
                             *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + ((size_t)(t0 + tok[nt][e]) * p.n_heads + h0 + h - tok[nt][e] * heads) * D + d) = packed;
@@ -689,7 +719,11 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
                         other[D] = top;
                         other[D + 1] = total;
                     }
-                    if (r == 0 && pass == 1 && !whole && h < nh) {
+                    if (CLUSTER && r == 0 && pass == 1) {
+                        other[D + 2] = top;
+                        other[D + 3] = total;
+                    }
+                    if (!CLUSTER && r == 0 && pass == 1 && !whole && h < nh) {
                         float* part = p.part + ((size_t)slot * COLS + h) * (D + 4);
                         part[D] = top;
                         part[D + 1] = total;
@@ -698,7 +732,42 @@ __global__ void __launch_bounds__(32 * kStreamWarps, NT == 1 ? 6 : 4) stream_ker
         }
     }
     cp_async_wait<0>();
-    zero_rows<D, TILED>(p, st);
+    if constexpr (!CLUSTER) {
+        zero_rows<D, TILED>(p, st);
+    } else {
+        // -- the blocks' parts meet: every block adds up its share of the lanes over all of them, in the order of their keys
+        const int rank = blockIdx.x % st.cluster;
+        if (here.n * rank / st.cluster == here.n * (rank + 1) / st.cluster) {         // (it had no page)
+            if (threadIdx.x < COLS) {
+                meet[threadIdx.x * (D + 4) + D + 2] = -INFINITY;
+                meet[threadIdx.x * (D + 4) + D + 3] = 0.0f;
+            }
+        }
+        cluster_barrier();
+        const Tile tile = tile_of<TILED>(p, st, here.t);
+        const int kvh = here.y / st.chunks, h0 = kvh * group + (here.y - kvh * st.chunks) * st.heads, heads = min(st.heads, (kvh + 1) * group - h0);
+        const int count = TILED && st.cu != nullptr ? tile.count : 1;      // (a row of no sequence is zeros, see zero_rows)
+        const int d0 = D * rank / st.cluster, lanes = D * (rank + 1) / st.cluster - d0;
+        const uint32_t at = (uint32_t)__cvta_generic_to_shared(meet);
+        for (int x = threadIdx.x; x < heads * count * lanes; x += 32 * kStreamWarps) {
+            const int h = x / lanes, d = d0 + x - h * lanes, tok = h / heads, head = h0 + h - tok * heads;
+            const uint32_t col = at + h * (D + 4) * 4;
+            float top = -INFINITY, sum = 0.0f, out = 0.0f;
+#pragma unroll 8
+            for (int k = 0; k < st.cluster; ++k) top = fmaxf(top, ld_cluster(col + (D + 2) * 4, k));
+#pragma unroll 8
+            for (int k = 0; k < st.cluster; ++k) {
+                const float ref = ld_cluster(col + (D + 2) * 4, k), l = ld_cluster(col + (D + 3) * 4, k), v = ld_cluster(col + d * 4, k);
+                if (ref == -INFINITY) continue;
+                const float f = exp2f(ref - top);
+                sum = fmaf(l, f, sum);
+                out = fmaf(v, f, out);
+            }
+            const float f = here.n == 0 ? 0.0f : closing_factor(p, tile.t0 + tok, head, top / kLog2e, sum);
+            reinterpret_cast<__nv_bfloat16*>(p.out)[((size_t)(tile.t0 + tok) * p.n_heads + head) * D + d] = __float2bfloat16_rn(here.n == 0 ? 0.0f : out * f);
+        }
+        cluster_barrier();          // a block's memory is read until every block is done
+    }
 }
 
 // The parts of a pair that lies in several blocks, in the order of its keys.  grid = (tiles, pairs, columns of a pair), a thread a lane.
@@ -902,21 +971,23 @@ static bool streams(int dt, int D) { return dt == DT_BF16 && D <= 128; }
 
 // Blocks of a token's pages' row, all of which run at once, and how the heads of a key/value head are dealt with.
 constexpr int kStreamMinPlaces = 4;
+constexpr int kClusterKeys = 8 * kPage;      // keys of a cluster's block at most, of the longest sequence there may be
 static int stream_tiles(int n_heads, int n_kv) { return n_heads / n_kv > 8 ? 2 : 1; }
 static int stream_smem(int D, int tiles) {
     return kStreamWarps * kStreamStages * 40 * D + 8 * tiles * (D + 4) * (int)sizeof(float);
 }
 typedef void (*StreamKernel)(AttnQ4, Stream);
+template <bool CLUSTER>
 static StreamKernel stream_kernel_of(int D, int tiles) {
     switch (D / 32 * 2 + tiles - 1) {
-        case 2: return stream_kernel<1, 1>;
-        case 3: return stream_kernel<1, 2>;
-        case 4: return stream_kernel<2, 1>;
-        case 5: return stream_kernel<2, 2>;
-        case 6: return stream_kernel<3, 1>;
-        case 7: return stream_kernel<3, 2>;
-        case 8: return stream_kernel<4, 1>;
-        default: return stream_kernel<4, 2>;
+        case 2: return stream_kernel<1, 1, CLUSTER>;
+        case 3: return stream_kernel<1, 2, CLUSTER>;
+        case 4: return stream_kernel<2, 1, CLUSTER>;
+        case 5: return stream_kernel<2, 2, CLUSTER>;
+        case 6: return stream_kernel<3, 1, CLUSTER>;
+        case 7: return stream_kernel<3, 2, CLUSTER>;
+        case 8: return stream_kernel<4, 1, CLUSTER>;
+        default: return stream_kernel<4, 2, CLUSTER>;
     }
 }
 // Blocks of one kernel that the current device runs at once (asked once for each).
@@ -926,7 +997,7 @@ static int stream_blocks(int D, int tiles) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sm_count();
     int& n = known[dev][D / 32 * 2 + tiles - 1];
     if (n == 0) {
-        const StreamKernel k = stream_kernel_of(D, tiles);
+        const StreamKernel k = stream_kernel_of<false>(D, tiles);
         int per = 0;
         if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, stream_smem(D, tiles)) != cudaSuccess ||
             cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, k, 32 * kStreamWarps, stream_smem(D, tiles)) != cudaSuccess || per < 1) {
@@ -936,6 +1007,42 @@ static int stream_blocks(int D, int tiles) {
         n = per * sm_count();
     }
     return n;
+}
+
+// Blocks of a cluster that shares a pair, or 0: the row of pages.  Where a cluster's blocks have a few pages each, and all clusters run at
+// once.
+static int cluster_of(long pairs, int longest, int D, int tiles) {
+    static int fit[64][10][2] = {};      // clusters of 8 and of 16 that the device runs at once (0: not asked yet)
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    for (int i = 1; i >= 0; --i) {
+        const int n = 8 << i;
+        if (longest > n * kClusterKeys || (i == 1 && longest <= 4 * kPage)) continue;
+        int& f = fit[dev][D / 32 * 2 + tiles - 1][i];
+        if (f == 0) {
+            const StreamKernel k = stream_kernel_of<true>(D, tiles);
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = (unsigned)n;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.gridDim = dim3((unsigned)n);
+            cfg.blockDim = dim3(32 * kStreamWarps);
+            cfg.dynamicSmemBytes = stream_smem(D, tiles);
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int clusters = 0;
+            if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, stream_smem(D, tiles)) != cudaSuccess ||
+                cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+                cudaOccupancyMaxActiveClusters(&clusters, k, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                clusters = 0;
+            }
+            f = clusters > 0 ? clusters : -1;
+        }
+        if (pairs <= f && pairs * n <= 2L * sm_count()) return n;
+    }
+    return 0;
 }
 
 // Floats of scratch for a call of these sizes, `longest` the most keys that a token may see.
@@ -975,23 +1082,35 @@ extern "C" int nncpu_attention_q4(const void* q, int dt, const uint8_t* k_pages,
         const int tiles = one_seq != nullptr && n > 1 ? 2 : stream_tiles(n_heads, n_kv), chunks = (group + 8 * tiles - 1) / (8 * tiles);
         const int heads = (group + chunks - 1) / chunks, tile = one_seq != nullptr && n > 1 ? 16 / heads : 1;
         const int n_tiles = (n + tile - 1) / tile;
+        const int cluster = cluster_of((long)n_tiles * n_kv * chunks, longest, D, tiles);
         NN_CHECK((long)n_tiles * n_kv * chunks * (bt_stride + 3L) < (1L << 31), "attention_q4: %d tokens of up to %d pages", n, bt_stride);
         NN_CHECK(n_kv <= 65535 / chunks, "attention_q4: %d key/value heads in %d parts", n_kv, chunks);
         Stream st{heads, chunks, n_kv * chunks, tile, n_tiles, one_seq, kStreamMinPlaces, stream_blocks(D, tiles), scale * kLog2e,
-                  score_cap(scale, cap), nullptr};
+                  score_cap(scale, cap), cluster, nullptr};
         st.parts = reinterpret_cast<int2*>(part + 2L * st.blocks * 8 * tiles * (D + 4));
         // All blocks of the first kernel have to run at once, six to an SM, so it is not launched to start under the end of the one
         // before: beside blocks of that one an SM may find room for five, and the sixth, begun when those are done, doubles the time
         // (64 sequences of up to 8 000 keys: 84 us instead of 71).  The second one is.
         cudaLaunchConfig_t cfg = {};
-        cudaLaunchAttribute attr[1];
-        cfg.gridDim = dim3((unsigned)st.blocks);
+        cudaLaunchAttribute attr[2];
         cfg.blockDim = dim3(32 * kStreamWarps);
         cfg.dynamicSmemBytes = stream_smem(D, tiles);
         cfg.stream = stream;
         cfg.attrs = attr;
+        cudaError_t e;
+        if (cluster > 0) {
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = (unsigned)cluster;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.gridDim = dim3((unsigned)(n_tiles * st.pairs * cluster));
+            cfg.numAttrs = 1 + overlap_attribute(attr + 1);
+            e = cudaLaunchKernelEx(&cfg, stream_kernel_of<true>(D, tiles), p, st);
+            NN_CHECK(e == cudaSuccess, "attention_q4: launch failed: %s", cudaGetErrorString(e));
+            return 0;
+        }
+        cfg.gridDim = dim3((unsigned)st.blocks);
         cfg.numAttrs = 0;
-        cudaError_t e = cudaLaunchKernelEx(&cfg, stream_kernel_of(D, tiles), p, st);
+        e = cudaLaunchKernelEx(&cfg, stream_kernel_of<false>(D, tiles), p, st);
         NN_CHECK(e == cudaSuccess, "attention_q4: launch failed: %s", cudaGetErrorString(e));
         cfg.gridDim = dim3((unsigned)n_tiles, (unsigned)st.pairs, (unsigned)(st.heads * tile));
         cfg.blockDim = dim3(D);

@@ -355,11 +355,11 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const Expand p) 
     const bool values = blockIdx.y >= p.n_kv;
     const int h = values ? blockIdx.y - p.n_kv : blockIdx.y;
     if (blockIdx.y == 0 && threadIdx.x == 0) p.table[row] = row;
+    int id = pi < p.bt_stride ? p.block_table[(size_t)b * p.bt_stride + pi] : -1;      // (asked for beside the next two)
     const int t0 = p.cu_seqlens[b], t1 = p.cu_seqlens[b + 1];
     if (t1 <= t0) return;
     const int first = first_visible_key(p.tok_pos[t0], p.window), last = p.tok_pos[t1 - 1];
     if (pi * kPage > last || (pi * kPage + kPage - 1 < first && pi * kPage >= p.keep)) return;      // no token sees the page
-    int id = pi < p.bt_stride ? p.block_table[(size_t)b * p.bt_stride + pi] : -1;
     if (id >= p.n_pages) id = -1;
     const int D = p.D, NG = D / kGroup, rows = id < 0 ? 0 : min(kPage, last + 1 - pi * kPage), per_row = p.lanes / 8;
     const uint8_t* base = (values ? p.v_pages : p.k_pages) + ((size_t)max(id, 0) * p.n_kv + h) * q4_page_bytes(D);
