@@ -971,7 +971,7 @@ static bool streams(int dt, int D) { return dt == DT_BF16 && D <= 128; }
 
 // Blocks of a token's pages' row, all of which run at once, and how the heads of a key/value head are dealt with.
 constexpr int kStreamMinPlaces = 4;
-constexpr int kClusterKeys = 8 * kPage;      // keys of a cluster's block at most, of the longest sequence there may be
+constexpr int kClusterKeys = 8 * kPage;      // see cluster_of
 static int stream_tiles(int n_heads, int n_kv) { return n_heads / n_kv > 8 ? 2 : 1; }
 static int stream_smem(int D, int tiles) {
     return kStreamWarps * kStreamStages * 40 * D + 8 * tiles * (D + 4) * (int)sizeof(float);
@@ -1009,15 +1009,16 @@ static int stream_blocks(int D, int tiles) {
     return n;
 }
 
-// Blocks of a cluster that shares a pair, or 0: the row of pages.  Where a cluster's blocks have a few pages each, and all clusters run at
-// once.
+// Blocks of a cluster that shares a pair, or 0: the row of pages.  Clusters, where they all run at once and either keep the device's blocks
+// half busy or have at most eight pages a block (32 heads over 8, us, the row / clusters of 8 / of 16): one sequence of 300 keys 11.5 / 6.9 /
+// 7.8, of 2 500 13.9 / 10.6 / 9.8, of 4 500 16.5 / 14.2 / 11.7; four of 2 500 15.7 / 11.3 / 13.3; twelve of 4 500 27.6 / 20.9 / -.
 static int cluster_of(long pairs, int longest, int D, int tiles) {
     static int fit[64][10][2] = {};      // clusters of 8 and of 16 that the device runs at once (0: not asked yet)
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
     for (int i = 1; i >= 0; --i) {
         const int n = 8 << i;
-        if (longest > n * kClusterKeys || (i == 1 && longest <= 4 * kPage)) continue;
+        if (i == 1 && (longest <= 2048 || pairs * n > 2L * sm_count())) continue;
         int& f = fit[dev][D / 32 * 2 + tiles - 1][i];
         if (f == 0) {
             const StreamKernel k = stream_kernel_of<true>(D, tiles);
@@ -1040,7 +1041,7 @@ static int cluster_of(long pairs, int longest, int D, int tiles) {
             }
             f = clusters > 0 ? clusters : -1;
         }
-        if (pairs <= f && pairs * n <= 2L * sm_count()) return n;
+        if (pairs <= f && (longest <= n * kClusterKeys || 2 * pairs >= f)) return n;
     }
     return 0;
 }

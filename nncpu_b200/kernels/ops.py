@@ -1813,10 +1813,11 @@ def attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_head
 
 
 # A portion of one sequence attends straight from the codes, as many of its tokens at a time as have columns on the tensor cores, while
-# its tokens are at most so many.  Longer ones, and several sequences, have their keys and values taken out of the codes once, for
+# its tokens are at most so many (32 heads over 8, us, straight / taken out first: 8 behind 3 000 19 / 33, 24 behind 700 17 / 21, 24 behind
+# 3 000 23 / 34, 48 behind 1 500 27.6 / 28.2, 64 behind 3 000 36.7 / 35.3).  Longer ones, and several sequences, have their keys and values taken out of the codes once, for
 # all query tiles and heads: float16 for the tcgen05 kernel, float32 for the 32-bit one; so many positions at a time (of whole sequences,
 # one at least).
-Q4_FEW_TOKENS = 64
+Q4_FEW_TOKENS = 48
 Q4_EXPAND_POSITIONS = 16384
 Q4_EXPAND_POSITIONS_F32 = 65536
 

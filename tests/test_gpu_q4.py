@@ -230,6 +230,21 @@ def test_attention_of_long_and_unequal_sequences(lens, dt):
     run_attention(lens, 8, 2, 64, dt, seed=4)
 
 
+@pytest.mark.parametrize("heads,kv,D", [(8, 8, 64), (32, 8, 128), (24, 2, 128)])
+def test_attention_of_many_sequences(heads, kv, D):
+    # more tokens than a warp looks at once, short ones beside long ones, rows of no sequence among them
+    lens = [1 + (37 * i * i) % 300 for i in range(70)] + [2500]
+    seq = list(range(71))
+    seq[5] = seq[40] = seq[69] = -1
+    run_attention(lens, heads, kv, D, BF16, seq=seq, pos=[n - 1 for n in lens], seed=11)
+
+
+@pytest.mark.parametrize("window,keep", [(0, 0), (9000, 70)])
+def test_attention_of_one_very_long_sequence(window, keep):
+    run_attention([20000], 4, 1, 64, BF16, seed=12, window=window, keep=keep)
+    run_attention([9003], 6, 2, 128, BF16, seed=13, window=window and 4000, keep=keep)
+
+
 OPTIONS = [dict(window=1), dict(window=64), dict(window=100, keep=3), dict(window=70, keep=130), dict(window=-48), dict(window=-64),
            dict(slope_base=8.0), dict(sinks=True), dict(cap=5.0), dict(gate=True), dict(cap=30.0, sinks=True, gate=True, window=90, keep=1),
            dict(slope_base=4.0, sinks=True, gate=True)]
@@ -265,7 +280,7 @@ def test_what_lies_behind_the_end_and_outside_the_pages_is_not_seen(dt):
 
 
 PROMPTS = [(([1],), ([0],)), (([2],), ([0],)), (([64],), ([64],)), (([200],), ([0],)), (([130, 1, 70],), ([0, 300, 59],)), (([24],), ([701],)),
-           (([300],), ([33],)), (([33, 40, 35],), ([0, 5, 190],))]
+           (([300],), ([33],)), (([33, 40, 35],), ([0, 5, 190],)), (([47],), ([0],)), (([5],), ([3000],))]
 
 
 @pytest.mark.parametrize("dt", [F32, BF16])
