@@ -3,8 +3,7 @@
 //
 //   stream_kernel: bfloat16 queries, heads of up to 128 lanes, on the tensor cores, straight from the codes (see there).
 //   any_kernel: any type of queries, any whole number of 32-lane groups; 32-bit arithmetic on numbers taken out of the pages.
-//     A block takes one token, up to eight query heads of one key/value head and a split of their pages, turns a page of keys and
-//     then one of values into 32-bit numbers in shared memory and works on those.
+//     A block takes one token, up to eight query heads of one key/value head and a split of their pages.
 // Parts of a token's keys meet in a second kernel, in the order of the keys.
 
 #include <math.h>
@@ -39,7 +38,6 @@ struct AttnQ4 {
     int n_splits;
 };
 
-constexpr int kAnyHeads = 8;      // query heads of a block
 constexpr int kAnyThreads = 128;
 
 __device__ __forceinline__ float slope_of(const AttnQ4& p, int h) {
@@ -808,30 +806,39 @@ __device__ __forceinline__ int2 split_pages(int n_walk, int n_splits, int s) {
     return make_int2(min(n_walk, s * per), min(n_walk, (s + 1) * per));
 }
 
+// A page at a time: keys as numbers to shared memory; scores, a thread a key and half of the heads; weights against the running
+// maximum, a warp a head; values to shared memory; outputs, a thread a lane (two of heads of more than 128) and, of heads of 32 and 64 lanes,
+// a part of the keys.  Bound by the latency of that chain (four sequences of up to 1 000 keys, 16 heads over 4 of 64 lanes: 14 us of which
+// the bytes are worth 0.2), so a split is a page where there are blocks to spare.
+template <int HEADS>
 __global__ void __launch_bounds__(kAnyThreads) any_kernel(const AttnQ4 p) {
-    extern __shared__ float any_smem[];
-    const int D = p.D, NG = D / kGroup, ld = D + 1, tid = threadIdx.x;
-    float* tile = any_smem;                    // [64][D + 1]
-    float* qs = tile + kPage * ld;             // [kAnyHeads][D]
-    float* ps = qs + kAnyHeads * D;            // [kAnyHeads][64] scores, then weights
-    float* stat = ps + kAnyHeads * kPage;      // [kAnyHeads][3]: maximum, sum, correction
+    extern __shared__ __align__(16) float any_smem[];
+    constexpr int kHalf = HEADS >= 2 ? HEADS / 2 : 1;      // heads of a thread's scores
+    const int D = p.D, NG = D / kGroup, ld = D + 4, tid = threadIdx.x;      // (rows 16 bytes further on than a multiple of all banks)
+    float* tile = any_smem;                    // [64][D + 4]
+    float* qs = tile + kPage * ld;             // [HEADS][D]
+    float* ps = qs + HEADS * D;                // [64][HEADS] scores, then weights
+    float* stat = ps + kPage * HEADS;          // [HEADS][3]: maximum, sum, correction
     const int t = blockIdx.x / p.n_splits, split = blockIdx.x % p.n_splits;
-    const int group = p.n_heads / p.n_kv, chunks = (group + kAnyHeads - 1) / kAnyHeads;
-    const int kvh = blockIdx.y / chunks, h0 = kvh * group + blockIdx.y % chunks * kAnyHeads;
-    const int nh = min(kAnyHeads, (kvh + 1) * group - h0);
+    const int group = p.n_heads / p.n_kv, chunks = (group + HEADS - 1) / HEADS;
+    const int kvh = blockIdx.y / chunks, h0 = kvh * group + blockIdx.y % chunks * HEADS;
+    const int nh = min(HEADS, (kvh + 1) * group - h0);
     const int seq = p.tok_seq[t], pos = p.tok_pos[t];
     const bool idle = seq < 0 || pos < 0;
     const int first = idle ? 0 : first_visible_key(pos, p.window);
     const PageWalk walk(first, idle ? 0 : pos, p.keep);
     const int2 mine = idle ? make_int2(0, 0) : split_pages(walk.n, p.n_splits, split);
-    for (int i = tid; i < nh * D; i += kAnyThreads) qs[i] = idle ? 0.0f : ld_f(p.q, ((size_t)t * p.n_heads + h0) * D + i, p.dt) * p.scale;
-    if (tid < kAnyHeads) {
+    for (int i = tid; i < HEADS * D; i += kAnyThreads)
+        qs[i] = idle || i >= nh * D ? 0.0f : ld_f(p.q, ((size_t)t * p.n_heads + h0) * D + i, p.dt) * p.scale;
+    if (tid < HEADS) {
         stat[tid * 3] = -INFINITY;
         stat[tid * 3 + 1] = 0.0f;
     }
-    float acc[kAnyHeads][2];
+    // the outputs' lanes and keys of this thread: lane d0 (and d0 + 128) of the keys from k0, every k_step-th
+    const int parts = D <= 32 ? 4 : D <= 64 ? 2 : 1, wide = kAnyThreads / parts, d0 = tid % wide, k0 = tid / wide;
+    float acc[HEADS][2];
 #pragma unroll
-    for (int h = 0; h < kAnyHeads; ++h) acc[h][0] = acc[h][1] = 0.0f;
+    for (int h = 0; h < HEADS; ++h) acc[h][0] = acc[h][1] = 0.0f;
     for (int i = mine.x; i < mine.y; ++i) {
         const int pi = walk.page(i), page = pi < p.bt_stride ? p.block_table[(size_t)seq * p.bt_stride + pi] : -1;
         if (page < 0 || page >= p.n_pages) continue;      // no such page: nothing is seen of it
@@ -841,35 +848,49 @@ __global__ void __launch_bounds__(kAnyThreads) any_kernel(const AttnQ4 p) {
         const uint8_t* vb = p.v_pages + at;
         auto seen = [&](int key) { return key <= pos && (key >= first || key < p.keep); };
         __syncthreads();
+#pragma unroll 4
         for (int w = tid; w < kPage * 4 * NG; w += kAnyThreads) {        // a word: eight lanes of one key
             const int row = w / (4 * NG), c = w % (4 * NG) / NG, g = w % NG;
             const uint32_t u = reinterpret_cast<const uint32_t*>(kb)[w];
             const float2 dm = __half22float2(reinterpret_cast<const __half2*>(kb + q4_scales_at(D))[row * NG + g]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) tile[row * ld + 32 * g + 8 * c + j] = q4_number(u >> (4 * j) & 15, dm);
+            float4* to = reinterpret_cast<float4*>(tile + row * ld + 32 * g + 8 * c);
+            to[0] = make_float4(q4_number(u & 15, dm), q4_number(u >> 4 & 15, dm), q4_number(u >> 8 & 15, dm), q4_number(u >> 12 & 15, dm));
+            to[1] = make_float4(q4_number(u >> 16 & 15, dm), q4_number(u >> 20 & 15, dm), q4_number(u >> 24 & 15, dm), q4_number(u >> 28, dm));
         }
         __syncthreads();
-        for (int k = tid; k < nh * kPage; k += kAnyThreads) {
-            const int h = k / kPage, row = k % kPage;
-            float z = -INFINITY;
-            if (seen(key0 + row)) {
-                z = 0.0f;
-                for (int d = 0; d < D; ++d) z = fmaf(qs[h * D + d], tile[row * ld + d], z);
-                if (p.cap != 0.0f) z = p.cap * tanhf(z / p.cap);
-                z -= slope_of(p, h0 + h) * (float)(pos - key0 - row);
+        {
+            const int row = tid % kPage, hb = tid / kPage * kHalf;
+            float z[kHalf];
+#pragma unroll
+            for (int h = 0; h < kHalf; ++h) z[h] = 0.0f;
+            if (hb < HEADS) {
+                for (int d = 0; d < D; d += 4) {
+                    const float4 k = *reinterpret_cast<const float4*>(tile + row * ld + d);
+#pragma unroll
+                    for (int h = 0; h < kHalf; ++h) {
+                        const float4 q = *reinterpret_cast<const float4*>(qs + (hb + h) * D + d);
+                        z[h] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, z[h]))));
+                    }
+                }
+                const bool see = seen(key0 + row);
+#pragma unroll
+                for (int h = 0; h < kHalf; ++h) {
+                    if (p.cap != 0.0f) z[h] = p.cap * tanhf(z[h] / p.cap);
+                    z[h] -= slope_of(p, h0 + hb + h) * (float)(pos - key0 - row);
+                    ps[row * HEADS + hb + h] = see ? z[h] : -INFINITY;
+                }
             }
-            ps[k] = z;
         }
         __syncthreads();
         // weights against the running maximum: a warp a head
         for (int h = tid >> 5; h < nh; h += kAnyThreads / 32) {
             const int lane = tid & 31;
-            const float a = ps[h * kPage + lane], b = ps[h * kPage + 32 + lane];
+            const float a = ps[lane * HEADS + h], b = ps[(32 + lane) * HEADS + h];
             const float m0 = stat[h * 3], m1 = fmaxf(m0, warp_max(fmaxf(a, b)));
             const float ea = m1 == -INFINITY ? 0.0f : expf(a - m1), eb = m1 == -INFINITY ? 0.0f : expf(b - m1);
             const float sum = warp_sum(ea + eb);
-            ps[h * kPage + lane] = ea;
-            ps[h * kPage + 32 + lane] = eb;
+            ps[lane * HEADS + h] = ea;
+            ps[(32 + lane) * HEADS + h] = eb;
             __syncwarp();
             if (lane == 0) {
                 const float corr = m1 == -INFINITY ? 1.0f : expf(m0 - m1);
@@ -879,52 +900,66 @@ __global__ void __launch_bounds__(kAnyThreads) any_kernel(const AttnQ4 p) {
             }
         }
         // values: what no query may see counts as zero whatever lies there
+#pragma unroll 4
         for (int w = tid; w < kPage * 4 * NG; w += kAnyThreads) {        // a word: four lanes of two positions
             const int g = w % NG, pr = w / NG % 4, r = w / (4 * NG) % 8, row = w / (32 * NG) * 8 + 2 * pr;
             const uint32_t u = reinterpret_cast<const uint32_t*>(vb)[w];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const float2 dm = __half22float2(reinterpret_cast<const __half2*>(vb + q4_scales_at(D))[(row + k) * NG + g]);
-                const bool use = seen(key0 + row + k);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) tile[(row + k) * ld + 32 * g + 4 * r + j] = use ? q4_number(u >> (16 * k + 4 * j) & 15, dm) : 0.0f;
+                const uint32_t c = u >> (16 * k);
+                float4 v = make_float4(q4_number(c & 15, dm), q4_number(c >> 4 & 15, dm), q4_number(c >> 8 & 15, dm), q4_number(c >> 12 & 15, dm));
+                if (!seen(key0 + row + k)) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                *reinterpret_cast<float4*>(tile + (row + k) * ld + 32 * g + 4 * r) = v;
             }
         }
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int d = tid + e * kAnyThreads;
+            const int d = d0 + e * kAnyThreads;
             if (d >= D) continue;
 #pragma unroll
-            for (int h = 0; h < kAnyHeads; ++h)
-                if (h < nh) acc[h][e] *= stat[h * 3 + 2];
-            for (int row = 0; row < kPage; ++row) {
+            for (int h = 0; h < HEADS; ++h) acc[h][e] *= h < nh ? stat[h * 3 + 2] : 0.0f;
+#pragma unroll 8
+            for (int row = k0; row < kPage; row += parts) {
                 const float v = tile[row * ld + d];
 #pragma unroll
-                for (int h = 0; h < kAnyHeads; ++h)
-                    if (h < nh) acc[h][e] = fmaf(ps[h * kPage + row], v, acc[h][e]);
+                for (int h = 0; h < HEADS; ++h) acc[h][e] = fmaf(h < nh ? ps[row * HEADS + h] : 0.0f, v, acc[h][e]);
             }
         }
     }
     __syncthreads();
+    if (parts > 1) {            // the keys' parts of heads of few lanes meet, in order
+        float* sums = tile;     // [HEADS][128]
 #pragma unroll
-    for (int h = 0; h < kAnyHeads; ++h) {
+        for (int h = 0; h < HEADS; ++h) sums[h * kAnyThreads + tid] = acc[h][0];
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < HEADS; ++h) {
+            float s = sums[h * kAnyThreads + d0];
+            for (int k = 1; k < parts; ++k) s += sums[h * kAnyThreads + k * wide + d0];
+            acc[h][0] = s;
+        }
+    }
+    if (k0 != 0) return;
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
         if (h >= nh) break;
         const float m = stat[h * 3], l = stat[h * 3 + 1];
         const size_t row = (size_t)t * p.n_heads + h0 + h;
         if (p.n_splits == 1) {
             const float f = idle ? 0.0f : closing_factor(p, t, h0 + h, m, l);
             for (int e = 0; e < 2; ++e) {
-                const int d = tid + e * kAnyThreads;
+                const int d = d0 + e * kAnyThreads;
                 if (d < D) st_f(p.out, row * D + d, p.dt, acc[h][e] * f);
             }
         } else {
             float* o = p.part + (row * p.n_splits + split) * D;
             for (int e = 0; e < 2; ++e) {
-                const int d = tid + e * kAnyThreads;
+                const int d = d0 + e * kAnyThreads;
                 if (d < D) o[d] = acc[h][e];
             }
-            if (tid == 0) {
+            if (d0 == 0) {
                 float* ml = p.part + (size_t)p.n * p.n_heads * p.n_splits * D + (row * p.n_splits + split) * 2;
                 ml[0] = m;
                 ml[1] = l;
@@ -933,31 +968,41 @@ __global__ void __launch_bounds__(kAnyThreads) any_kernel(const AttnQ4 p) {
     }
 }
 
-// grid = (n_heads, n): a block a row of a head.
+// grid = (n, n_heads): a block a row of a head, a warp of which makes the splits' factors.
 __global__ void __launch_bounds__(kAnyThreads) merge_any_kernel(const AttnQ4 p) {
-    const int h = blockIdx.y, t = blockIdx.x;
+    __shared__ float factor[64];
+    __shared__ float whole;
+    const int h = blockIdx.y, t = blockIdx.x, lane = threadIdx.x;
     const size_t row = (size_t)t * p.n_heads + h;
-    const float* ml = p.part + (size_t)p.n * p.n_heads * p.n_splits * p.D + row * p.n_splits * 2;
-    float m = -INFINITY, l = 0.0f;
-    for (int s = 0; s < p.n_splits; ++s) m = fmaxf(m, ml[2 * s]);
-    for (int s = 0; s < p.n_splits; ++s) l = fmaf(ml[2 * s + 1], ml[2 * s] == -INFINITY ? 0.0f : expf(ml[2 * s] - m), l);
-    const bool idle = p.tok_seq[t] < 0 || p.tok_pos[t] < 0;
-    const float f = idle ? 0.0f : closing_factor(p, t, h, m, l);
+    const float2* ml = reinterpret_cast<const float2*>(p.part + (size_t)p.n * p.n_heads * p.n_splits * p.D) + row * p.n_splits;
+    if (lane < 32) {
+        float2 a = make_float2(-INFINITY, 0.0f), b = a;
+        if (lane < p.n_splits) a = ml[lane];
+        if (lane + 32 < p.n_splits) b = ml[lane + 32];
+        const float m = warp_max(fmaxf(a.x, b.x));
+        const float fa = a.x == -INFINITY ? 0.0f : expf(a.x - m), fb = b.x == -INFINITY ? 0.0f : expf(b.x - m);
+        factor[lane] = fa;
+        factor[lane + 32] = fb;
+        const float l = warp_sum(fmaf(a.y, fa, b.y * fb));
+        if (lane == 0) whole = p.tok_seq[t] < 0 || p.tok_pos[t] < 0 ? 0.0f : closing_factor(p, t, h, m, l);
+    }
+    __syncthreads();
     for (int d = threadIdx.x; d < p.D; d += kAnyThreads) {
         float o = 0.0f;
-        for (int s = 0; s < p.n_splits; ++s)
-            o = fmaf(p.part[(row * p.n_splits + s) * p.D + d], ml[2 * s] == -INFINITY ? 0.0f : expf(ml[2 * s] - m), o);
-        st_f(p.out, row * p.D + d, p.dt, o * f);
+#pragma unroll 8
+        for (int s = 0; s < p.n_splits; ++s) o = fmaf(p.part[(row * p.n_splits + s) * p.D + d], factor[s], o);
+        st_f(p.out, row * p.D + d, p.dt, o * whole);
     }
 }
 
 }  // namespace
 
-// Splits of a token's pages: enough blocks for the device, each with at least two pages of the longest token.
+// Heads of a block, and splits of a token's pages: enough blocks for the device, each with a page of the longest token at least.
+static int any_heads(int group) { return group >= 8 ? 8 : group > 2 ? 4 : group; }
 static int any_splits(int n, int n_heads, int n_kv, int longest) {
     const int group = n_heads / n_kv;
-    const long blocks = (long)n * n_kv * ((group + kAnyHeads - 1) / kAnyHeads);
-    const long want = (4L * sm_count() + blocks - 1) / blocks, room = (longest / kPage + 1 + 1) / 2;
+    const long blocks = (long)n * n_kv * ((group + any_heads(group) - 1) / any_heads(group));
+    const long want = (4L * sm_count() + blocks - 1) / blocks, room = longest / kPage + 1;
     const long s = want < room ? want : room;
     return s < 1 ? 1 : (s > 64 ? 64 : (int)s);
 }
@@ -1121,15 +1166,17 @@ extern "C" int nncpu_attention_q4(const void* q, int dt, const uint8_t* k_pages,
         NN_CHECK(e == cudaSuccess, "attention_q4 (merge): launch failed: %s", cudaGetErrorString(e));
         return 0;
     }
-    const int chunks = (group + kAnyHeads - 1) / kAnyHeads;
-    const size_t smem = sizeof(float) * ((size_t)kPage * (D + 1) + (size_t)kAnyHeads * (D + kPage + 3));
+    const int heads = any_heads(group), chunks = (group + heads - 1) / heads;
+    const size_t smem = sizeof(float) * ((size_t)kPage * (D + 4) + (size_t)heads * (D + kPage + 3));
+    NN_CHECK((uintptr_t)part % 16 == 0, "attention_q4: scratch starts on a 16-byte boundary");
+    const auto any = heads == 8 ? any_kernel<8> : heads == 4 ? any_kernel<4> : heads == 2 ? any_kernel<2> : any_kernel<1>;
     NN_CHECK((long)n * p.n_splits < (1L << 31) && n_kv <= 65535 / chunks && n_heads <= 65535, "attention_q4: %d tokens in %d splits", n, p.n_splits);
-    static bool done[64];
-    if (first_use_on_this_device(done)) {
-        const cudaError_t e = cudaFuncSetAttribute(any_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+    static bool done[4][64];
+    if (first_use_on_this_device(done[heads == 8 ? 3 : heads / 2])) {
+        const cudaError_t e = cudaFuncSetAttribute(any, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
         NN_CHECK(e == cudaSuccess, "attention_q4: shared memory: %s", cudaGetErrorString(e));
     }
-    any_kernel<<<dim3((unsigned)(n * p.n_splits), (unsigned)(n_kv * chunks)), kAnyThreads, smem, stream>>>(p);
+    any<<<dim3((unsigned)(n * p.n_splits), (unsigned)(n_kv * chunks)), kAnyThreads, smem, stream>>>(p);
     NN_LAUNCH_OK("attention_q4");
     if (p.n_splits > 1) {
         merge_any_kernel<<<dim3((unsigned)n, (unsigned)n_heads), kAnyThreads, 0, stream>>>(p);
