@@ -15,7 +15,7 @@ def quantise(x):
     with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
         g = np.clip(g, np.float32(-65504), np.float32(65504))       # (a NaN stays one)
         lo, hi = g.min(-1), g.max(-1)                               # (of a group with a NaN: NaN)
-        d = ((hi - lo) / np.float32(15)).astype(np.float16)
+        d = ((hi - lo) * np.float32(1 / 15)).astype(np.float16)
         m = lo.astype(np.float16)
         d32, m32 = d.astype(np.float32), m.astype(np.float32)
         inv = np.where(d32 > 0, np.float32(1) / np.where(d32 > 0, d32, np.float32(1)), np.float32(0))
