@@ -784,19 +784,30 @@ __global__ void __launch_bounds__(128) stream_merge_kernel(const AttnQ4 p, const
     const float* first = p.part + ((size_t)(2 * b.x + 1) * cols + h) * (D + 4);
     const float* rest = p.part + ((size_t)(2 * b.x + 2) * cols + h) * (D + 4);
     const int n = b.y - b.x;
-    float top = first[D];
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) top = fmaxf(top, rest[i * step + D]);
-    float f = first[D] == -INFINITY ? 0.0f : exp2f(first[D] - top);
-    float sum = first[D + 1] * f, out = first[d] * f;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-        const float* from = rest + i * step;
-        f = from[D] == -INFINITY ? 0.0f : exp2f(from[D] - top);
-        sum = fmaf(from[D + 1], f, sum);
-        out = fmaf(from[d], f, out);
+    // eight parts at a time, all asked for before any is needed
+    float top = first[D], sum = first[D + 1], out = first[d];
+    for (int i0 = 0; i0 < n; i0 += 8) {
+        float ref[8], l[8], v[8], was = top;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float* from = rest + min(i0 + i, n - 1) * step;
+            ref[i] = i0 + i < n ? from[D] : -INFINITY;
+            l[i] = from[D + 1];
+            v[i] = from[d];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, ref[i]);
+        float f = was == -INFINITY ? 0.0f : exp2f(was - top);
+        sum *= f;
+        out *= f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            f = ref[i] == -INFINITY ? 0.0f : exp2f(ref[i] - top);
+            sum = fmaf(l[i], f, sum);
+            out = fmaf(v[i], f, out);
+        }
     }
-    f = closing_factor(p, tile.t0 + tok, head, top / kLog2e, sum);
+    const float f = closing_factor(p, tile.t0 + tok, head, top / kLog2e, sum);
     reinterpret_cast<__nv_bfloat16*>(p.out)[((size_t)(tile.t0 + tok) * p.n_heads + head) * D + d] = __float2bfloat16_rn(out * f);
 }
 

@@ -83,6 +83,17 @@ def test_ties_go_to_the_lowest_id(vocab):
     check(x, torch.tensor([0, vocab - 1, vocab // 2, 2], dtype=torch.int32, device=DEV), k)
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_rows_in_order_and_masked_rows(dt):
+    # ascending logits pass every bar, descending ones none; a mask that leaves fewer tokens than are asked for
+    vocab = 40001
+    up = torch.linspace(-3, 3, vocab, device=DEV)
+    x = torch.stack([up, up.flip(0), torch.full_like(up, -torch.inf), torch.full_like(up, 2.5), torch.full_like(up, -1e30)]).to(dt)
+    x[2, torch.tensor([39999, 7, 20000], device=DEV)] = 1.0
+    x[4, 17::5000] = torch.arange(8, device=DEV).to(dt)
+    check(x, torch.tensor([vocab - 1, 0, 7, 3, 17], dtype=torch.int32, device=DEV), 20)
+
+
 @pytest.mark.parametrize("vocab", [9, 3001, 151936])
 def test_rows_of_nothing_of_infinities_and_nan(vocab):
     x = torch.randn(7, vocab, generator=torch.Generator().manual_seed(1)).to(DEV)
