@@ -21,8 +21,8 @@ struct AttnQ4 {
     const uint8_t* k_pages;    // [n_pages, n_kv, 40 D]
     const uint8_t* v_pages;
     int n_pages;
-    const int* block_table;
-    int bt_stride;
+    const int* block_table;    // [bt_rows, bt_stride]
+    int bt_rows, bt_stride;
     const int* tok_seq;
     const int* tok_pos;
     void* out;                 // [n, n_heads D]
@@ -189,13 +189,13 @@ template <bool TILED>
 __device__ __forceinline__ Tile tile_of(const AttnQ4& p, const Stream& st, int i) {
     Tile w{i, 1, 0, 0, 0};
     if (TILED && st.cu != nullptr) {
-        w.t0 = st.cu[0] + i * st.tile;
-        w.count = max(0, min(st.tile, st.cu[1] - w.t0));
+        w.t0 = max(0, st.cu[0]) + i * st.tile;
+        w.count = max(0, min(st.tile, min(st.cu[1], p.n) - w.t0));
     }
     if (w.count > 0) {
         w.pos = p.tok_pos[w.t0];
         const int seq = p.tok_seq[w.t0];        // (both asked for at once)
-        if (min(w.pos, seq) < 0) w.count = 0;
+        if (min(w.pos, seq) < 0 || seq >= p.bt_rows) w.count = 0;
     }
     w.last = w.pos + w.count - 1;
     w.first = first_visible_key(w.pos, p.window);
@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(kAnyThreads) any_kernel(const AttnQ4 p) {
     const int kvh = blockIdx.y / chunks, h0 = kvh * group + blockIdx.y % chunks * HEADS;
     const int nh = min(HEADS, (kvh + 1) * group - h0);
     const int seq = p.tok_seq[t], pos = p.tok_pos[t];
-    const bool idle = seq < 0 || pos < 0;
+    const bool idle = seq < 0 || pos < 0 || seq >= p.bt_rows;
     const int first = idle ? 0 : first_visible_key(pos, p.window);
     const PageWalk walk(first, idle ? 0 : pos, p.keep);
     const int2 mine = idle ? make_int2(0, 0) : split_pages(walk.n, p.n_splits, split);
@@ -995,7 +995,7 @@ __global__ void __launch_bounds__(kAnyThreads) merge_any_kernel(const AttnQ4 p) 
         factor[lane] = fa;
         factor[lane + 32] = fb;
         const float l = warp_sum(fmaf(a.y, fa, b.y * fb));
-        if (lane == 0) whole = p.tok_seq[t] < 0 || p.tok_pos[t] < 0 ? 0.0f : closing_factor(p, t, h, m, l);
+        if (lane == 0) whole = p.tok_seq[t] < 0 || p.tok_pos[t] < 0 || p.tok_seq[t] >= p.bt_rows ? 0.0f : closing_factor(p, t, h, m, l);
     }
     __syncthreads();
     for (int d = threadIdx.x; d < p.D; d += kAnyThreads) {
@@ -1118,18 +1118,19 @@ extern "C" long nncpu_attention_q4_scratch(int n, int n_heads, int n_kv, int D, 
 // one_seq (bfloat16, at most 128 lanes): the tokens are those of ONE sequence, at consecutive positions, from one_seq[0] to before
 // one_seq[1] of the n; several of them then go through the pages together.
 extern "C" int nncpu_attention_q4(const void* q, int dt, const uint8_t* k_pages, const uint8_t* v_pages, int n_pages,
-                                  const int* block_table, int bt_stride, const int* tok_seq, const int* tok_pos, void* out, float* part,
+                                  const int* block_table, int bt_rows, int bt_stride, const int* tok_seq, const int* tok_pos, void* out, float* part,
                                   long part_floats, int n, int n_heads, int n_kv, int D, float scale, int window, int keep,
                                   float slope_base, const float* sinks, float cap, const float* head_gate, int gate_ld, int longest,
                                   const int* one_seq, cudaStream_t stream) {
     NN_CHECK(sizes_ok(n, n_heads, n_kv, D), "attention_q4: %d tokens, %d heads over %d of %d lanes (whole groups of 32, at most 256)", n, n_heads, n_kv, D);
     NN_CHECK(cap >= 0.0f && keep >= 0 && (keep == 0 || window > 0) && (head_gate == nullptr || gate_ld >= n_heads),
              "attention_q4: cap %f, %d kept keys, gate rows of %d", cap, keep, gate_ld);
-    NN_CHECK(bt_stride > 0 && n_pages > 0 && longest > 0, "attention_q4: %d pages, tables of %d, at most %d keys", n_pages, bt_stride, longest);
+    NN_CHECK(bt_rows > 0 && bt_stride > 0 && n_pages > 0 && longest > 0, "attention_q4: %d pages, %d tables of %d, at most %d keys", n_pages, bt_rows,
+             bt_stride, longest);
     const long need = nncpu_attention_q4_scratch(n, n_heads, n_kv, D, dt, longest);
     NN_CHECK(need <= part_floats, "attention_q4: %ld floats of scratch, %ld are needed", part_floats, need);
     if (n == 0) return 0;
-    AttnQ4 p{q, dt, k_pages, v_pages, n_pages, block_table, bt_stride, tok_seq, tok_pos, out, part, n, n_heads, n_kv, D, scale, window, keep,
+    AttnQ4 p{q, dt, k_pages, v_pages, n_pages, block_table, bt_rows, bt_stride, tok_seq, tok_pos, out, part, n, n_heads, n_kv, D, scale, window, keep,
              slope_base, sinks, cap, head_gate, gate_ld, any_splits(n, n_heads, n_kv, longest)};
     const int group = n_heads / n_kv;
     if (streams(dt, D)) {

@@ -344,7 +344,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                     for (int pg = 0; pg < pages; ++pg)
                         for (int s = 0; s < kSlabs; ++s)
                             tma_load_4d(smem_k + st * kKBytes + s * kKvSlab + pg * (kPage * 128), &map_k, &k_full[st],
-                                        64 * s, 0, kvh, table[walk.page(2 * (s0 + jk) + pg)]);
+                                        64 * s, 0, kvh, table[kHalf ? min(walk.page(2 * (s0 + jk) + pg), p.bt_stride - 1) : walk.page(2 * (s0 + jk) + pg)]);
                     ++jk;
                     moved = true;
                 }
@@ -355,7 +355,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                     for (int pg = 0; pg < pages; ++pg)
                         for (int s = 0; s < kVSlabs; ++s)
                             tma_load_4d(smem_v + st * kVBytes + s * kKvSlab + pg * (kPage * 128), &map_v, &v_full[st],
-                                        64 * s, 0, kvh, table[walk.page(2 * (s0 + jv) + pg)]);
+                                        64 * s, 0, kvh, table[kHalf ? min(walk.page(2 * (s0 + jv) + pg), p.bt_stride - 1) : walk.page(2 * (s0 + jv) + pg)]);
                     ++jv;
                     moved = true;
                 }

@@ -24,8 +24,8 @@ struct Append {
     int half;
     const int* tok_seq;
     const int* tok_pos;
-    const int* block_table; // [*, bt_stride]
-    int bt_stride;
+    const int* block_table; // [bt_rows, bt_stride]
+    int bt_rows, bt_stride;
     uint8_t* k_pages;       // [n_pages, n_kv, 40 D]
     uint8_t* v_pages;
     int n_pages;
@@ -43,8 +43,8 @@ __device__ __forceinline__ double warp_sum64(double v) {
 }
 
 // The page of a token's key, or -1 (a padding row, a position without a page).
-__device__ __forceinline__ int page_of(const int* block_table, int bt_stride, int n_pages, int seq, int pos) {
-    if (seq < 0 || pos < 0 || pos / kPage >= bt_stride) return -1;
+__device__ __forceinline__ int page_of(const int* block_table, int bt_rows, int bt_stride, int n_pages, int seq, int pos) {
+    if (seq < 0 || seq >= bt_rows || pos < 0 || pos / kPage >= bt_stride) return -1;
     const int p = block_table[(size_t)seq * bt_stride + pos / kPage];
     return p < n_pages ? p : -1;
 }
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(256) append_kernel(const Append a) {
     }
     const bool value = h >= a.n_heads + a.n_kv;
     const int kvh = (h - a.n_heads) - (value ? a.n_kv : 0);
-    const int page = page_of(a.block_table, a.bt_stride, a.n_pages, seq, pos);
+    const int page = page_of(a.block_table, a.bt_rows, a.bt_stride, a.n_pages, seq, pos);
     if (page < 0) return;
     if (!value) {
         // In 64 bits: a key next to the border of two codes takes one or the other by its last bit.  B200's 64-bit rate is half of
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(256) append_fast_kernel(const Append a) {
     if (a.k_gamma != nullptr) k_gamma = ld_f4(a.k_gamma, 4 * j, a.g_dt);
     float times = 1.0f;
     if (a.temp_coef != 0.0f) times = 1.0f + a.temp_coef * logf(floorf((float)(pos + 1) / (float)a.temp_every) + 1.0f);
-    const int page = a.n_kv > 0 ? page_of(a.block_table, a.bt_stride, a.n_pages, seq, pos) : -1;
+    const int page = a.n_kv > 0 ? page_of(a.block_table, a.bt_rows, a.bt_stride, a.n_pages, seq, pos) : -1;
     const int at = page < 0 ? 0 : pos % kPage;
     const float* row = reinterpret_cast<const float*>(a.qkv) + (size_t)t * a.ld;
     // The heads of two rounds ahead are asked for before a round's are worked on.  (All threads of a warp go round together: a round's
@@ -284,7 +284,7 @@ __device__ __forceinline__ void put8(void* out, long i, int dt, const float (&x)
     }
 }
 __global__ void __launch_bounds__(256) read_kernel(const uint8_t* k_pages, const uint8_t* v_pages, int n_pages, const int* block_table,
-                                                   int bt_stride, const int* tok_seq, const int* tok_pos, void* k_out, void* v_out,
+                                                   int bt_rows, int bt_stride, const int* tok_seq, const int* tok_pos, void* k_out, void* v_out,
                                                    int out_dt, int n, int n_kv, int D) {
     wait_for_previous_kernels();
     let_next_kernel_start();
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(256) read_kernel(const uint8_t* k_pages, const
     if (i >= (long)n * per_tok) return;
     const int t = (int)(i / per_tok), rest = (int)(i - (long)t * per_tok), h = rest / (D / 8), lane = (rest - h * (D / 8)) * 8;
     const int g = lane >> 5, c = (lane & 31) >> 3, pos = tok_pos[t];
-    const int page = page_of(block_table, bt_stride, n_pages, tok_seq[t], pos), at = page < 0 ? 0 : pos % kPage;
+    const int page = page_of(block_table, bt_rows, bt_stride, n_pages, tok_seq[t], pos), at = page < 0 ? 0 : pos % kPage;
     float k[8] = {}, v[8] = {};
     if (page >= 0) {
         const size_t base = ((size_t)page * n_kv + h) * q4_page_bytes(D);
@@ -324,11 +324,13 @@ struct Expand {
     const int* block_table;
     int bt_stride;
     const int* cu_seqlens;
+    const int* tok_seq;
     const int* tok_pos;
     void* k_out;            // [n_seqs * width, n_kv, 64, lanes]
     void* v_out;
     int* table;             // [n_seqs, width]
-    int n_kv, D, lanes, window, keep;
+    int* places;            // null, or [2, n_tok]: the tokens' sequences (-1: without a table) and positions (within it)
+    int n_tok, n_kv, D, lanes, window, keep;
 };
 
 __device__ __forceinline__ void put8_row(float* row, const float (&x)[8]) {
@@ -355,6 +357,12 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const Expand p) 
     const bool values = blockIdx.y >= p.n_kv;
     const int h = values ? blockIdx.y - p.n_kv : blockIdx.y;
     if (blockIdx.y == 0 && threadIdx.x == 0) p.table[row] = row;
+    if (blockIdx.y == 1 && p.places != nullptr)
+        for (int i = row * kExpandThreads + threadIdx.x; i < p.n_tok; i += gridDim.x * gridDim.z * kExpandThreads) {
+            const int seq = p.tok_seq[i], pos = p.tok_pos[i];
+            p.places[i] = pos < 0 || seq >= (int)gridDim.z ? -1 : seq;
+            p.places[p.n_tok + i] = min(pos, (int)gridDim.x * kPage - 1);
+        }
     int id = pi < p.bt_stride ? p.block_table[(size_t)b * p.bt_stride + pi] : -1;      // (asked for beside the next two)
     const int t0 = p.cu_seqlens[b], t1 = p.cu_seqlens[b + 1];
     if (t1 <= t0) return;
@@ -400,7 +408,7 @@ static bool q4_lanes_ok(int D) { return D >= 32 && D <= 256 && D % 32 == 0; }
 
 extern "C" int nncpu_qk_norm_rope_append_q4(const void* qkv, int qkv_dt, int ld, const void* q_gamma, const void* k_gamma, int g_dt,
                                             double eps, const float* cos_sin, int half, const int* tok_seq, const int* tok_pos,
-                                            const int* block_table, int bt_stride, uint8_t* k_pages, uint8_t* v_pages, int n_pages,
+                                            const int* block_table, int bt_rows, int bt_stride, uint8_t* k_pages, uint8_t* v_pages, int n_pages,
                                             void* q_out, int q_dt, int n, int n_heads, int n_kv, int D, float temp_coef,
                                             int temp_every, cudaStream_t stream) {
     NN_CHECK(q4_lanes_ok(D), "qk_norm_rope_append_q4: heads of %d lanes (whole groups of 32, at most 256)", D);
@@ -410,7 +418,7 @@ extern "C" int nncpu_qk_norm_rope_append_q4(const void* qkv, int qkv_dt, int ld,
     NN_CHECK(temp_coef == 0.0f || temp_every > 0, "qk_norm_rope_append_q4: a temperature every %d positions", temp_every);
     if (n == 0) return 0;
     Append a{qkv, qkv_dt, ld, q_gamma, k_gamma, g_dt, eps, reinterpret_cast<const float2*>(cos_sin), half, tok_seq, tok_pos, block_table,
-             bt_stride, k_pages, v_pages, n_pages, q_out, q_dt, n, n_heads, n_kv, D, temp_coef, temp_every};
+             bt_rows, bt_stride, k_pages, v_pages, n_pages, q_out, q_dt, n, n_heads, n_kv, D, temp_coef, temp_every};
     if ((D == 32 || D == 64 || D == 128) && qkv_dt == DT_F32 && ld % 4 == 0 && (cos_sin == nullptr || half == D / 2) && (uintptr_t)qkv % 16 == 0 &&
         (uintptr_t)q_out % 16 == 0 && (uintptr_t)cos_sin % 16 == 0 && (uintptr_t)q_gamma % 16 == 0 && (uintptr_t)k_gamma % 16 == 0) {
         const int rounds = (n_heads + 2 * n_kv + 1024 / D - 1) / (1024 / D);      // a block's rounds, were it alone with a token
@@ -444,11 +452,11 @@ extern "C" int nncpu_qk_norm_rope_append_q4(const void* qkv, int qkv_dt, int ld,
     return 0;
 }
 
-extern "C" int nncpu_q4_read(const uint8_t* k_pages, const uint8_t* v_pages, int n_pages, const int* block_table, int bt_stride,
+extern "C" int nncpu_q4_read(const uint8_t* k_pages, const uint8_t* v_pages, int n_pages, const int* block_table, int bt_rows, int bt_stride,
                              const int* tok_seq, const int* tok_pos, void* k_out, void* v_out, int out_dt, int n, int n_kv, int D,
                              cudaStream_t stream) {
     NN_CHECK(q4_lanes_ok(D), "q4_read: heads of %d lanes (whole groups of 32, at most 256)", D);
-    NN_CHECK(n >= 0 && n_kv > 0 && bt_stride > 0 && n_pages > 0, "q4_read: %d tokens, %d heads, %d pages", n, n_kv, n_pages);
+    NN_CHECK(n >= 0 && n_kv > 0 && bt_rows >= 0 && bt_stride > 0 && n_pages > 0, "q4_read: %d tokens, %d heads, %d pages", n, n_kv, n_pages);
     if (n == 0) return 0;
     NN_CHECK((uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0, "q4_read: outputs start on 16-byte boundaries");
     const long items = (long)n * n_kv * D / 8;
@@ -460,16 +468,17 @@ extern "C" int nncpu_q4_read(const uint8_t* k_pages, const uint8_t* v_pages, int
     cudaLaunchAttribute attr[1];
     cfg.attrs = attr;
     cfg.numAttrs = overlap_attribute(attr);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, read_kernel, k_pages, v_pages, n_pages, block_table, bt_stride, tok_seq, tok_pos, k_out, v_out,
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, read_kernel, k_pages, v_pages, n_pages, block_table, bt_rows, bt_stride, tok_seq, tok_pos, k_out, v_out,
                                              out_dt, n, n_kv, D);
     NN_CHECK(e == cudaSuccess, "q4_read: launch failed: %s", cudaGetErrorString(e));
     return 0;
 }
 
-// half: float16, else float32.  q (or null): bfloat16 [n_tok, n_heads * D] to q_out [n_tok, n_heads * lanes].
+// half: float16, else float32.  places (or null): int32 [2, n_tok].  q (or null): bfloat16 [n_tok, n_heads * D] to q_out [n_tok, n_heads * lanes].
 extern "C" int nncpu_q4_expand(const uint8_t* k_pages, const uint8_t* v_pages, int n_pages, const int* block_table, int bt_stride,
-                               const int* cu_seqlens, const int* tok_pos, int n_seqs, int width, int n_kv, int D, int lanes, int window,
-                               int keep, int half, void* k_out, void* v_out, int* table, const void* q, void* q_out, int n_tok, int n_heads,
+                               const int* cu_seqlens, const int* tok_seq, const int* tok_pos, int n_seqs, int width, int n_kv, int D,
+                               int lanes, int window, int keep, int half, void* k_out, void* v_out, int* table, int* places, const void* q,
+                               void* q_out, int n_tok, int n_heads,
                                cudaStream_t stream) {
     NN_CHECK(q4_lanes_ok(D) && lanes >= D && lanes % 8 == 0, "q4_expand: heads of %d lanes in rows of %d", D, lanes);
     NN_CHECK(n_seqs > 0 && n_seqs <= 65535 && width > 0 && n_kv > 0 && n_kv <= 32767 && n_pages > 0 && bt_stride > 0,
@@ -479,7 +488,8 @@ extern "C" int nncpu_q4_expand(const uint8_t* k_pages, const uint8_t* v_pages, i
         longer_heads_kernel<<<(unsigned)((pieces + 255) / 256), 256, 0, stream>>>((const uint16_t*)q, (uint16_t*)q_out, (long)n_tok * n_heads, D, lanes);
         NN_LAUNCH_OK("q4_expand (queries)");
     }
-    const Expand p{k_pages, v_pages, n_pages, block_table, bt_stride, cu_seqlens, tok_pos, k_out, v_out, table, n_kv, D, lanes, window, keep};
+    const Expand p{k_pages, v_pages, n_pages, block_table, bt_stride, cu_seqlens, tok_seq, tok_pos, k_out, v_out, table, places,
+                   n_tok, n_kv, D, lanes, window, keep};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)width, (unsigned)(2 * n_kv), (unsigned)n_seqs);
     cfg.blockDim = dim3(kExpandThreads);

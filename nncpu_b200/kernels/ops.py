@@ -117,8 +117,8 @@ def launch_overlap(on: bool) -> None:
     """Whether kernels that can do so are launched to start while the kernel before them ends: a few-token
     product after a kernel of little shared memory and the float32 products of few rows (they ask for their first weights
     before they wait for that one's results), the tensor-core products (their set-up; up to 64 bfloat16 tokens also their first
-    weight tiles; above, and for float32 products of 96 tokens and more and the norms, the first weights go into L2 only), prefill attention (its set-up), float32 attention token by token, the norms and the small kernels of routers,
-    routed experts, gates and the stream between them.
+    weight tiles; above, and for float32 products of 96 tokens and more and the norms, the first weights go into L2 only), prefill attention (its set-up), float32 attention token by token, the norms, the small kernels of routers,
+    routed experts, gates and the stream between them, and a 4-bit cache's append, reads and merge.
     On by default; off, every kernel waits for the one before it to be over, and the results are the same bits.  Where a product
     asks for its first weights themselves, the kernel of this library right before it in the stream must not be the one that
     writes them."""
@@ -1672,7 +1672,7 @@ def _q4_places(fn: str, n: int, block_table, tok_seq, tok_pos) -> None:
     _need(tok_seq.numel() >= n and tok_pos.numel() >= n, fn, f"{n} tokens, {tok_seq.numel()} sequences and {tok_pos.numel()} positions of them")
 
 
-_APPEND_Q4 = [_P, _I, _I, _P, _P, _I, _D, _P, _I, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _F, _I]
+_APPEND_Q4 = [_P, _I, _I, _P, _P, _I, _D, _P, _I, _P, _P, _P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _F, _I]
 
 
 def qk_norm_rope_append_q4(qkv, q_gamma, k_gamma, eps: float, cos_sin, tok_seq, tok_pos, block_table, k_pages, v_pages, q_out,
@@ -1685,7 +1685,7 @@ def qk_norm_rope_append_q4(qkv, q_gamma, k_gamma, eps: float, cos_sin, tok_seq, 
     d = (hi - lo) / 15 and lo both float16, and c = round((x - lo) / d) one of 0 to 15: a number is off by at most half a step d (and
     lo's rounding).  Numbers beyond +-65504 count as that; a group with a NaN is NaN.  Keys are normed and rotated in 64 bits, so
     that a code does not hang on the order of a sum.  ``n_kv`` 0: qkv holds q only and nothing is appended.  A token of sequence -1, or
-    whose position has no page, is not appended; two tokens at one place leave either.  ``q_temp`` as in ``qk_norm_rope_append``."""
+    whose position has no page, is not appended; two tokens of a call must not have the same place.  ``q_temp`` as in ``qk_norm_rope_append``."""
     n, rows = q_out.shape[0], qkv.shape
     half = 0 if cos_sin is None else cos_sin.shape[1]
     coef, every = q_temp if q_temp is not None else (0.0, 1)
@@ -1708,16 +1708,16 @@ def qk_norm_rope_append_q4(qkv, q_gamma, k_gamma, eps: float, cos_sin, tok_seq, 
         _need(False, fn, f"{n_heads} heads over {n_kv} of {head_dim} lanes of {tok_seq.numel()} tokens in rows of {list(rows)}, "
               f"queries to {list(q_out.shape)}")
     g = q_gamma if q_gamma is not None else k_gamma
-    width, n_pages = (block_table.shape[1], k_pages.shape[0]) if n_kv else (0, 0)
+    (tables, width), n_pages = (block_table.shape, k_pages.shape[0]) if n_kv else ((0, 0), 0)
     if not n_kv:
         block_table = k_pages = v_pages = None
     qkv_at, qg_at, kg_at, cs_at, seq_at, pos_at, table_at, k_at, v_at, q_at = _addresses(
         "qk_norm_rope_append_q4", qkv, q_gamma, k_gamma, cos_sin, tok_seq, tok_pos, block_table, k_pages, v_pages, q_out)
     _launch("cache_q4", "nncpu_qk_norm_rope_append_q4", _APPEND_Q4, qkv_at, _code(qkv), rows[1], qg_at, kg_at, _code(g), eps, cs_at, half, seq_at,
-            pos_at, table_at, width, k_at, v_at, n_pages, q_at, _code(q_out), n, n_heads, n_kv, head_dim, coef, every)
+            pos_at, table_at, tables, width, k_at, v_at, n_pages, q_at, _code(q_out), n, n_heads, n_kv, head_dim, coef, every)
 
 
-_READ_Q4 = [_P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I]
+_READ_Q4 = [_P, _P, _I, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I]
 
 
 def q4_read(k_pages, v_pages, block_table, tok_seq, tok_pos, k_out, v_out) -> None:
@@ -1732,8 +1732,8 @@ def q4_read(k_pages, v_pages, block_table, tok_seq, tok_pos, k_out, v_out) -> No
         _q4_places("q4_read", n, block_table, tok_seq, tok_pos)
         _need(False, "q4_read", f"keys to {k_out.dtype} {list(k_out.shape)}, values to {v_out.dtype} {list(v_out.shape)}")
     k_at, v_at, table_at, seq_at, pos_at, k_to, v_to = _addresses("q4_read", k_pages, v_pages, block_table, tok_seq, tok_pos, k_out, v_out)
-    _launch("cache_q4", "nncpu_q4_read", _READ_Q4, k_at, v_at, pages[0], table_at, block_table.shape[1], seq_at, pos_at, k_to, v_to, _code(k_out), n,
-            n_kv, head_dim)
+    _launch("cache_q4", "nncpu_q4_read", _READ_Q4, k_at, v_at, pages[0], table_at, *block_table.shape, seq_at, pos_at, k_to, v_to, _code(k_out), n, n_kv,
+            head_dim)
 
 
 def _attention_q4_check(fn: str, q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads: int, n_kv: int, head_dim: int,
@@ -1782,7 +1782,7 @@ def attention_q4_scratch_floats(n_tok: int, n_heads: int, n_kv: int, head_dim: i
     return _attention_q4_scratch(torch._C._cuda_getDevice(), n_tok, n_heads, n_kv, head_dim, _DT[dtype], longest)
 
 
-_ATTENTION_Q4 = [_P, _I, _P, _P, _I, _P, _I, _P, _P, _P, _P, _L, _I, _I, _I, _I, _F, _I, _I, _F, _P, _F, _P, _I, _I, _P]
+_ATTENTION_Q4 = [_P, _I, _P, _P, _I, _P, _I, _I, _P, _P, _P, _P, _L, _I, _I, _I, _I, _F, _I, _I, _F, _P, _F, _P, _I, _I, _P]
 
 
 def attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads: int, n_kv: int, head_dim: int, scale: float,
@@ -1807,7 +1807,7 @@ def attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_head
     elif scratch is not None and scratch.dtype is not torch.float32:
         raise InvalidArgument("attention_q4: scratch is float32")
     gate_at, gate_ld = _q4_gate("attention_q4", head_gate, n, n_heads)
-    _launch("attention_q4", "nncpu_attention_q4", _ATTENTION_Q4, q_at, code, k_at, v_at, k_pages.shape[0], table_at, block_table.shape[1], seq_at,
+    _launch("attention_q4", "nncpu_attention_q4", _ATTENTION_Q4, q_at, code, k_at, v_at, k_pages.shape[0], table_at, *block_table.shape, seq_at,
             pos_at, out_at, scratch_at, 0 if scratch is None else scratch.numel(), n, n_heads, n_kv, head_dim, scale, window, keep, slope_base,
             sinks_at, cap, gate_at, gate_ld, longest, None)
 
@@ -1825,7 +1825,7 @@ Q4_EXPAND_POSITIONS_F32 = 65536
 @functools.lru_cache(maxsize=4096)
 def _q4_prompt_plan(n: int, n_seqs: int, n_heads: int, n_kv: int, head_dim: int, bf16: bool, longest: int, slope_and_cap: bool):
     """How a prompt attends: (lanes of the rows that the keys are taken out to, or 0: straight from the codes; pages of a sequence;
-    sequences at a time; bytes of keys; of keys, values and table; of all)."""
+    sequences at a time; bytes of keys; of keys, values, table and (float32) the tokens' sequences and positions; of all)."""
     width = (longest + 63) // 64
     lanes = 0
     if n <= n_seqs or (bf16 and n_seqs == 1 and n <= Q4_FEW_TOKENS and head_dim <= 128):
@@ -1839,17 +1839,19 @@ def _q4_prompt_plan(n: int, n_seqs: int, n_heads: int, n_kv: int, head_dim: int,
     at_once = max(1, min(n_seqs, Q4_EXPAND_POSITIONS // (width * 64))) if bf16 else n_seqs
     kv_bytes = at_once * width * n_kv * 64 * lanes * (2 if bf16 else 4)
     table = 2 * kv_bytes + (at_once * width * 4 + 255) // 256 * 256
+    if not bf16:
+        table += n * 8
     return lanes, width, at_once, kv_bytes, table, table + (n * n_heads * lanes * 2 if bf16 and lanes != head_dim else 0)
 
 
 def attention_q4_prompt_scratch_bytes(n_tok: int, n_seqs: int, n_heads: int, n_kv: int, head_dim: int, dtype, longest: int,
                                       slope_base: float = 0.0, cap: float = 0.0) -> int:
-    """Bytes of scratch that ``attention_q4_prompt`` needs at these sizes on the current device."""
+    """Bytes of scratch that ``attention_q4_prompt`` needs at these sizes on the current device; ``longest``: that call's."""
     plan = _q4_prompt_plan(n_tok, n_seqs, n_heads, n_kv, head_dim, dtype == torch.bfloat16, longest, slope_base != 0.0 and cap != 0.0)
     return plan[5] if plan[0] else 4 * attention_q4_scratch_floats(n_tok, n_heads, n_kv, head_dim, dtype, longest)
 
 
-_EXPAND_Q4 = [_P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I]
+_EXPAND_Q4 = [_P, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I]
 _PREFILL_HALF = [_P, _P, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _F, _P, _F, _P, _I, _I, _P]
 
 
@@ -1860,7 +1862,8 @@ def attention_q4_prompt(q, k_pages, v_pages, block_table, cu_seqlens, tok_seq, t
     int32 [n_seqs + 1]: each sequence's first token).  ``longest``: at least as many keys as any token sees.  ``status``: an int32 word on
     the device that receives a code if a bounded wait runs out, as in ``attention_prefill_tc``.  ``scratch``: uint8,
     ``attention_q4_prompt_scratch_bytes`` elements (None: taken from the allocator).  What is left in the rows of no sequence is not said;
-    a page that is not there may count as zeros."""
+    a page that is not there may count as zeros, and a NaN that the cache holds may reach tokens before it in the same step, as in the
+    attention over a bfloat16 cache."""
     fn = "attention_q4_prompt"
     n = _attention_q4_check(fn, q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads, n_kv, head_dim, window, keep, cap, sinks)
     if not (cu_seqlens.dtype is torch.int32 and cu_seqlens.dim() == 1 and 0 < n_seqs < cu_seqlens.shape[0] and longest > 0
@@ -1887,26 +1890,28 @@ def attention_q4_prompt(q, k_pages, v_pages, block_table, cu_seqlens, tok_seq, t
     if n == 0:
         return
     if lanes == 0:
-        _launch("attention_q4", "nncpu_attention_q4", _ATTENTION_Q4, q_at, code, k_at, v_at, k_pages.shape[0], table_at, table_width, seq_at, pos_at,
-                out_at, base, need // 4, n, n_heads, n_kv, head_dim, scale, window, keep, slope_base, sinks_at, cap, gate_at, gate_ld, longest,
+        _launch("attention_q4", "nncpu_attention_q4", _ATTENTION_Q4, q_at, code, k_at, v_at, k_pages.shape[0], table_at, *block_table.shape, seq_at,
+                pos_at, out_at, base, need // 4, n, n_heads, n_kv, head_dim, scale, window, keep, slope_base, sinks_at, cap, gate_at, gate_ld, longest,
                 cu_at if bf16 and n_seqs == 1 and head_dim <= 128 else None)
         return
     if _dry:
         table_at = cu_at = base = 0
     k_to, v_to, table_to, q_to = base, base + kv_bytes, base + 2 * kv_bytes, base + table_end
+    seq_to, pos_to = base + table_end - 8 * n, base + table_end - 4 * n         # (float32 only)
     longer = bf16 and lanes != head_dim
     for b in range(0, n_seqs, at_once):
         count = min(at_once, n_seqs - b)
         cu = cu_at + 4 * b
-        _launch("cache_q4", "nncpu_q4_expand", _EXPAND_Q4, k_at, v_at, k_pages.shape[0], table_at + 4 * b * table_width, table_width, cu, pos_at,
-                count, width, n_kv, head_dim, lanes, window, keep, bf16, k_to, v_to, table_to, q_at if longer and b == 0 else None,
+        _launch("cache_q4", "nncpu_q4_expand", _EXPAND_Q4, k_at, v_at, k_pages.shape[0], table_at + 4 * b * table_width, table_width, cu, seq_at,
+                pos_at, count, width, n_kv, head_dim, lanes, window, keep, bf16, k_to, v_to, table_to, None if bf16 else seq_to,
+                q_at if longer and b == 0 else None,
                 q_to if longer else None, n, n_heads)
         if bf16:
             _launch("attention_tc", "nncpu_attention_prefill_tc_half", _PREFILL_HALF, q_to if longer else q_at, k_to, v_to, count * width,
                     table_to, width, cu, pos_at, out_at, n, count, n_heads, n_kv, lanes, head_dim, scale, window, keep, slope_base, sinks_at,
                     cap, gate_at, gate_ld, longest, status_at)
         else:
-            _launch("attention_f32", "nncpu_attention_f32", _PROMPT_F32, q_at, k_to, v_to, table_to, width, seq_at, pos_at, out_at, None, n,
+            _launch("attention_f32", "nncpu_attention_f32", _PROMPT_F32, q_at, k_to, v_to, table_to, width, seq_to, pos_to, out_at, None, n,
                     n_heads, n_kv, head_dim, head_dim, head_dim, scale, window, keep, slope_base, sinks_at, cap, gate_at, gate_ld, 0, 0, n_seqs,
                     148 if _dry else torch.cuda.get_device_properties(q.device).multi_processor_count)
 

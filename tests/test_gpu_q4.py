@@ -330,3 +330,135 @@ def test_too_little_scratch_is_refused():
     assert ops.attention_q4_scratch_floats(1, 1, 1, 64, F32, 4096) > 8
     with pytest.raises(Exception, match="scratch"):
         ops.attention_q4(q, kp, kp, table, one, one, out, 1, 1, 64, 1.0, scratch=torch.zeros(8, device=DEV))
+
+
+# -- as a program calls them -----------------------------------------------------------------------------------------------
+
+
+def prompt_call(dt, lens, new, heads=8, kv=2, D=128, seed=0, pad=0):
+    """A call of attention_q4_prompt over sequences of ``lens`` keys that bring ``new`` tokens: (call(out), q, out, what check_rows needs).
+    ``pad`` rows of no sequence stand behind the last."""
+    kp, vp, table, ks, vs = Q.filled_cache(lens, kv, D, seed)
+    seq, pos, cu = places(new, [n - m for n, m in zip(lens, new)])
+    seq, pos = np.concatenate([seq, np.full(pad, -1, np.int32)]), np.concatenate([pos, np.full(pad, 0, np.int32)])
+    kp, vp, table, ts, tp, cud = Q.as_cuda(kp, vp, table, seq, pos, cu)
+    q = rand(len(seq), heads * D, seed=seed + 1).to(dt).to(DEV)
+    out, status = torch.zeros_like(q), torch.zeros(1, dtype=torch.int32, device=DEV)
+
+    def call(to=out):
+        ops.attention_q4_prompt(q, kp, vp, table, cud, ts, tp, to, len(new), heads, kv, D, D ** -0.5, max(lens), status)
+    return call, q, out, (ks, vs, seq, pos, dt, heads, D ** -0.5), tp
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("lens,new", [([700, 33, 400], [200, 33, 0]), ([500], [20]), ([128, 300], [128, 1])])
+def test_prompts_with_padding_and_with_sequences_that_bring_nothing(lens, new, dt):
+    call, q, out, (ks, vs, seq, pos, *rest), _ = prompt_call(dt, lens, new, pad=5)
+    call()
+    n = sum(new)
+    check_rows(out[:n], q[:n], ks, vs, seq[:n], pos[:n], *rest)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("lens,new", [([700, 200], [200, 90]), ([500], [20])])
+def test_prompts_captured_and_replayed_on_other_places(lens, new, dt):
+    call, q, out, (ks, vs, seq, pos, *rest), tp = prompt_call(dt, lens, new)
+    call()
+    check_rows(out, q, ks, vs, seq, pos, *rest)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    out.zero_()
+    tp -= 60        # the same tokens, each 60 positions earlier
+    q.copy_(rand(*q.shape, seed=9).to(dt))
+    graph.replay()
+    check_rows(out, q, ks, vs, seq, pos - 60, *rest)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_calls_on_two_streams_do_not_disturb_one_another(dt):
+    a, _, out_a, _, _ = prompt_call(dt, [900, 300], [300, 200], seed=3)
+    b, _, out_b, _, _ = prompt_call(dt, [500], [40], seed=4)
+    a(), b()
+    torch.cuda.synchronize()
+    want_a, want_b = out_a.clone(), out_b.clone()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[torch.zeros_like(out_a) for _ in range(6)], [torch.zeros_like(out_b) for _ in range(6)]]
+    torch.cuda.synchronize()
+    for i in range(6):
+        for call, to, stream in zip((a, b), got, streams):
+            with torch.cuda.stream(stream):
+                call(to[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, want_a) for t in got[0]) and all(torch.equal(t, want_b) for t in got[1])
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_the_same_bits_without_launches_that_overlap(dt):
+    def run():
+        kp, vp, table, _, _ = Q.filled_cache([200, 4097, 65], 2, 128, 6)
+        kp, vp, table, seq, pos = Q.as_cuda(kp, vp, table, np.arange(3, dtype=np.int32), np.array([199, 4096, 64], np.int32))
+        q, out = torch.empty(3, 1024, dtype=dt, device=DEV), torch.empty(3, 1024, dtype=dt, device=DEV)
+        qkv = rand(3, 12 * 128, seed=2).to(DEV)
+        ops.qk_norm_rope_append_q4(qkv, None, None, 1e-6, None, seq, pos, table, kp, vp, q, 8, 2, 128)
+        ops.attention_q4(q, kp, vp, table, seq, pos, out, 8, 2, 128, 0.1)
+        k = torch.empty(3, 256, device=DEV)
+        ops.q4_read(kp, vp, table, seq, pos, k, torch.empty_like(k))
+        call, _, prompt, _, _ = prompt_call(dt, [700, 200], [200, 90])
+        call()
+        torch.cuda.synchronize()
+        return out, k, prompt
+    want = run()
+    ops.launch_overlap(False)
+    try:
+        got = run()
+    finally:
+        ops.launch_overlap(True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_no_tokens(dt):
+    kp, vp, table, _, _ = Q.filled_cache([64], 1, 64, 0)
+    before = kp.copy()
+    kp, vp, table, none = Q.as_cuda(kp, vp, table, np.zeros(0, np.int32))
+    cu, status = torch.zeros(2, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    q, kv = torch.empty(0, 64, dtype=dt, device=DEV), torch.empty(0, 64, device=DEV)
+    ops.qk_norm_rope_append_q4(torch.empty(0, 192, device=DEV), None, None, 1e-6, None, none, none, table, kp, vp, q, 1, 1, 64)
+    ops.q4_read(kp, vp, table, none, none, kv, kv.clone())
+    ops.attention_q4(q, kp, vp, table, none, none, torch.empty_like(q), 1, 1, 64, 0.1)
+    ops.attention_q4_prompt(q, kp, vp, table, cu, none, none, torch.empty_like(q), 1, 1, 1, 64, 0.1, 64, status)
+    assert np.array_equal(kp.cpu().numpy(), before)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_sequences_without_a_table(dt):
+    """A token of a sequence behind the tables' last is nobody's: nothing is written, zeros are read, and it attends to nothing."""
+    kp, vp, table, ks, vs = Q.filled_cache([100, 70], 2, 128, 0)
+    before = kp.copy()
+    seq = np.array([1, 2, 900, 0], np.int32)
+    pos = np.array([69, 5, 0, 99], np.int32)
+    kp, vp, table, ts, tp = Q.as_cuda(kp, vp, table, seq, pos)
+    q = rand(4, 1024).to(dt).to(DEV)
+    out = torch.full_like(q, 3.0)
+    ops.attention_q4(q, kp, vp, table, ts, tp, out, 8, 2, 128, 0.1)
+    check_rows(out, q, ks, vs, [1, -1, -1, 0], pos, dt, 8, 0.1)
+    k, v = torch.ones(4, 256, device=DEV), torch.ones(4, 256, device=DEV)
+    ops.q4_read(kp, vp, table, ts, tp, k, v)
+    assert (k[1:3] == 0).all() and (v[1:3] == 0).all() and (k[0] != 0).any() and (k[3] != 0).any()
+    ops.qk_norm_rope_append_q4(rand(2, 12 * 128).to(DEV), None, None, 1e-6, None, ts[1:3].clone(), tp[1:3].clone(), table, kp, vp, q[:2], 8, 2, 128)
+    assert np.array_equal(kp.cpu().numpy(), before)
+
+
+def test_scratch_that_starts_off_its_boundary_is_refused():
+    lens, new = [700, 200], [200, 90]
+    kp, vp, table, _, _ = Q.filled_cache(lens, 2, 128, 0)
+    seq, pos, cu = places(new, [500, 110])
+    kp, vp, table, ts, tp, cu = Q.as_cuda(kp, vp, table, seq, pos, cu)
+    q = rand(290, 1024).bfloat16().to(DEV)
+    need = ops.attention_q4_prompt_scratch_bytes(290, 2, 8, 2, 128, BF16, 700)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for scratch in (torch.empty(need + 8, dtype=torch.uint8, device=DEV)[8:], torch.empty(need - 1, dtype=torch.uint8, device=DEV),
+                    torch.empty(need, dtype=torch.int8, device=DEV)):
+        with pytest.raises(Exception, match="scratch"):
+            ops.attention_q4_prompt(q, kp, vp, table, cu, ts, tp, torch.empty_like(q), 2, 8, 2, 128, 0.1, 700, status, scratch=scratch)

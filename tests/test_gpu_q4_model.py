@@ -233,3 +233,22 @@ def test_command_line(folders, tmp_path):
     f.write_text("7")
     assert main(["--perplexity", folder, str(f)]) == 1
     assert main(["--perplexity", folder, str(tmp_path / "none")]) == 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_arena_is_sized_ahead_and_steps_take_nothing_from_the_allocator(folders, dtype):
+    engine = Engine(Model.load(folders["D", dtype], dtype=dtype), max_tokens=64 * 24, kv_dtype="q4", max_step_tokens=256)
+    assert engine.arena.peak > 0
+    a, b = engine.alloc_slot(), engine.alloc_slot()
+
+    def steps():
+        engine.step([a, b], [ids(100, 1), ids(30, 2)])
+        engine.step([a, b], [[5], [6]])
+        engine.step([a], [ids(17, 3)])
+    steps()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    steps()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before and torch.cuda.max_memory_allocated() - before < 1 << 16     # (metadata and ids)
