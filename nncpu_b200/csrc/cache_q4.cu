@@ -152,35 +152,42 @@ __global__ void __launch_bounds__(256) append_kernel(const Append a) {
 }
 
 // ---------------------------------------------------------------------------
-// Heads of 32, 64 and 128 lanes, rotated whole or not at all, in float32 rows of whole 16-byte pieces: T = D / 4 threads a head, each
-// with four neighbouring lanes, so that a rotation's partner is T / 2 threads away, a group is eight threads, and a thread's four
-// codes are the half of a word that it stores.  A block takes a token and as many heads as it has rounds for, which share the token's
-// angles.  grid = (n, blocks a token), 256 threads.
+// Heads of 32, 64 and 128 lanes, rotated whole or not at all, in float32 rows of whole 16-byte pieces: T = D / 8 threads a head, each
+// with four neighbouring lanes of either half, so that a rotation's partners are in one thread, a group is eight threads, and a
+// thread's codes are two halves of words, which it stores.  A block takes a token and as many heads as it has rounds for, which share
+// the token's angles.  grid = (n, blocks a token), 256 threads.
+// Bound by instructions (62 % of the issue slots with four lanes a thread, whose rotation and norm took nine exchanges a head): 2 048
+// tokens of 32 heads over 8 of 128 lanes, read back after, take 25.3 us; 31.8 with four lanes a thread; 32.5 and 27.2 in the registers
+// of two and three blocks an SM.  Their bytes alone would take 12.1 us.
 // ---------------------------------------------------------------------------
 template <int D, typename F>
-__device__ __forceinline__ void norm_rotate4(F (&x)[4], const float4* gamma, const float2 (&cs)[4], bool rotated, F eps, int j) {
-    constexpr int T = D / 4;
+__device__ __forceinline__ void norm_rotate8(F (&x)[8], const float4* gamma, const float2 (&cs)[4], bool rotated, F eps) {
+    constexpr int T = D / 8;
     if (gamma != nullptr) {
-        F s = (x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]);
+        F s = ((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])) + ((x[4] * x[4] + x[5] * x[5]) + (x[6] * x[6] + x[7] * x[7]));
 #pragma unroll
         for (int o = T / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         F r;
         if constexpr (sizeof(F) == 8) r = rsqrt(s / F(D) + eps);
         else r = rsqrtf(s * (1.0f / D) + eps);
-        x[0] *= r * F(gamma->x); x[1] *= r * F(gamma->y); x[2] *= r * F(gamma->z); x[3] *= r * F(gamma->w);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[4 * i] *= r * F(gamma[i].x); x[4 * i + 1] *= r * F(gamma[i].y); x[4 * i + 2] *= r * F(gamma[i].z); x[4 * i + 3] *= r * F(gamma[i].w);
+        }
     }
     if (rotated) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const F other = __shfl_xor_sync(0xffffffffu, x[e], T / 2);
-            x[e] = j >= T / 2 ? x[e] * F(cs[e].x) + other * F(cs[e].y) : x[e] * F(cs[e].x) - other * F(cs[e].y);
+            const F a = x[e], b = x[e + 4];
+            x[e] = a * F(cs[e].x) - b * F(cs[e].y);
+            x[e + 4] = b * F(cs[e].x) + a * F(cs[e].y);
         }
     }
 }
 
 template <int D>
-__global__ void __launch_bounds__(256) append_fast_kernel(const Append a) {
-    constexpr int T = D / 4, NG = D / 32, kHeads = 256 / T;
+__global__ void __launch_bounds__(256, 4) append_fast_kernel(const Append a) {
+    constexpr int T = D / 8, NG = D / 32, kHeads = 256 / T;
     const int t = blockIdx.x, j = threadIdx.x % T, per_tok = a.n_heads + 2 * a.n_kv;
     wait_for_previous_kernels();
     let_next_kernel_start();
@@ -188,83 +195,103 @@ __global__ void __launch_bounds__(256) append_fast_kernel(const Append a) {
     const bool rotated = a.cs != nullptr;
     float2 cs[4] = {};
     if (rotated) {
-        const float4* at = reinterpret_cast<const float4*>(a.cs + (size_t)t * (D / 2) + j % (T / 2) * 4);
+        const float4* at = reinterpret_cast<const float4*>(a.cs + (size_t)t * (D / 2) + 4 * j);
         const float4 u = at[0], v = at[1];
         cs[0] = make_float2(u.x, u.y); cs[1] = make_float2(u.z, u.w); cs[2] = make_float2(v.x, v.y); cs[3] = make_float2(v.z, v.w);
     }
-    float4 q_gamma = {}, k_gamma = {};
-    if (a.q_gamma != nullptr) q_gamma = ld_f4(a.q_gamma, 4 * j, a.g_dt);
-    if (a.k_gamma != nullptr) k_gamma = ld_f4(a.k_gamma, 4 * j, a.g_dt);
     float times = 1.0f;
     if (a.temp_coef != 0.0f) times = 1.0f + a.temp_coef * logf(floorf((float)(pos + 1) / (float)a.temp_every) + 1.0f);
     const int page = a.n_kv > 0 ? page_of(a.block_table, a.bt_rows, a.bt_stride, a.n_pages, seq, pos) : -1;
     const int at = page < 0 ? 0 : pos % kPage;
-    const float* row = reinterpret_cast<const float*>(a.qkv) + (size_t)t * a.ld;
-    // The heads of two rounds ahead are asked for before a round's are worked on.  (All threads of a warp go round together: a round's
-    // last heads may not be there.)
+    const float* row = reinterpret_cast<const float*>(a.qkv) + (size_t)t * a.ld + 4 * j;
+    // The next round's heads are asked for before a round's are worked on.  (All threads of a warp go round together: a round's last
+    // heads may not be there.)
     const int stride = gridDim.y * kHeads, first = blockIdx.y * kHeads + threadIdx.x / T;
-    auto ask = [&](int h) { return h < per_tok ? *reinterpret_cast<const float4*>(row + (size_t)h * D + 4 * j) : make_float4(0, 0, 0, 0); };
-    float4 v = ask(first), v1 = ask(first + stride), v2 = ask(first + 2 * stride);
+    auto ask = [&](int h, int half) {
+        return h < per_tok ? *reinterpret_cast<const float4*>(row + (size_t)h * D + half * (D / 2)) : make_float4(0, 0, 0, 0);
+    };
+    float4 next0 = ask(first, 0), next1 = ask(first, 1);
     for (int h0 = blockIdx.y * kHeads; h0 < per_tok; h0 += stride) {
         const int h = h0 + threadIdx.x / T;
         const bool there = h < per_tok;
-        if (h0 > blockIdx.y * kHeads) {
-            v = v1;
-            v1 = v2;
-            v2 = ask(h + 2 * stride);
-        }
+        const float4 v0 = next0, v1 = next1;
+        next0 = ask(h + stride, 0);
+        next1 = ask(h + stride, 1);
+        float x[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
         // a warp's heads are of one kind (all of q, all of k, ...) or take every branch that one of them takes
         const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv;
+        float4 gamma[2] = {};
+        if (const void* g = is_q ? a.q_gamma : is_v ? nullptr : a.k_gamma) {
+            gamma[0] = ld_f4(g, 4 * j, a.g_dt);
+            gamma[1] = ld_f4(g, D / 2 + 4 * j, a.g_dt);
+        }
         if (__any_sync(0xffffffffu, there && is_q)) {
-            float x[4] = {v.x, v.y, v.z, v.w};
-            norm_rotate4<D, float>(x, a.q_gamma != nullptr ? &q_gamma : nullptr, cs, rotated, (float)a.eps, j);
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = x[e];
+            norm_rotate8<D, float>(y, a.q_gamma != nullptr ? gamma : nullptr, cs, rotated, (float)a.eps);
             if (there && is_q) {
                 const size_t to = ((size_t)t * a.n_heads + h) * D + 4 * j;
-                if (a.q_dt == DT_F32) {
-                    *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.q_out) + to) = make_float4(x[0] * times, x[1] * times, x[2] * times, x[3] * times);
-                } else {
-                    const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0] * times, x[1] * times), hi = __floats2bfloat162_rn(x[2] * times, x[3] * times);
-                    uint2 u;
-                    u.x = *reinterpret_cast<const uint32_t*>(&lo);
-                    u.y = *reinterpret_cast<const uint32_t*>(&hi);
-                    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.q_out) + to) = u;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float4 z = make_float4(y[4 * i] * times, y[4 * i + 1] * times, y[4 * i + 2] * times, y[4 * i + 3] * times);
+                    if (a.q_dt == DT_F32) {
+                        *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.q_out) + to + i * (D / 2)) = z;
+                    } else {
+                        const __nv_bfloat162 lo = __floats2bfloat162_rn(z.x, z.y), hi = __floats2bfloat162_rn(z.z, z.w);
+                        uint2 u;
+                        u.x = *reinterpret_cast<const uint32_t*>(&lo);
+                        u.y = *reinterpret_cast<const uint32_t*>(&hi);
+                        *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.q_out) + to + i * (D / 2)) = u;
+                    }
                 }
             }
         }
         if (!__any_sync(0xffffffffu, there && !is_q && page >= 0)) continue;
-        float x[4] = {v.x, v.y, v.z, v.w};
         if (__any_sync(0xffffffffu, there && !is_q && !is_v)) {
             // in 64 bits, see append_kernel
-            double y[4] = {v.x, v.y, v.z, v.w};
-            norm_rotate4<D, double>(y, a.k_gamma != nullptr ? &k_gamma : nullptr, cs, rotated, a.eps, j);
+            double y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = x[e];
+            norm_rotate8<D, double>(y, a.k_gamma != nullptr ? gamma : nullptr, cs, rotated, a.eps);
             if (!is_v)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = (float)y[e];
+                for (int e = 0; e < 8; ++e) x[e] = (float)y[e];
         }
-        bool bad = false;
-        float lo = kHalfMax, hi = -kHalfMax;
+        bool bad[2] = {};
+        float lo[2] = {kHalfMax, kHalfMax}, hi[2] = {-kHalfMax, -kHalfMax};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 8; ++e) {
             x[e] = q4_in_range(x[e]);
-            bad |= x[e] != x[e];
-            lo = fminf(lo, x[e]);
-            hi = fmaxf(hi, x[e]);
+            bad[e / 4] |= x[e] != x[e];
+            lo[e / 4] = fminf(lo[e / 4], x[e]);
+            hi[e / 4] = fmaxf(hi[e / 4], x[e]);
         }
+        if (D == 32) {          // (both halves are of one group, of four threads)
+            bad[0] = bad[1] = bad[0] | bad[1];
+            lo[0] = lo[1] = fminf(lo[0], lo[1]);
+            hi[0] = hi[1] = fmaxf(hi[0], hi[1]);
+        }
+        const int kvh = h - a.n_heads - (is_v ? a.n_kv : 0), quad = j & 7;
+        uint8_t* base = (is_v ? a.v_pages : a.k_pages) + ((size_t)max(page, 0) * a.n_kv + kvh) * q4_page_bytes(D);
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        for (int i = 0; i < 2; ++i) {
+            constexpr int kThreads = D == 32 ? 4 : 8;       // of a group
+#pragma unroll
+            for (int o = kThreads / 2; o > 0; o >>= 1) {
+                lo[i] = fminf(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
+                hi[i] = fmaxf(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
+            }
+            const unsigned any_bad = __ballot_sync(0xffffffffu, bad[i]);
+            if (any_bad >> (threadIdx.x & 31 & ~(kThreads - 1)) & ((1u << kThreads) - 1)) lo[i] = hi[i] = __int_as_float(0x7FC00000);
+            const Q4Scale s = q4_scale(lo[i], hi[i]);
+            const uint16_t codes = (uint16_t)q4_codes(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], s);
+            if (!there || is_q || page < 0) continue;
+            const int g = D == 32 ? 0 : j / 8 + i * (NG / 2), four = D == 32 ? j + 4 * i : quad;     // the group, and the four of its eight
+            const int half = is_v ? 2 * q4_value_word(at, four, g, NG) + (at & 1) : 2 * q4_key_word(at, four >> 1, g, NG) + (four & 1);
+            reinterpret_cast<uint16_t*>(base)[half] = codes;
+            if (four == 0) reinterpret_cast<__half2*>(base + q4_scales_at(D))[at * NG + g] = __halves2half2(s.d, s.m);
         }
-        const unsigned any_bad = __ballot_sync(0xffffffffu, bad);
-        if (any_bad >> (threadIdx.x & 24) & 255) lo = hi = __int_as_float(0x7FC00000);
-        const Q4Scale s = q4_scale(lo, hi);
-        const uint32_t codes = q4_code(x[0], s) | q4_code(x[1], s) << 4 | q4_code(x[2], s) << 8 | q4_code(x[3], s) << 12;
-        if (!there || is_q || page < 0) continue;
-        const int kvh = h - a.n_heads - (is_v ? a.n_kv : 0), g = j >> 3, quad = j & 7;
-        uint8_t* base = (is_v ? a.v_pages : a.k_pages) + ((size_t)page * a.n_kv + kvh) * q4_page_bytes(D);
-        const int half = is_v ? 2 * q4_value_word(at, quad, g, NG) + (at & 1) : 2 * q4_key_word(at, quad >> 1, g, NG) + (quad & 1);
-        reinterpret_cast<uint16_t*>(base)[half] = (uint16_t)codes;
-        if (quad == 0) reinterpret_cast<__half2*>(base + q4_scales_at(D))[at * NG + g] = __halves2half2(s.d, s.m);
     }
 }
 
@@ -421,7 +448,7 @@ extern "C" int nncpu_qk_norm_rope_append_q4(const void* qkv, int qkv_dt, int ld,
              bt_rows, bt_stride, k_pages, v_pages, n_pages, q_out, q_dt, n, n_heads, n_kv, D, temp_coef, temp_every};
     if ((D == 32 || D == 64 || D == 128) && qkv_dt == DT_F32 && ld % 4 == 0 && (cos_sin == nullptr || half == D / 2) && (uintptr_t)qkv % 16 == 0 &&
         (uintptr_t)q_out % 16 == 0 && (uintptr_t)cos_sin % 16 == 0 && (uintptr_t)q_gamma % 16 == 0 && (uintptr_t)k_gamma % 16 == 0) {
-        const int rounds = (n_heads + 2 * n_kv + 1024 / D - 1) / (1024 / D);      // a block's rounds, were it alone with a token
+        const int rounds = (n_heads + 2 * n_kv + 2048 / D - 1) / (2048 / D);      // a block's rounds, were it alone with a token
         // as many blocks as eight on each SM ask for
         long per = (8L * sm_count() + n - 1) / n;
         per = per < rounds ? per : rounds;

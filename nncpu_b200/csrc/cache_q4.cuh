@@ -14,7 +14,7 @@
 //
 // So that attention_q4.cu reads whole tensor-core operands: in a key row the four lanes of a quad find their words of all groups
 // side by side (16 bytes for D = 128), and two codes 16 bits apart are neighbours along the product's inner dimension (lanes of a
-// key; positions of a value lane), which one mask and one OR turn into two bfloat16 numbers 128 + c.
+// key; positions of a value lane), which one mask and one OR turn into two float16 numbers 1 024 + c.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -49,6 +49,14 @@ __device__ __forceinline__ Q4Scale q4_scale(float lo, float hi) {
 __device__ __forceinline__ uint32_t q4_code(float x, const Q4Scale& s) {
     const float t = rintf(__fmul_rn(__fsub_rn(x, s.m32), s.inv));
     return (uint32_t)fminf(fmaxf(t, 0.0f), 15.0f);      // (a NaN's code is 0)
+}
+// Four neighbours' codes, the first in the lowest four bits (of 16; the others are not said).  Clamped before it is rounded, which
+// gives the same; 1.5 x 2^23 is added, so that the sum's last bits are the rounded number.
+__device__ __forceinline__ uint32_t q4_codes(float x0, float x1, float x2, float x3, const Q4Scale& s) {
+    auto one = [&](float x) {
+        return __float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(__fsub_rn(x, s.m32), s.inv), 0.0f), 15.0f), 12582912.0f));
+    };
+    return ((one(x3) * 16 + one(x2)) * 16 + one(x1)) * 16 + one(x0);
 }
 // x within float16's range; a NaN stays one (fminf and fmaxf would drop it).
 __device__ __forceinline__ float q4_in_range(float x) { return fabsf(x) > kHalfMax ? copysignf(kHalfMax, x) : x; }
