@@ -7,8 +7,12 @@
 // One pass over the logits, which is what bounds it: a thread keeps (maximum, sum, weighted sum) of what it has seen and
 // follows the maximum 16 logits (32 of bfloat16) at a time.  Alternatives ride along: a warp keeps its best 32 as sorted keys
 // (the order of the logit's bits above the complement of the index), one a lane, and a bar that a logit must reach to be
-// looked at, the k-th best of what any warp of the block has seen or less.  The first bar is the least of what the warps offer, each the
-// ceil(k / warps)-th largest of its lanes' first maxima: at least k logits reach that, and few more.  Those that that do gather in shared memory and are sorted into the list 32 at a time.
+// looked at: the k-th best of what any warp of the block has sorted, or the least of what the warps offer now and then, each the
+// ceil(k / warps)-th largest of its lanes' maxima so far, whichever is higher.  At least k logits reach either, and few more.  Those
+// that do gather in shared memory and are sorted into the list 32 at a time.
+// (300 rows of 50 257, three sets of them in turn: without alternatives 16.7 us, one 23.5, 20 25.9; 14 instructions a logit and some ten
+// more with alternatives fill half of the issue slots.  With offers at the first turn alone 25.7 and 29.8; one list a block 52.  64
+// rows of 151 936: 12.1 and, with 20, 19.6.  1 001 rows of those: 100, bytes, 608 MB at 6 080 GB/s.)
 // Where there are few rows several blocks, a cluster, share one, each a stretch of it, and meet in distributed shared memory.
 
 #include <math.h>
@@ -33,6 +37,7 @@ constexpr int kMaxTop = 32;
 constexpr int kMaxSplits = 16;      // blocks of a cluster
 constexpr int kVectors = 4;         // 16-byte vectors of a thread's turn
 constexpr int kStages = 3;          // turns in flight
+constexpr int kBelow = (int)0x80000000;      // a bar below everything
 constexpr int kRing = kStages * kVectors * kThreads * 16;
 typedef unsigned long long Key;
 
@@ -116,7 +121,8 @@ __global__ void __launch_bounds__(kThreads, 4) rows_kernel(const Rows p, int spl
     __shared__ Key lists[TOP ? kWarps : 1][32];
     __shared__ Sums sums[kWarps];
     __shared__ Sums whole;
-    __shared__ int bar_bits, first_bar;          // the bar, as an integer of the same order; the least of the warps' offers
+    __shared__ int bar_bits;                     // the bar, as an integer of the same order
+    __shared__ int offers[kWarps];               // a logit that ceil(k / kWarps) lanes of a warp have reached, as such integers
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const size_t row = blockIdx.x / splits;
     const int split = blockIdx.x % splits;
@@ -127,17 +133,15 @@ __global__ void __launch_bounds__(kThreads, 4) rows_kernel(const Rows p, int spl
     const int n_vec = (p.vocab + shift + E - 1) / E;
     const int v0 = (int)((long)n_vec * split / splits), v1 = (int)((long)n_vec * (split + 1) / splits);
     if (TOP) {
-        if (tid == 0) {
-            bar_bits = 0x80000000;               // below everything
-            first_bar = 0x7FFFFFFF;
-        }
+        if (tid == 0) bar_bits = kBelow;
+        if (lane == 0) offers[warp] = kBelow;
         __syncthreads();
     }
     Sums mine{-INFINITY, 0.0f, 0.0f};
     Key list = 0;                                // this lane's of the warp's best 32
     Key last = 0;                                // the k-th of them
     int n_waiting = 0;
-    bool first = true;
+    unsigned turn_number = 0;
     auto settle = [&]() {                        // sorts what waits into the list
         __syncwarp();
         Key got = lane < n_waiting ? waiting[warp][lane] : 0;
@@ -216,25 +220,30 @@ __global__ void __launch_bounds__(kThreads, 4) rows_kernel(const Rows p, int spl
             mine.e += e;
         }
         if (TOP) {
-            if (first) {
-                first = false;
-                float mine_of_all = mx, offer = warp_max(mx);
+            // At turns 0, 1, 2, 4, 8, ... : k logits or more reach what every warp offers, since each has that many lanes whose own maximum
+            // does.  (What another warp has not written yet is less, and as good a bar.)
+            if ((turn_number & (turn_number - 1)) == 0) {
+                int reach = ordered(mine.m), offer = __reduce_max_sync(0xffffffffu, reach);
                 for (int k = kWarps; k < p.k; k += kWarps) {
-                    const unsigned has = __ballot_sync(0xffffffffu, mine_of_all == offer);
-                    if (lane == __ffs(has) - 1) mine_of_all = -INFINITY;
-                    offer = warp_max(mine_of_all);
+                    const unsigned has = __ballot_sync(0xffffffffu, reach == offer);
+                    if (lane == __ffs(has) - 1) reach = kBelow;
+                    offer = __reduce_max_sync(0xffffffffu, reach);
                 }
-                if (lane == 0) atomicMin(&first_bar, ordered(offer));
-                __syncthreads();
-                if (lane == 0) atomicMax(&bar_bits, first_bar);
+                volatile int* o = offers;
+                if (lane == 0) o[warp] = offer;
+                if (turn_number == 0) __syncthreads();
+                else __syncwarp();
+                offer = __reduce_min_sync(0xffffffffu, o[lane % kWarps]);
+                if (lane == 0) atomicMax(&bar_bits, offer);
                 __syncwarp();
             }
+            ++turn_number;
             const int bits = *reinterpret_cast<volatile int*>(&bar_bits);
-            const float bar = bits == (int)0x80000000 ? -INFINITY : logit_of((Key)((uint32_t)bits ^ 0x80000000u) << 32);
+            const float bar = bits == kBelow ? -INFINITY : logit_of((Key)((uint32_t)bits ^ 0x80000000u) << 32);
             unsigned pass = 0;
             if (__any_sync(0xffffffffu, mx >= bar))
 #pragma unroll
-                for (int j = 0; j < kVectors * E; ++j) pass |= (x[j] >= bar || bar == -INFINITY ? 1u : 0u) << j;
+                for (int j = 0; j < kVectors * E; ++j) pass |= (x[j] < bar ? 0u : 1u) << j;        // (a NaN passes, as -inf)
             while (__any_sync(0xffffffffu, pass != 0)) {
                 const int j = __ffs(pass) - 1;           // one of each lane's at a time
                 const int at = v + j / E * kThreads + tid, i = at * E - shift + j % E;
@@ -324,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 4) rows_kernel(const Rows p, int spl
 
 // Blocks that share a row.  Few rows: as many as give the device's SMs two blocks each (8 rows of 151 936, best 5: 1 block 33 us, 4 16.5,
 // 8 or 16 12.4).  A few hundred: one, because a cluster's own cost is that of some 10 000 logits (300 rows of 50 257, best 20: 1
-// block 30.8 us, 2 31.5, 4 36.4).  Many long rows: two, which end together more nearly (1 001 rows of 151 936: 1 block 102 us, 2 98.8, 4 107).
+// block 25.9 us, 2 28.6, 4 34.1).  Many long rows: two, which end together more nearly (1 001 rows of 151 936: 1 block 102 us, 2 98.8, 4 107).
 static int splits_of(int n, int vocab) {
     if (n >= 5L * sm_count()) return vocab >= 1 << 16 ? 2 : 1;
     int s = 1;
