@@ -10,6 +10,9 @@ GFLOP/s for its row kernels and one attention block.
     python -m nncpu_b200.kernels.microbench attention-f32 SEQUENCES TOKENS [--past KEYS]
     python -m nncpu_b200.kernels.microbench attention-decode BATCH CONTEXT [--splits S] [--cluster] [--from-projections]
     python -m nncpu_b200.kernels.microbench attention-prefill BATCH TOKENS [--past KEYS] [--capacity KEYS] [--cap C]
+    python -m nncpu_b200.kernels.microbench append-q4 BATCH TOKENS [--past KEYS]
+    python -m nncpu_b200.kernels.microbench attention-q4 BATCH TOKENS [--past KEYS] [--float32]
+    python -m nncpu_b200.kernels.microbench logprobs ROWS VOCAB [--top K]
     python -m nncpu_b200.kernels.microbench qk-conv BATCH TOKENS [--taps 4]
     python -m nncpu_b200.kernels.microbench rmsnorm ROWS DIM
     python -m nncpu_b200.kernels.microbench gla BATCH TOKENS [--columns 2|4]
@@ -241,6 +244,72 @@ def attention_prefill(args) -> None:
     print(f"attention-prefill batch={b} tokens={t}{f' past={args.past}' if args.past else ''}{f' cap={args.cap:g}' if args.cap else ''}: {ms * 1e3:.1f} us, {flops / ms / 1e9:.0f} TFLOP/s (causal)")
 
 
+def _cache_q4(batch, ctx, nkv, hd, copies):
+    """Caches of 4 bits that hold normal numbers, appended by the kernel itself."""
+    pages = batch * ((ctx + 63) // 64)
+    table = torch.randperm(pages, device=DEV).to(torch.int32).view(batch, -1)
+    pos = torch.arange(ctx, dtype=torch.int32, device=DEV)
+    sets = []
+    for _ in range(copies):
+        kp, vp = (torch.zeros(pages, nkv, ops.q4_page_bytes(hd), dtype=torch.uint8, device=DEV) for _ in range(2))
+        for b in range(batch):
+            qkv = torch.randn(ctx, 3 * nkv * hd, device=DEV)
+            ops.qk_norm_rope_append_q4(qkv, None, None, 1e-6, None, torch.full_like(pos, b), pos, table, kp, vp,
+                                       torch.empty(ctx, nkv * hd, device=DEV), nkv, nkv, hd)
+        sets.append((kp, vp))
+    return sets, table
+
+
+def append_q4(args) -> None:
+    """Per-head norm, rotation and append to a cache of 4 bits, from float32 projections."""
+    nh, nkv, hd, b, t, past = args.heads, args.kv_heads, args.head_dim, args.batch, args.tokens, args.past
+    copies = max(2, min(64, 2 * L2_BYTES // (b * t * (nh + 2 * nkv) * hd * 4) + 1))
+    ((kp, vp),), table = _cache_q4(b, past + t, nkv, hd, 1)
+    seq = torch.arange(b, dtype=torch.int32, device=DEV).repeat_interleave(t)
+    pos = torch.arange(past, past + t, dtype=torch.int32, device=DEV).repeat(b)
+    gamma = torch.ones(hd, device=DEV).bfloat16()
+    angle = pos[:, None] * torch.pow(1e6, -2.0 * torch.arange(hd // 2, device=DEV) / hd)
+    cs = torch.stack((angle.cos(), angle.sin()), -1).contiguous()
+    qkvs = [torch.randn(b * t, (nh + 2 * nkv) * hd, device=DEV) for _ in range(copies)]
+    q = torch.empty(b * t, nh * hd, dtype=torch.bfloat16, device=DEV)
+    ms = _time([lambda x=x: ops.qk_norm_rope_append_q4(x, gamma, gamma, 1e-6, cs, seq, pos, table, kp, vp, q, nh, nkv, hd) for x in qkvs],
+               args.once)
+    moved = b * t * ((nh + 2 * nkv) * hd * 4 + hd * 4 + nh * hd * 2 + 2 * nkv * hd * 5 // 8)
+    print(f"append-q4 batch={b} tokens={t} past={past}: {ms * 1e3:.1f} us, {moved / ms / 1e6:.0f} GB/s")
+
+
+def attention_q4(args) -> None:
+    """Attention over a cache of 4 bits of sequences that bring `tokens` tokens each behind `past` keys, as a step calls it."""
+    nh, nkv, hd, b, t, ctx = args.heads, args.kv_heads, args.head_dim, args.batch, args.tokens, args.past + args.tokens
+    kv_bytes = 2 * b * ctx * nkv * hd * 5 // 8
+    sets, table = _cache_q4(b, ctx, nkv, hd, max(2, min(32, 2 * L2_BYTES // kv_bytes + 1)))
+    seq = torch.arange(b, dtype=torch.int32, device=DEV).repeat_interleave(t)
+    pos = torch.arange(args.past, ctx, dtype=torch.int32, device=DEV).repeat(b)
+    cu = torch.arange(b + 1, dtype=torch.int32, device=DEV) * t
+    q = torch.randn(b * t, nh * hd, device=DEV).to(torch.float32 if args.float32 else torch.bfloat16)
+    out, status = torch.empty_like(q), torch.zeros(1, dtype=torch.int32, device=DEV)
+    if t == 1:
+        run = lambda kp, vp: ops.attention_q4(q, kp, vp, table, seq, pos, out, nh, nkv, hd, hd ** -0.5, longest=ctx)
+    else:
+        run = lambda kp, vp: ops.attention_q4_prompt(q, kp, vp, table, cu, seq, pos, out, b, nh, nkv, hd, hd ** -0.5, ctx, status)
+    ms = _time([lambda kp=kp, vp=vp: run(kp, vp) for kp, vp in sets], args.once)
+    if int(status.item()):
+        raise SystemExit(f"the kernel gave up waiting (status {int(status.item())})")
+    flops = 4.0 * nh * hd * b * t * (args.past + (t + 1) / 2)
+    print(f"attention-q4 batch={b} tokens={t} past={args.past}{' float32' if args.float32 else ''}: {ms * 1e3:.1f} us, "
+          f"{kv_bytes / ms / 1e6:.0f} GB/s of cache, {flops / ms / 1e9:.1f} TFLOP/s")
+
+
+def logprobs(args) -> None:
+    n, vocab, k = args.rows, args.vocab, args.top
+    xs = [2 * torch.randn(n, vocab, device=DEV) for _ in range(max(2, min(64, 2 * L2_BYTES // (n * vocab * 4) + 1)))]
+    targets = torch.randint(0, vocab, (n,), dtype=torch.int32, device=DEV)
+    lp, entropy = torch.empty(n, device=DEV), torch.empty(n, device=DEV)
+    top, ids = (torch.empty(n, k, device=DEV), torch.empty(n, k, dtype=torch.int32, device=DEV)) if k else (None, None)
+    ms = _time([lambda x=x: ops.token_logprobs(x, targets, lp, entropy, top, ids) for x in xs], args.once)
+    print(f"logprobs rows={n} vocab={vocab}{f' top={k}' if k else ''}: {ms * 1e3:.1f} us, {n * vocab * 4 / ms / 1e6:.0f} GB/s")
+
+
 def qk_conv(args) -> None:
     """The stage between the q/k product and the attention of a layer with short convolutions: convolution, per-head norm,
     rotation of half a head's lanes, queries, keys and values to their places, the state left advanced."""
@@ -409,6 +478,17 @@ def main(argv=None) -> int:
     p.add_argument("--heads", type=int, default=16); p.add_argument("--kv-heads", type=int, default=4)
     p.add_argument("--head-dim", type=int, default=128)
     p.set_defaults(fn=attention_f32)
+    for name, fn in (("append-q4", append_q4), ("attention-q4", attention_q4)):
+        p = sub.add_parser(name)
+        p.add_argument("batch", type=int); p.add_argument("tokens", type=int); p.add_argument("--past", type=int, default=0)
+        p.add_argument("--heads", type=int, default=32); p.add_argument("--kv-heads", type=int, default=8)
+        p.add_argument("--head-dim", type=int, default=128)
+        if fn is attention_q4:
+            p.add_argument("--float32", action="store_true", help="queries and result in 32 bits")
+        p.set_defaults(fn=fn)
+    p = sub.add_parser("logprobs")
+    p.add_argument("rows", type=int); p.add_argument("vocab", type=int); p.add_argument("--top", type=int, default=0)
+    p.set_defaults(fn=logprobs)
     p = sub.add_parser("rmsnorm")
     p.add_argument("rows", type=int); p.add_argument("dim", type=int)
     p.set_defaults(fn=rmsnorm)
