@@ -79,6 +79,10 @@ __device__ __forceinline__ float closing_factor(const AttnQ4& p, int t, int h, f
 // the others every block leaves its part (its first and its last pair at most) in scratch for stream_merge_kernel.  Where there are few
 // pairs of not too many pages (CLUSTER), a cluster of blocks shares each of them instead, and its parts meet in distributed
 // shared memory: one launch, and no way through global memory.
+//
+// Bound by instructions where there is much to read (some 300 a warp for 16 keys, a little over half of the issue slots): 64 sequences of up to
+// 8 000 keys, 32 heads over 8 of 128 lanes, 70 us for 328 MB (4 700 GB/s); 64 of 4 000 each 73 us where bfloat16 takes 154.  One
+// sequence of 2 500 keys takes 9.7 us, launch and latency.
 // ---------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kStreamWarps = 2;
@@ -819,8 +823,8 @@ __device__ __forceinline__ int2 split_pages(int n_walk, int n_splits, int s) {
 
 // A page at a time: keys as numbers to shared memory; scores, a thread a key and half of the heads; weights against the running
 // maximum, a warp a head; values to shared memory; outputs, a thread a lane (two of heads of more than 128) and, of heads of 32 and 64 lanes,
-// a part of the keys.  Bound by the latency of that chain (four sequences of up to 1 000 keys, 16 heads over 4 of 64 lanes: 14 us of which
-// the bytes are worth 0.2), so a split is a page where there are blocks to spare.
+// a part of the keys.  Bound by the latency of that chain (four sequences of up to 1 000 keys, 16 heads over 4 of 64 lanes: 11 us of which
+// the bytes are worth 0.2; 25 with several pages a split), so a split is a page where there are blocks to spare.
 template <int HEADS>
 __global__ void __launch_bounds__(kAnyThreads) any_kernel(const AttnQ4 p) {
     extern __shared__ __align__(16) float any_smem[];

@@ -333,6 +333,8 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             // K tiles are free again once their scores are computed, V tiles once O has been updated, so the two
             // rings advance on their own: one thread polls both without blocking on either
             int jk = 0, jv = 0;
+            // (kHalf: the table has the pages that the call was told of; keys beyond them are the last page's)
+            auto page_at = [&](int i) { return table[kHalf ? min(walk.page(i), p.bt_stride - 1) : walk.page(i)]; };
             bool ok = true;
             unsigned long long t0 = global_ns();
             while (jk < n_steps || jv < n_steps) {
@@ -344,7 +346,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                     for (int pg = 0; pg < pages; ++pg)
                         for (int s = 0; s < kSlabs; ++s)
                             tma_load_4d(smem_k + st * kKBytes + s * kKvSlab + pg * (kPage * 128), &map_k, &k_full[st],
-                                        64 * s, 0, kvh, table[kHalf ? min(walk.page(2 * (s0 + jk) + pg), p.bt_stride - 1) : walk.page(2 * (s0 + jk) + pg)]);
+                                        64 * s, 0, kvh, page_at(2 * (s0 + jk) + pg));
                     ++jk;
                     moved = true;
                 }
@@ -355,7 +357,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                     for (int pg = 0; pg < pages; ++pg)
                         for (int s = 0; s < kVSlabs; ++s)
                             tma_load_4d(smem_v + st * kVBytes + s * kKvSlab + pg * (kPage * 128), &map_v, &v_full[st],
-                                        64 * s, 0, kvh, table[kHalf ? min(walk.page(2 * (s0 + jv) + pg), p.bt_stride - 1) : walk.page(2 * (s0 + jv) + pg)]);
+                                        64 * s, 0, kvh, page_at(2 * (s0 + jv) + pg));
                     ++jv;
                     moved = true;
                 }

@@ -81,7 +81,8 @@ __device__ __forceinline__ void norm_rotate(F (&x)[NG], const void* gamma, int g
     }
 }
 
-// A warp per (token, head of q, k or v).
+// A warp per (token, head of q, k or v): any sizes, types and strides.  Bound by instructions, its lanes' exchanges among them (2 048
+// tokens of 32 heads over 8 of 128 lanes with what is read back took 57 us; append_fast_kernel takes what models commonly have).
 template <int NG>
 __global__ void __launch_bounds__(256) append_kernel(const Append a) {
     constexpr int D = 32 * NG;
@@ -295,7 +296,8 @@ __global__ void __launch_bounds__(256, 4) append_fast_kernel(const Append a) {
     }
 }
 
-// What the cache holds of given tokens: a thread takes eight neighbouring lanes of a key and of a value.
+// What the cache holds of given tokens: a thread takes eight neighbouring lanes of a key and of a value.  (2 048 tokens of 8 heads of 128
+// lanes to bfloat16: 6 us for 11 MB, most of it the latency of three loads one after another and the launch.)
 __device__ __forceinline__ void put8(void* out, long i, int dt, const float (&x)[8]) {
     if (dt == DT_F32) {
         reinterpret_cast<float4*>(out)[2 * i] = make_float4(x[0], x[1], x[2], x[3]);
@@ -343,7 +345,9 @@ __global__ void __launch_bounds__(256) read_kernel(const uint8_t* k_pages, const
 // The pages that a step's tokens see, as numbers in pages of their own: float16 or float32 rows of `lanes` >= D lanes, zeros behind a
 // head's own and in rows behind the sequence's end (whatever the cache holds there).  Page i of sequence b goes to page b * width + i,
 // and the table for the attention kernels is written too.  A block takes a page of keys or of values of one head, a thread eight
-// neighbouring lanes of a row at a time: grid = (width, 2 n_kv, n_seqs).
+// neighbouring lanes of a row at a time: grid = (width, 2 n_kv, n_seqs).  (2 048 positions of 8 heads of 128 lanes to float16: 5.5 us
+// for 2.6 MB read and 8.4 written; the attention over them takes 48.  To take the codes out inside the attention kernel would do it
+// again for every tile of queries: 16 times here.)
 struct Expand {
     const uint8_t* k_pages;
     const uint8_t* v_pages;
