@@ -162,19 +162,22 @@ __global__ void __launch_bounds__(256) append_kernel(const Append a) {
 // of two and three blocks an SM.  Their bytes alone would take 12.1 us.
 // ---------------------------------------------------------------------------
 template <int D, typename F>
-__device__ __forceinline__ void norm_rotate8(F (&x)[8], const float4* gamma, const float2 (&cs)[4], bool rotated, F eps) {
+__device__ __forceinline__ void norm_rotate8(F (&x)[8], const float4* gamma, const float2 (&cs)[4], bool rotated, F eps, F times) {
     constexpr int T = D / 8;
+    F r = times;
     if (gamma != nullptr) {
         F s = ((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])) + ((x[4] * x[4] + x[5] * x[5]) + (x[6] * x[6] + x[7] * x[7]));
 #pragma unroll
         for (int o = T / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        F r;
-        if constexpr (sizeof(F) == 8) r = rsqrt(s / F(D) + eps);
-        else r = rsqrtf(s * (1.0f / D) + eps);
+        if constexpr (sizeof(F) == 8) r = rsqrt(s * (F(1) / D) + eps);
+        else r = rsqrtf(s * (1.0f / D) + eps) * times;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             x[4 * i] *= r * F(gamma[i].x); x[4 * i + 1] *= r * F(gamma[i].y); x[4 * i + 2] *= r * F(gamma[i].z); x[4 * i + 3] *= r * F(gamma[i].w);
         }
+    } else if (sizeof(F) == 4) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= r;
     }
     if (rotated) {
 #pragma unroll
@@ -184,6 +187,17 @@ __device__ __forceinline__ void norm_rotate8(F (&x)[8], const float4* gamma, con
             x[e + 4] = b * F(cs[e].x) + a * F(cs[e].y);
         }
     }
+}
+
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+    float m;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
 }
 
 template <int D>
@@ -230,12 +244,12 @@ __global__ void __launch_bounds__(256, 4) append_fast_kernel(const Append a) {
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = x[e];
-            norm_rotate8<D, float>(y, a.q_gamma != nullptr ? gamma : nullptr, cs, rotated, (float)a.eps);
+            norm_rotate8<D, float>(y, a.q_gamma != nullptr ? gamma : nullptr, cs, rotated, (float)a.eps, times);
             if (there && is_q) {
                 const size_t to = ((size_t)t * a.n_heads + h) * D + 4 * j;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float4 z = make_float4(y[4 * i] * times, y[4 * i + 1] * times, y[4 * i + 2] * times, y[4 * i + 3] * times);
+                    const float4 z = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
                     if (a.q_dt == DT_F32) {
                         *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.q_out) + to + i * (D / 2)) = z;
                     } else {
@@ -254,37 +268,43 @@ __global__ void __launch_bounds__(256, 4) append_fast_kernel(const Append a) {
             double y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = x[e];
-            norm_rotate8<D, double>(y, a.k_gamma != nullptr ? gamma : nullptr, cs, rotated, a.eps);
+            norm_rotate8<D, double>(y, a.k_gamma != nullptr ? gamma : nullptr, cs, rotated, a.eps, 1.0);
             if (!is_v)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = (float)y[e];
         }
-        bool bad[2] = {};
-        float lo[2] = {kHalfMax, kHalfMax}, hi[2] = {-kHalfMax, -kHalfMax};
+        // A NaN stays in lo and hi.  (Limits of what is limited are limits of the limits: the lanes themselves only where one passes.)
+        float lo[2], hi[2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            x[e] = q4_in_range(x[e]);
-            bad[e / 4] |= x[e] != x[e];
-            lo[e / 4] = fminf(lo[e / 4], x[e]);
-            hi[e / 4] = fmaxf(hi[e / 4], x[e]);
+        for (int i = 0; i < 2; ++i) {
+            lo[i] = min_or_nan(min_or_nan(x[4 * i], x[4 * i + 1]), min_or_nan(x[4 * i + 2], x[4 * i + 3]));
+            hi[i] = max_or_nan(max_or_nan(x[4 * i], x[4 * i + 1]), max_or_nan(x[4 * i + 2], x[4 * i + 3]));
         }
         if (D == 32) {          // (both halves are of one group, of four threads)
-            bad[0] = bad[1] = bad[0] | bad[1];
-            lo[0] = lo[1] = fminf(lo[0], lo[1]);
-            hi[0] = hi[1] = fmaxf(hi[0], hi[1]);
+            lo[0] = lo[1] = min_or_nan(lo[0], lo[1]);
+            hi[0] = hi[1] = max_or_nan(hi[0], hi[1]);
+        }
+        constexpr int kThreads = D == 32 ? 4 : 8;       // of a group
+#pragma unroll
+        for (int o = kThreads / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                lo[i] = min_or_nan(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
+                hi[i] = max_or_nan(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
+            }
+        if (fminf(lo[0], lo[1]) < -kHalfMax || fmaxf(hi[0], hi[1]) > kHalfMax) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = q4_in_range(x[e]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                lo[i] = q4_in_range(lo[i]);
+                hi[i] = q4_in_range(hi[i]);
+            }
         }
         const int kvh = h - a.n_heads - (is_v ? a.n_kv : 0), quad = j & 7;
         uint8_t* base = (is_v ? a.v_pages : a.k_pages) + ((size_t)max(page, 0) * a.n_kv + kvh) * q4_page_bytes(D);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            constexpr int kThreads = D == 32 ? 4 : 8;       // of a group
-#pragma unroll
-            for (int o = kThreads / 2; o > 0; o >>= 1) {
-                lo[i] = fminf(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
-                hi[i] = fmaxf(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
-            }
-            const unsigned any_bad = __ballot_sync(0xffffffffu, bad[i]);
-            if (any_bad >> (threadIdx.x & 31 & ~(kThreads - 1)) & ((1u << kThreads) - 1)) lo[i] = hi[i] = __int_as_float(0x7FC00000);
             const Q4Scale s = q4_scale(lo[i], hi[i]);
             const uint16_t codes = (uint16_t)q4_codes(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], s);
             if (!there || is_q || page < 0) continue;
