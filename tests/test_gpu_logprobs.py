@@ -155,3 +155,22 @@ def test_on_another_stream_and_twice_the_same_bits():
         got = run(x, t, 9)
     s.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_rows_behind_two_to_the_31_logits():
+    n, vocab = 32800, 65536
+    logits = torch.zeros(n, vocab, dtype=torch.bfloat16, device=DEV)
+    logits[-3:] = torch.randn(3, vocab, generator=torch.Generator().manual_seed(0)).to(DEV)
+    targets = torch.arange(n, dtype=torch.int32, device=DEV)
+
+    def ask(x, t):
+        lp, entropy, top, ids = (torch.empty(len(x), *s, device=DEV, dtype=d) for s, d in (((), torch.float32), ((), torch.float32),
+                                                                                           ((4,), torch.float32), ((4,), torch.int32)))
+        ops.token_logprobs(x, t, lp, entropy, top, ids)
+        return lp, entropy, top, ids
+    got = ask(logits, targets)
+    few = ask(logits[-3:].clone(), targets[-3:].clone())
+    assert torch.equal(got[3][-3:], few[3]) and (got[3][:-3] == torch.arange(4, device=DEV)).all()
+    for a, b in zip(got[:3], few[:3]):       # (the few rows are shared by clusters: another order of 32-bit sums of 65 536 terms)
+        assert torch.allclose(a[-3:], b, rtol=0, atol=1e-5)
+    assert torch.allclose(got[0][:-3].double(), torch.tensor(-np.log(vocab)).double().to(DEV), rtol=0, atol=1e-5)

@@ -462,3 +462,31 @@ def test_scratch_that_starts_off_its_boundary_is_refused():
                     torch.empty(need, dtype=torch.int8, device=DEV)):
         with pytest.raises(Exception, match="scratch"):
             ops.attention_q4_prompt(q, kp, vp, table, cu, ts, tp, torch.empty_like(q), 2, 8, 2, 128, 0.1, 700, status, scratch=scratch)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_pages_behind_four_gigabytes(dt):
+    """The same pages at the end of a cache of more than 2^32 bytes: the same bits."""
+    kv, D, lens = 8, 128, [300, 64, 1]
+    kp, vp, table, _, _ = Q.filled_cache(lens, kv, D, 4)
+    first = (1 << 32) // (kv * 40 * D) + 50
+    small = Q.as_cuda(kp, vp, table)
+    big = [torch.empty(first + len(kp), kv, 40 * D, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    for b, s in zip(big, small):
+        b[first:] = s
+    seq, pos, cu = places([200, 64, 1], [100, 0, 0])
+    ts, tp, cud, every, last = Q.as_cuda(seq, pos, cu, np.arange(3, dtype=np.int32), np.array(lens, np.int32) - 1)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    qkv, q = rand(3, 48 * 128, seed=1).to(DEV), rand(len(seq), 32 * 128, seed=2).to(dt).to(DEV)
+
+    def results(k, v, bt):
+        token, prompt, held = torch.zeros(3, 32 * 128, dtype=dt, device=DEV), torch.zeros_like(q), torch.zeros(len(seq), kv * D, device=DEV)
+        new_q = torch.empty_like(token)
+        ops.qk_norm_rope_append_q4(qkv, None, None, 1e-6, None, every, last, bt, k, v, new_q, 32, kv, D)
+        ops.attention_q4(new_q, k, v, bt, every, last, token, 32, kv, D, 0.1)
+        ops.attention_q4_prompt(q, k, v, bt, cud, ts, tp, prompt, 3, 32, kv, D, 0.1, 300, status)
+        ops.q4_read(k, v, bt, ts, tp, held, torch.empty_like(held))
+        return token, prompt, held
+    want = results(*small)
+    got = results(*big, torch.where(small[2] < 0, small[2], small[2] + first))
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and (want[2] != 0).any()
