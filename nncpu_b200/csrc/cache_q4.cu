@@ -402,8 +402,7 @@ constexpr int kExpandThreads = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const Expand p) {
-    wait_for_previous_kernels();       // (before anything is read: the kernel after this one reads the step's metadata before it waits)
-    let_next_kernel_start();
+    let_next_kernel_start();           // (which reads the step's metadata before it waits for this one)
     const int pi = blockIdx.x, b = blockIdx.z, row = b * gridDim.x + pi;
     const bool values = blockIdx.y >= p.n_kv;
     const int h = values ? blockIdx.y - p.n_kv : blockIdx.y;
@@ -541,14 +540,11 @@ extern "C" int nncpu_q4_expand(const uint8_t* k_pages, const uint8_t* v_pages, i
     }
     const Expand p{k_pages, v_pages, n_pages, block_table, bt_stride, cu_seqlens, tok_seq, tok_pos, k_out, v_out, table, places,
                    n_tok, n_kv, D, lanes, window, keep};
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)width, (unsigned)(2 * n_kv), (unsigned)n_seqs);
-    cfg.blockDim = dim3(kExpandThreads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    cfg.attrs = attr;
-    cfg.numAttrs = overlap_attribute(attr);
-    const cudaError_t e = half ? cudaLaunchKernelEx(&cfg, expand_kernel<__half>, p) : cudaLaunchKernelEx(&cfg, expand_kernel<float>, p);
-    NN_CHECK(e == cudaSuccess, "q4_expand: launch failed: %s", cudaGetErrorString(e));
+    // Not launched to start under the kernel before it: its blocks would wait in places that blocks of that one could take (a prompt of
+    // 2 048 tokens with its append 83.6 us instead of 80.2).
+    const dim3 grid((unsigned)width, (unsigned)(2 * n_kv), (unsigned)n_seqs);
+    if (half) expand_kernel<__half><<<grid, kExpandThreads, 0, stream>>>(p);
+    else expand_kernel<float><<<grid, kExpandThreads, 0, stream>>>(p);
+    NN_LAUNCH_OK("q4_expand");
     return 0;
 }
