@@ -1813,8 +1813,8 @@ def attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_head
 
 
 # A portion of one sequence attends straight from the codes, as many of its tokens at a time as have columns on the tensor cores, while
-# its tokens are at most so many (32 heads over 8, us, straight / taken out first: 8 behind 3 000 19 / 33, 24 behind 700 17 / 21, 24 behind
-# 3 000 23 / 34, 48 behind 1 500 27.6 / 28.2, 64 behind 3 000 36.7 / 35.3).  Longer ones, and several sequences, have their keys and values taken out of the codes once, for
+# its tokens are at most so many and its keys more than two pages (32 heads over 8, us, straight / taken out first: 8 behind 3 000 22 / 30, 24
+# behind 700 17 / 21, 24 behind 3 000 24 / 31, 48 behind 1 500 24.5 / 25.7, 64 behind 3 000 35.9 / 32.9; 24 behind none 15.6 / 11.5).  Longer ones, and several sequences, have their keys and values taken out of the codes once, for
 # all query tiles and heads: float16 for the tcgen05 kernel, float32 for the 32-bit one; so many positions at a time (of whole sequences,
 # one at least).
 Q4_FEW_TOKENS = 48
@@ -1828,7 +1828,7 @@ def _q4_prompt_plan(n: int, n_seqs: int, n_heads: int, n_kv: int, head_dim: int,
     sequences at a time; bytes of keys; of keys, values, table and (float32) the tokens' sequences and positions; of all)."""
     width = (longest + 63) // 64
     lanes = 0
-    if n <= n_seqs or (bf16 and n_seqs == 1 and n <= Q4_FEW_TOKENS and head_dim <= 128):
+    if n <= n_seqs or (bf16 and n_seqs == 1 and n <= Q4_FEW_TOKENS and longest > 128 and head_dim <= 128):
         pass
     elif bf16:
         lanes = 0 if slope_and_cap else 64 if head_dim <= 64 else 128 if head_dim <= 128 else 0
