@@ -1,8 +1,9 @@
 // Causal attention over the 4-bit cache (cache_q4.cuh says how its pages lie), token by token: every token of the step attends to
 // the pages of its sequence up to its own position (crates/nncpu/src/model/forward.rs:383-426).
 //
-//   stream_kernel: bfloat16 queries, heads of up to 128 lanes, on the tensor cores, straight from the codes (see there).
-//   any_kernel: any type of queries, any whole number of 32-lane groups; 32-bit arithmetic on numbers taken out of the pages.
+//   stream_kernel: bfloat16 queries, heads of up to 128 lanes, score caps of up to 4 096, on the tensor cores, straight from the codes
+//     (see there).
+//   any_kernel: any type of queries, any whole number of 32-lane groups, any cap; 32-bit arithmetic on numbers taken out of the pages.
 //     A block takes one token, up to eight query heads of one key/value head and a split of their pages.
 // Parts of a token's keys meet in a second kernel, in the order of the keys.
 
@@ -1026,8 +1027,10 @@ static bool sizes_ok(int n, int n_heads, int n_kv, int D) {
     return n >= 0 && n_heads > 0 && n_kv > 0 && n_heads % n_kv == 0 && D >= 32 && D <= 256 && D % 32 == 0;
 }
 
-// Whether the tensor-core kernel takes these sizes.
-static bool streams(int dt, int D) { return dt == DT_BF16 && D <= 128; }
+// Whether the tensor-core kernel takes these sizes.  It has a capped score as a difference of two numbers of the cap's size: an error of
+// some 1e-7 of the cap in the exponent, which beyond this one would show (a hundredth at 65 536, a tenth at 10^6).
+constexpr float kMaxStreamCap = 4096.0f;
+static bool streams(int dt, int D, float cap) { return dt == DT_BF16 && D <= 128 && cap <= kMaxStreamCap; }
 
 // Blocks of a token's pages' row, all of which run at once, and how the heads of a key/value head are dealt with.
 constexpr int kStreamMinPlaces = 4;
@@ -1107,9 +1110,9 @@ static int cluster_of(long pairs, int longest, int D, int tiles) {
 }
 
 // Floats of scratch for a call of these sizes, `longest` the most keys that a token may see.
-extern "C" long nncpu_attention_q4_scratch(int n, int n_heads, int n_kv, int D, int dt, int longest) {
+extern "C" long nncpu_attention_q4_scratch(int n, int n_heads, int n_kv, int D, int dt, int longest, float cap) {
     if (n <= 0 || !sizes_ok(n, n_heads, n_kv, D)) return 0;
-    if (streams(dt, D)) {
+    if (streams(dt, D, cap)) {
         // (enough for one column tile and for two, and for parts token by token)
         const int group = n_heads / n_kv, chunks = (group + 7) / 8;
         const long one = 8L * stream_blocks(D, 1), two = 16L * stream_blocks(D, 2);
@@ -1119,7 +1122,7 @@ extern "C" long nncpu_attention_q4_scratch(int n, int n_heads, int n_kv, int D, 
     return s > 1 ? (long)n * n_heads * s * (D + 2) : 0;
 }
 
-// one_seq (bfloat16, at most 128 lanes): the tokens are those of ONE sequence, at consecutive positions, from one_seq[0] to before
+// one_seq (what the tensor-core kernel takes; the other one leaves it aside): the tokens are those of ONE sequence, at consecutive positions, from one_seq[0] to before
 // one_seq[1] of the n; several of them then go through the pages together.
 extern "C" int nncpu_attention_q4(const void* q, int dt, const uint8_t* k_pages, const uint8_t* v_pages, int n_pages,
                                   const int* block_table, int bt_rows, int bt_stride, const int* tok_seq, const int* tok_pos, void* out, float* part,
@@ -1131,13 +1134,13 @@ extern "C" int nncpu_attention_q4(const void* q, int dt, const uint8_t* k_pages,
              "attention_q4: cap %f, %d kept keys, gate rows of %d", cap, keep, gate_ld);
     NN_CHECK(bt_rows > 0 && bt_stride > 0 && n_pages > 0 && longest > 0, "attention_q4: %d pages, %d tables of %d, at most %d keys", n_pages, bt_rows,
              bt_stride, longest);
-    const long need = nncpu_attention_q4_scratch(n, n_heads, n_kv, D, dt, longest);
+    const long need = nncpu_attention_q4_scratch(n, n_heads, n_kv, D, dt, longest, cap);
     NN_CHECK(need <= part_floats, "attention_q4: %ld floats of scratch, %ld are needed", part_floats, need);
     if (n == 0) return 0;
     AttnQ4 p{q, dt, k_pages, v_pages, n_pages, block_table, bt_rows, bt_stride, tok_seq, tok_pos, out, part, n, n_heads, n_kv, D, scale, window, keep,
              slope_base, sinks, cap, head_gate, gate_ld, any_splits(n, n_heads, n_kv, longest)};
     const int group = n_heads / n_kv;
-    if (streams(dt, D)) {
+    if (streams(dt, D, cap)) {
         NN_CHECK((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)part % 16 == 0,
                  "attention_q4: bfloat16 queries, output and scratch start on 16-byte boundaries");
         // several tokens of one sequence: in two column tiles, as many as have columns there

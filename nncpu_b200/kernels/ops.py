@@ -1564,6 +1564,10 @@ def sample_temperature(logits, uniforms, out, temperature: float) -> None:
 
 Q4_GROUP = 32      # neighbouring lanes of a head that share a step and a least value
 
+# The greatest score cap that the tensor-core attention kernels take: they have a capped score as a difference of two numbers of the
+# cap's size, whose rounding beyond this one would show.
+MAX_FAST_CAP = 4096.0
+
 
 def q4_supported(head_dim: int) -> bool:
     """Whether a cache of 4 bits holds heads of ``head_dim`` lanes: whole groups of 32, at most 256 lanes."""
@@ -1771,15 +1775,15 @@ def _q4_longest(block_table, longest: int, window: int, keep: int) -> int:
 
 
 @functools.lru_cache(maxsize=4096)
-def _attention_q4_scratch(device: int, n_tok: int, n_heads: int, n_kv: int, head_dim: int, code: int, longest: int) -> int:
+def _attention_q4_scratch(device: int, n_tok: int, n_heads: int, n_kv: int, head_dim: int, code: int, longest: int, cap: float) -> int:
     lib = library.load("attention_q4")
     lib.nncpu_attention_q4_scratch.restype = ctypes.c_long
-    return lib.nncpu_attention_q4_scratch(_i(n_tok), _i(n_heads), _i(n_kv), _i(head_dim), _i(code), _i(longest))
+    return lib.nncpu_attention_q4_scratch(_i(n_tok), _i(n_heads), _i(n_kv), _i(head_dim), _i(code), _i(longest), _f(cap))
 
 
-def attention_q4_scratch_floats(n_tok: int, n_heads: int, n_kv: int, head_dim: int, dtype, longest: int) -> int:
-    """Floats of scratch that ``attention_q4`` needs at these sizes on the current device."""
-    return _attention_q4_scratch(torch._C._cuda_getDevice(), n_tok, n_heads, n_kv, head_dim, _DT[dtype], longest)
+def attention_q4_scratch_floats(n_tok: int, n_heads: int, n_kv: int, head_dim: int, dtype, longest: int, cap: float = 0.0) -> int:
+    """Floats of scratch that ``attention_q4`` needs at these sizes and with this score cap on the current device."""
+    return _attention_q4_scratch(torch._C._cuda_getDevice(), n_tok, n_heads, n_kv, head_dim, _DT[dtype], longest, cap)
 
 
 _ATTENTION_Q4 = [_P, _I, _P, _P, _I, _P, _I, _I, _P, _P, _P, _P, _L, _I, _I, _I, _I, _F, _I, _I, _F, _P, _F, _P, _I, _I, _P]
@@ -1791,7 +1795,7 @@ def attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_head
     """Causal attention of each token over its sequence's pages of a cache of 4 bits, token by token (decode steps, and a few tokens a
     sequence); q and out [n, n_heads * head_dim] of one type.  The options are those of ``attention``.  ``longest``: at least as many
     keys as any token sees (0: as the block tables have room for).  ``scratch``: float32, ``attention_q4_scratch_floats``
-    elements for the same ``longest`` (None: taken from the allocator).  A token of sequence -1 gives zeros; a page that
+    elements for the same ``longest`` and ``cap`` (None: taken from the allocator).  A token of sequence -1 gives zeros; a page that
     is not there (an id outside the pages) holds no keys."""
     n = _attention_q4_check("attention_q4", q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads, n_kv, head_dim, window,
                             keep, cap, sinks)
@@ -1800,7 +1804,7 @@ def attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_head
     q_at, k_at, v_at, table_at, seq_at, pos_at, out_at, sinks_at, scratch_at = _addresses(
         "attention_q4", q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, sinks, scratch)
     if scratch is None and not _dry:
-        need = _attention_q4_scratch(_cuda_device(), n, n_heads, n_kv, head_dim, code, longest)
+        need = _attention_q4_scratch(_cuda_device(), n, n_heads, n_kv, head_dim, code, longest, cap)
         if need:
             scratch = torch.empty(need, dtype=torch.float32, device=q.device)
             scratch_at = scratch.data_ptr()
@@ -1823,7 +1827,7 @@ Q4_EXPAND_POSITIONS_F32 = 65536
 
 
 @functools.lru_cache(maxsize=4096)
-def _q4_prompt_plan(n: int, n_seqs: int, n_heads: int, n_kv: int, head_dim: int, bf16: bool, longest: int, slope_and_cap: bool):
+def _q4_prompt_plan(n: int, n_seqs: int, n_heads: int, n_kv: int, head_dim: int, bf16: bool, longest: int, slope: bool, cap: float):
     """How a prompt attends: (lanes of the rows that the keys are taken out to, or 0: straight from the codes; pages of a sequence;
     sequences at a time; bytes of keys; of keys, values, table and (float32) the tokens' sequences and positions; of all)."""
     width = (longest + 63) // 64
@@ -1831,7 +1835,7 @@ def _q4_prompt_plan(n: int, n_seqs: int, n_heads: int, n_kv: int, head_dim: int,
     if n <= n_seqs or (bf16 and n_seqs == 1 and n <= Q4_FEW_TOKENS and longest > 128 and head_dim <= 128):
         pass
     elif bf16:
-        lanes = 0 if slope_and_cap else 64 if head_dim <= 64 else 128 if head_dim <= 128 else 0
+        lanes = 0 if (slope and cap > 0.0) or cap > MAX_FAST_CAP else 64 if head_dim <= 64 else 128 if head_dim <= 128 else 0
     elif head_dim <= 128 and n_heads // n_kv <= 32 and n_seqs * width * 64 <= Q4_EXPAND_POSITIONS_F32:
         lanes = head_dim
     if lanes == 0:
@@ -1847,8 +1851,8 @@ def _q4_prompt_plan(n: int, n_seqs: int, n_heads: int, n_kv: int, head_dim: int,
 def attention_q4_prompt_scratch_bytes(n_tok: int, n_seqs: int, n_heads: int, n_kv: int, head_dim: int, dtype, longest: int,
                                       slope_base: float = 0.0, cap: float = 0.0) -> int:
     """Bytes of scratch that ``attention_q4_prompt`` needs at these sizes on the current device; ``longest``: that call's."""
-    plan = _q4_prompt_plan(n_tok, n_seqs, n_heads, n_kv, head_dim, dtype == torch.bfloat16, longest, slope_base != 0.0 and cap != 0.0)
-    return plan[5] if plan[0] else 4 * attention_q4_scratch_floats(n_tok, n_heads, n_kv, head_dim, dtype, longest)
+    plan = _q4_prompt_plan(n_tok, n_seqs, n_heads, n_kv, head_dim, dtype == torch.bfloat16, longest, slope_base != 0.0, cap)
+    return plan[5] if plan[0] else 4 * attention_q4_scratch_floats(n_tok, n_heads, n_kv, head_dim, dtype, longest, cap)
 
 
 _EXPAND_Q4 = [_P, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I]
@@ -1875,12 +1879,12 @@ def attention_q4_prompt(q, k_pages, v_pages, block_table, cu_seqlens, tok_seq, t
     code = _code(q)
     bf16 = code == 1
     lanes, width, at_once, kv_bytes, table_end, need = _q4_prompt_plan(n, n_seqs, n_heads, n_kv, head_dim, bf16, longest,
-                                                                       slope_base != 0.0 and cap != 0.0)
+                                                                       slope_base != 0.0, cap)
     q_at, k_at, v_at, table_at, cu_at, seq_at, pos_at, out_at, sinks_at, status_at, base = _addresses(
         fn, q, k_pages, v_pages, block_table, cu_seqlens, tok_seq, tok_pos, out, sinks, status, scratch)
     if not _dry:
         if lanes == 0:
-            need = 4 * _attention_q4_scratch(_cuda_device(), n, n_heads, n_kv, head_dim, code, longest)
+            need = 4 * _attention_q4_scratch(_cuda_device(), n, n_heads, n_kv, head_dim, code, longest, cap)
         if scratch is None and need:
             scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
             base = scratch.data_ptr()

@@ -51,8 +51,7 @@ from . import base
 from .base import Mixer, register_mixer
 
 
-# The tensor-core kernels' cap is a difference of two numbers of the cap's size; beyond this one its rounding would show.
-MAX_FAST_CAP = 4096.0
+MAX_FAST_CAP = ops.MAX_FAST_CAP
 
 
 @register_mixer("attention")
@@ -220,7 +219,7 @@ class Attention(Mixer):
         with self._core_phase(ctx, cache):
             if ctx.is_decode:
                 longest = self._longest_span(ctx) + 128 if self.span else ctx.max_kv_len
-                floats = ops.attention_q4_scratch_floats(n, *sizes, rt.dtype, longest)
+                floats = ops.attention_q4_scratch_floats(n, *sizes, rt.dtype, longest, s.score_cap)
                 scratch = rt.empty(floats, dtype=torch.float32) if floats else None
                 ops.attention_q4(q, cache.k_pages, cache.v_pages, cache.block_table, ctx.tok_seq, ctx.tok_pos, attn, *sizes, s.scale,
                                  longest=longest, scratch=scratch, **options)
