@@ -39,7 +39,9 @@
 // Keys and values may be float16 instead (kHalf: a 4-bit cache's, taken out of its codes by cache_q4.cu; eight times finer than
 // bfloat16, and within float16's range by that cache's format).  Both operands of a product are of one type, so a row's thread then turns
 // its query into float16 in shared memory, times a power of two that makes its greatest lane at most 1, which is
-// exact for all but what is 2^-14 below that; the power of two goes into the factor of the row's scores.  The weights are float16 too.
+// exact for all but what is 2^-14 below that; the power of two goes into the factor of the row's scores.  The weights are float16 too: they
+// are taken against a reference 2^kHalfRoom below the greatest score, so that what is 2^-22 of the greatest weight is a normal number still and what
+// is 2^-32 of it counts (against the greatest score itself all below 2^-25 was lost: a tail under a first key without value).
 //
 // Every wait on an mbarrier is bounded in time; a wait that runs out sets
 // *status, the other roles run into their own limits, copies in flight are
@@ -67,6 +69,8 @@ constexpr int kAloneSteps = 4;
 constexpr int kStreamCols = 256;  // tensor-memory columns per head: S (P over its second half) | O
 constexpr int kPOffset = 64;      // P lies over the second half of S
 constexpr float kSumLimit = 256.0f;  // a step's weights of a row may add up to this before the row's reference maximum is moved
+// The same with float16 weights, which start at 2^kHalfRoom (128 of them add up to 2^15) and must stay below 65 520.
+constexpr float kHalfRoom = 8.0f, kHalfSumLimit = 65024.0f;
 
 enum AttnStatus : int { kTimeoutQ = 201, kTimeoutStage = 202, kTimeoutK = 203, kTimeoutV = 204, kTimeoutS = 205,
                         kTimeoutP = 206, kTimeoutPv = 207 };
@@ -495,8 +499,8 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             const int halves = min(2, n_pages - 2 * (s0 + i));
             const int k_base[2] = {walk.page(2 * (s0 + i)) * kPage, walk.page(2 * (s0 + i) + 1) * kPage};
             // A step costs one pass over the row's scores: weights against the reference maximum as it stands (as
-            // bfloat16 pairs) and their sum.  The largest score is not looked for: a sum of at most 2^8 proves that
-            // no weight is above 2^8.  Only when a row's sum says otherwise (or the row has seen no key yet) is the
+            // bfloat16 pairs; kHalf: see the head of this file) and their sum.  The largest score is not looked for: a sum of at
+            // most 2^8 proves that no weight is above 2^8.  Only when a row's sum says otherwise (or the row has seen no key yet) is the
             // largest score found in a pass of its own; then the reference moves up to it, O and the sum so far
             // follow, and the weights are computed again.  The O update of the step before is complete (these
             // scores were issued after it), so O may be touched.
@@ -567,7 +571,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             };
             const bool unseen = __any_sync(0xffffffffu, m_ref == -INFINITY && valid);
             if (!unseen) weights();
-            if (unseen || __any_sync(0xffffffffu, valid && !(sum <= kSumLimit))) {
+            if (unseen || __any_sync(0xffffffffu, valid && !(sum <= (kHalf ? kHalfSumLimit : kSumLimit)))) {
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
@@ -578,7 +582,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                         for (int c = 0; c < 64; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(u[c]));
                     }
                 }
-                const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * score_mul;   // the factor is positive
+                const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * score_mul - (kHalf ? kHalfRoom : 0.0f);   // the factor is positive
                 float alpha = 1.0f;
                 if (tmax > m_ref) {
                     alpha = fast_exp2(m_ref - tmax);    // 0 when nothing was seen yet
