@@ -28,7 +28,7 @@ import torch
 from .. import perf
 from ..cache import pages_for
 from ..kernels import ops
-from ..parts.runtime import Arena
+from ..parts.runtime import Arena, SharedScratch
 from .step import StepContext
 
 _RING = 4  # pinned host copies of the metadata in flight
@@ -204,7 +204,7 @@ class PromptGraph:
     no sequence (index -1), so nothing is written to the cache for them, attention leaves them out, and what the
     products compute in their rows is never read."""
 
-    def __init__(self, engine, size: int):
+    def __init__(self, engine, size: int, scratch: SharedScratch):
         self._engine, self.size = weakref.ref(engine), size
         cache = engine.cache
         dev = cache.device
@@ -228,9 +228,10 @@ class PromptGraph:
             tok_pos=m[self.o_pos:self.o_pos + T], seq_slots=m[self.o_slot:self.o_slot + 1],
             cu_seqlens=m[self.o_cu:self.o_cu + 2], logit_rows=m[self.o_row:self.o_row + 1],
             block_tables=[m[o:o + self.width].view(1, self.width) for o in self.o_tables],
-            q_lens=[T], kv_lens=[T], is_decode=False, max_kv_len=cache.max_seq_len)
+            q_lens=[T], kv_lens=[T], is_decode=False, max_kv_len=cache.max_seq_len, scratch=scratch)
         self.logits: Optional[torch.Tensor] = None
         self.arena = Arena(dev)
+        self.shared: Optional[torch.Tensor] = None      # the shared scratch that the graph was captured with
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.n_kernels = 0
         self.h2d_bytes = 0
@@ -300,6 +301,7 @@ class PromptGraph:
                 self.n_kernels = ops.launch_count() - before
                 ops.add_launches(-self.n_kernels)
                 self.graph = g
+                self.shared = self.ctx.scratch.buf
                 self.logits.copy_(eager)
             else:
                 self.graph.replay()
@@ -312,6 +314,7 @@ class DecodeGraphs:
         self._engine = weakref.ref(engine)
         self.by_size: Dict[int, DecodeGraph] = {}
         self.prompts: Dict[int, PromptGraph] = {}
+        self.prompt_scratch = SharedScratch(engine.model.rt.device, PROMPT_GRAPH_MAX)
 
     def get(self, n: int) -> DecodeGraph:
         size = bucket(n)
@@ -325,5 +328,5 @@ class DecodeGraphs:
         size = max(PROMPT_GRAPH_MIN, bucket(n))
         g = self.prompts.get(size)
         if g is None:
-            g = self.prompts[size] = PromptGraph(self._engine(), size)
+            g = self.prompts[size] = PromptGraph(self._engine(), size, self.prompt_scratch)
         return g

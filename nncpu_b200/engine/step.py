@@ -49,6 +49,7 @@ class StepContext:
     branch_is_fresh: bool = False         # the "residual" a part was given is an uninitialised branch: its last product writes, not adds
     closing: Optional[object] = None      # a parts.base.SublayerClosing for a part that says ``closes_sublayer``
     out_scale: float = 1.0                # a part that says ``scales_output`` multiplies what it adds to the stream by this
+    scratch: Optional[object] = None      # a parts.runtime.SharedScratch for what is as large as the context (None: the step's arena)
 
     def span_sum(self, window: int = 0, chunk: int = 0, keep_first: int = 0) -> int:
         """Keys that the step's tokens attend to, summed over the tokens: a token at position p sees p + 1

@@ -224,8 +224,12 @@ class Attention(Mixer):
                 ops.attention_q4(q, cache.k_pages, cache.v_pages, cache.block_table, ctx.tok_seq, ctx.tok_pos, attn, *sizes, s.scale,
                                  longest=longest, scratch=scratch, **options)
             else:
-                need = ops.attention_q4_prompt_scratch_bytes(n, ctx.n_seqs, *sizes, rt.dtype, ctx.max_kv_len, s.slope_base, s.score_cap)
-                scratch = rt.empty(need, dtype=torch.uint8) if need else None
+                def need(tokens):
+                    return ops.attention_q4_prompt_scratch_bytes(tokens, ctx.n_seqs, *sizes, rt.dtype, ctx.max_kv_len, s.slope_base, s.score_cap)
+                if ctx.scratch is None:
+                    scratch = rt.empty(need(n), dtype=torch.uint8)
+                else:       # (all steps that take the keys out of their codes: room for the largest of them at once)
+                    scratch = ctx.scratch.take(max(need(n), need(ctx.scratch.tokens) if n > ops.Q4_FEW_TOKENS else 0))
                 ops.attention_q4_prompt(q, cache.k_pages, cache.v_pages, cache.block_table, ctx.cu_seqlens, ctx.tok_seq, ctx.tok_pos, attn,
                                         ctx.n_seqs, *sizes, s.scale, ctx.max_kv_len, rt.workspace.status, scratch=scratch, **options)
         if s.out_gate:

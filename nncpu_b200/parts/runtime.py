@@ -93,6 +93,24 @@ class Arena:
         return t
 
 
+class SharedScratch:
+    """Device memory that the captured prompt steps of an engine share for what is as large as the context: they run one
+    after another, and nothing in it outlives the part that asked for it.  ``tokens``: the most that such a step has.  The first run of a
+    step, which is not captured, makes it; should a later step need more, a larger one takes its place, and graphs that have
+    the old one's address keep that."""
+
+    def __init__(self, device, tokens: int):
+        self.device, self.tokens = torch.device(device), tokens
+        self.buf: Optional[torch.Tensor] = None
+
+    def take(self, nbytes: int) -> torch.Tensor:
+        """uint8, ``nbytes`` elements or more."""
+        if self.buf is None or self.buf.numel() < nbytes:
+            self.buf = None             # the old one goes back before the new one is asked for
+            self.buf = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        return self.buf
+
+
 class Runtime:
     def __init__(self, device, dtype: torch.dtype):
         self.device = torch.device(device)
