@@ -262,10 +262,11 @@ class Engine:
             page = table[0, pos.long() // PAGE].long()
             there = (page >= 0)[:, None, None]
             return tuple(torch.where(there, t[page.clamp(min=0), :, pos.long() % PAGE].float(), 0.0) for t in (k, v))
-        heads = k.shape[1]
-        out = [torch.empty(n, heads * self.cache.groups[g].request.head_dim, device=self.cache.device) for _ in range(2)]
-        ops.q4_read(k, v, table, torch.zeros_like(pos), pos, *out)
-        return tuple(t.view(n, heads, -1) for t in out)
+        heads, lanes = k.shape[1], self.cache.groups[g].request.head_dim
+        out = [torch.empty(n, heads * lanes, device=self.cache.device) for _ in range(2)]
+        if n:       # (without tokens the table has no width)
+            ops.q4_read(k, v, table, torch.zeros_like(pos), pos, *out)
+        return tuple(t.view(n, heads, lanes) for t in out)
 
     # -- the step ----------------------------------------------------------------
 

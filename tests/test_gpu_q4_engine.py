@@ -1,4 +1,4 @@
-"""An engine over a cache of 4 bits: what its captured portions hold."""
+"""An engine over a cache of 4 bits: what captured portions hold, and slots without tokens."""
 import gc
 
 import pytest
@@ -40,3 +40,10 @@ def test_captured_portions_of_all_sizes_share_what_the_keys_are_taken_out_to(fol
     want = plain(folders[dtype], text, engine, slot)[[n - 1 for n, _ in used]]
     check(torch.stack(rows), want, TOL[dtype], "portions")
     assert all(b[1] - a[1] < taken_out // 4 for a, b in zip(used, used[1:])), used
+
+
+@pytest.mark.parametrize("kv_dtype", [None, "q4"])
+def test_a_slot_without_tokens_holds_nothing(folders, kv_dtype):
+    engine = Engine(Model.load(folders["bfloat16"]), max_tokens=256, kv_dtype=kv_dtype)
+    k, v = engine.cached(engine.alloc_slot())
+    assert k.shape == v.shape == (0, 2, 128) and k.dtype == v.dtype == torch.float32
