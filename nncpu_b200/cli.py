@@ -233,6 +233,12 @@ def _logprob_line(t) -> str:
     return json.dumps({"token": t.token, "logprob": t.logprob, "entropy": t.entropy, "top": [list(x) for x in t.top]})
 
 
+def _print_logprobs(tokens, err) -> None:
+    """A line of JSON for each of a reply's or a text's tokens (None: they were not asked for)."""
+    for t in tokens or ():
+        print(_logprob_line(t), file=err)
+
+
 def run_generate(o: Options, out=sys.stdout, err=sys.stderr) -> int:
     from . import Model, Session, SessionParams
     from .text import load_tokenizer
@@ -267,8 +273,7 @@ def run_generate(o: Options, out=sys.stdout, err=sys.stderr) -> int:
     out.write("\n")
     out.flush()
     for r in res:
-        for t in r.logprobs or ():
-            print(_logprob_line(t), file=err)
+        _print_logprobs(r.logprobs, err)
     if o.perf or o.verbose:
         r = res[0]
         n = sum(x.n_generated for x in res)
@@ -363,6 +368,7 @@ def chat_loop(session, o: Options, lines, out=sys.stdout, err=sys.stderr, intera
                 continue
             out.write("\n")
             out.flush()
+            _print_logprobs(res.logprobs, err)
             print(_stats_line(res, o.verbose, o.n_predict), file=err)
             _perf_end(o, "reply", res.n_prompt + res.n_generated, err)
     return 0
@@ -427,8 +433,7 @@ def run_perplexity(o: Options, out=sys.stdout, err=sys.stderr) -> int:
         r = session.score([part], k)[0]
         n, total = n + len(r.tokens), total + r.logprob
         if o.logprobs is not None:
-            for t in r.tokens:
-                print(_logprob_line(t), file=err)
+            _print_logprobs(r.tokens, err)
     dt = time.perf_counter() - t0
     mean = ScoreResult([TokenLogprob(0, total / n, 0.0)])
     out.write(f"{n} predictions of {len(ids)} tokens: {total / n:.6f} nats a token, perplexity {mean.perplexity:.4f} "

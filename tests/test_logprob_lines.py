@@ -1,0 +1,43 @@
+"""What the command line says about log probabilities, and what it refuses (no GPU)."""
+import io
+import json
+import math
+from types import SimpleNamespace
+
+import pytest
+
+import nncpu_b200
+from nncpu_b200 import cli
+from nncpu_b200.cli import Options, chat_loop, parse_options, run_gen, run_perplexity
+from nncpu_b200.errors import InvalidArgument
+from nncpu_b200.sampling import GenerateResult, ScoreResult, StopReason, TokenLogprob
+
+FOUND = [TokenLogprob(5, -0.5, 1.25, ((5, -0.5), (9, -1.0))), TokenLogprob(6, -2.0, 0.75, ((7, -0.25), (6, -2.0)))]
+
+
+def lines(text):
+    return [json.loads(x) for x in text.splitlines() if x.startswith("{")]
+
+
+class Chat:
+    """Stands in for a session: every reply is FOUND's tokens."""
+    n_ctx = 100
+
+    def cancel_handle(self):
+        return SimpleNamespace(cancel=lambda: None)
+
+    def chat(self, message, params, on_text):
+        on_text(SimpleNamespace(text="yes"))
+        return GenerateResult(StopReason.END_OF_TURN, 3, 2, 0.1, 0.1, [5, 6], FOUND if params.logprobs is not None else None)
+
+
+@pytest.mark.parametrize("asked", [True, False])
+def test_a_chats_replies_come_with_their_log_probabilities(asked):
+    o = parse_options(["chat", "-m", "d", *(["--logprobs", "2"] if asked else [])])
+    out, err = io.StringIO(), io.StringIO()
+    assert chat_loop(Chat(), o, iter(["a\n", "b\n", "/exit\n"]), out, err) == 0
+    got = lines(err.getvalue())
+    assert out.getvalue() == "yes\nyes\n" and err.getvalue().count("tok/s") == 2
+    assert [t["token"] for t in got] == ([5, 6, 5, 6] if asked else [])
+    if asked:
+        assert got[1] == {"token": 6, "logprob": -2.0, "entropy": 0.75, "top": [[7, -0.25], [6, -2.0]]}
