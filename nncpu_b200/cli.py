@@ -391,7 +391,7 @@ def run_chat(o: Options, stdin=None, out=sys.stdout, err=sys.stderr) -> int:
     return chat_loop(session, o, iter(stdin.readline, ""), out, err, interactive=stdin.isatty())
 
 
-def run_gen(o: Options, out=sys.stdout) -> int:
+def run_gen(o: Options, out=sys.stdout, err=sys.stderr) -> int:
     """Greedy token-level harness (crates/nncpu-cli/src/devtools.rs:635-705)."""
     from . import Model, Session, SessionParams
     folder, ids = o.args[0], _token_list(o.args[1])
@@ -400,11 +400,12 @@ def run_gen(o: Options, out=sys.stdout) -> int:
     model = Model.load(folder, dtype=o.dtype)
     session = Session(model, SessionParams(n_ctx=ctx, seed=1, kv_f32=o.kv_f32, kv_q4=o.kv_q4, max_batch=1))
     _perf_begin(o)
-    res = session.generate([ids], GenerateParams(n, SamplerParams.greedy()))[0]
+    res = session.generate([ids], GenerateParams(n, SamplerParams.greedy(), o.logprobs))[0]
     out.write(" ".join(str(t) for t in res.tokens) + "\n")
     out.write(f"prefill: {res.n_prompt} tokens, {res.prefill * 1e3:.1f} ms ({res.n_prompt / max(res.prefill, 1e-9):.1f} tok/s)\n")
     out.write(f"decode: {res.n_generated} tokens, {res.decode * 1e3:.1f} ms ({res.n_generated / max(res.decode, 1e-9):.1f} tok/s)\n")
     out.write(f"stop: {res.stop.value}\n")
+    _print_logprobs(res.logprobs, err)
     _perf_end(o, "gen", res.n_prompt + res.n_generated, out)
     return 0
 

@@ -41,3 +41,27 @@ def test_a_chats_replies_come_with_their_log_probabilities(asked):
     assert [t["token"] for t in got] == ([5, 6, 5, 6] if asked else [])
     if asked:
         assert got[1] == {"token": 6, "logprob": -2.0, "entropy": 0.75, "top": [[7, -0.25], [6, -2.0]]}
+
+
+class Token:
+    """Stands in for a session that generates or scores."""
+
+    def __init__(self, model, params, tokenizer=None):
+        self.n_ctx, self.params = params.n_ctx or 100, params
+
+    def generate(self, prompts, params, on_piece=None):
+        return [GenerateResult(StopReason.MAX_TOKENS, len(p), 2, 0.1, 0.1, [5, 6], FOUND if params.logprobs is not None else None) for p in prompts]
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    monkeypatch.setattr(nncpu_b200, "Model", SimpleNamespace(load=lambda folder, dtype: None))
+    monkeypatch.setattr(nncpu_b200, "Session", Token)
+
+
+@pytest.mark.parametrize("asked", [True, False])
+def test_the_greedy_run_tells_them_too(fake, asked):
+    out, err = io.StringIO(), io.StringIO()
+    assert run_gen(parse_options(["--gen", "d", "1 2 3", "2", *(["--logprobs", "2"] if asked else [])]), out, err) == 0
+    assert out.getvalue().startswith("5 6\nprefill: 3 tokens")
+    assert [t["token"] for t in lines(err.getvalue())] == ([5, 6] if asked else [])
