@@ -7,12 +7,14 @@ its token-level harness (crates/nncpu-cli/src/devtools.rs:70-90,632-705) as
     nncpu-b200 -m DIR -p TEXT                           answer one message (needs tokenizer.json), streamed
     nncpu-b200 chat -m DIR                              chat: a message per line, /reset /exit /help
     nncpu-b200 --gen DIR "ID ID ..." [N] [CTX]          greedy token-level run with timings
+    nncpu-b200 --perplexity DIR FILE                    how well the model predicts a file
     nncpu-b200 --info DIR                               what the folder holds
     nncpu-b200 --random-weights CONFIG.json SEED OUT    write a model folder with random weights
 """
 from __future__ import annotations
 
 import json
+import math
 import os
 import signal
 import sys
@@ -230,7 +232,11 @@ def _stats_line(res, verbose: bool, n_predict: int) -> str:
 
 
 def _logprob_line(t) -> str:
-    return json.dumps({"token": t.token, "logprob": t.logprob, "entropy": t.entropy, "top": [list(x) for x in t.top]})
+    """(JSON has no infinities and no NaN: such a number, of a token that cannot come, is null.)"""
+    def number(x):
+        return x if math.isfinite(x) else None
+    return json.dumps({"token": t.token, "logprob": number(t.logprob), "entropy": number(t.entropy),
+                       "top": [[i, number(x)] for i, x in t.top]})
 
 
 def _print_logprobs(tokens, err) -> None:

@@ -2,6 +2,7 @@
 import io
 import json
 import math
+import math
 from types import SimpleNamespace
 
 import pytest
@@ -65,3 +66,12 @@ def test_the_greedy_run_tells_them_too(fake, asked):
     assert run_gen(parse_options(["--gen", "d", "1 2 3", "2", *(["--logprobs", "2"] if asked else [])]), out, err) == 0
     assert out.getvalue().startswith("5 6\nprefill: 3 tokens")
     assert [t["token"] for t in lines(err.getvalue())] == ([5, 6] if asked else [])
+
+
+@pytest.mark.parametrize("value", [-math.inf, math.nan, math.inf])
+def test_every_line_is_json_whatever_the_numbers(value):
+    """JSON has no infinities and no NaN: such a number is null."""
+    def refuse(name):
+        raise AssertionError(f"{name} is not JSON")
+    line = cli._logprob_line(TokenLogprob(3, value, value, ((3, -0.5), (4, value))))
+    assert json.loads(line, parse_constant=refuse) == {"token": 3, "logprob": None, "entropy": None, "top": [[3, -0.5], [4, None]]}
