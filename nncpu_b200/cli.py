@@ -432,6 +432,8 @@ def run_perplexity(o: Options, out=sys.stdout, err=sys.stderr) -> int:
         raise InvalidArgument(f"{path}: {len(ids)} tokens, a prediction takes two")
     model = Model.load(folder, dtype=o.dtype)
     session = Session(model, SessionParams(n_ctx=o.n_ctx, seed=1, kv_f32=o.kv_f32, kv_q4=o.kv_q4, max_batch=1))
+    if session.n_ctx < 2:
+        raise InvalidArgument(f"a context of {session.n_ctx} token: a prediction takes two")
     _perf_begin(o)
     n, total, k = 0, 0.0, o.logprobs or 0
     t0 = time.perf_counter()

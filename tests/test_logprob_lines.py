@@ -75,3 +75,25 @@ def test_every_line_is_json_whatever_the_numbers(value):
         raise AssertionError(f"{name} is not JSON")
     line = cli._logprob_line(TokenLogprob(3, value, value, ((3, -0.5), (4, value))))
     assert json.loads(line, parse_constant=refuse) == {"token": 3, "logprob": None, "entropy": None, "top": [[3, -0.5], [4, None]]}
+
+
+def perplexity(tmp_path, monkeypatch, text, n_ctx, logprob=-1.0):
+    """run_perplexity over a file of ``text``: what it prints, and the stretches that were scored."""
+    scored = []
+
+    def score(self, texts, k):
+        scored.extend(texts)
+        return [ScoreResult([TokenLogprob(x, logprob, 0.0) for x in t[1:]]) for t in texts]
+    monkeypatch.setattr(Token, "score", score, raising=False)
+    f = tmp_path / "text"
+    f.write_text(text)
+    out = io.StringIO()
+    assert run_perplexity(parse_options(["--perplexity", "d", str(f), "-c", str(n_ctx)]), out, io.StringIO()) == 0
+    return out.getvalue(), scored
+
+
+def test_a_perplexity_needs_a_context_of_two(fake, tmp_path, monkeypatch):
+    with pytest.raises(InvalidArgument, match="context"):
+        perplexity(tmp_path, monkeypatch, "1 2 3", 1)
+    out, scored = perplexity(tmp_path, monkeypatch, "1 2 3 4 5", 2)
+    assert scored == [[1, 2], [3, 4], [5]] and out.startswith("2 predictions of 5 tokens: -1.000000 nats a token, perplexity 2.7183")
