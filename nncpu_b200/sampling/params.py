@@ -94,7 +94,7 @@ class ScoreResult:
         if not self.tokens:
             return math.nan
         mean = -self.logprob / len(self.tokens)
-        return math.exp(mean) if mean < 700 else math.inf
+        return math.inf if mean >= 700 else math.exp(mean)
 
 
 class StopReason(Enum):

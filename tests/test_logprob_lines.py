@@ -97,3 +97,10 @@ def test_a_perplexity_needs_a_context_of_two(fake, tmp_path, monkeypatch):
         perplexity(tmp_path, monkeypatch, "1 2 3", 1)
     out, scored = perplexity(tmp_path, monkeypatch, "1 2 3 4 5", 2)
     assert scored == [[1, 2], [3, 4], [5]] and out.startswith("2 predictions of 5 tokens: -1.000000 nats a token, perplexity 2.7183")
+
+
+def test_a_perplexity_of_no_number_is_none(fake, tmp_path, monkeypatch):
+    """Logits of +inf give NaN, of which the perplexity is not infinite."""
+    assert math.isnan(ScoreResult([TokenLogprob(1, -1.0, 0.0), TokenLogprob(1, math.nan, 0.0)]).perplexity)
+    assert "perplexity nan" in perplexity(tmp_path, monkeypatch, "1 2 3", 9, math.nan)[0]
+    assert "perplexity inf" in perplexity(tmp_path, monkeypatch, "1 2 3", 9, -math.inf)[0]
