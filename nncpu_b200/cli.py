@@ -427,7 +427,7 @@ def run_perplexity(o: Options, out=sys.stdout, err=sys.stderr) -> int:
     except (OSError, UnicodeDecodeError) as e:
         raise InvalidArgument(f"{path}: {e}") from None
     words = text.replace(",", " ").split()
-    ids = [int(t) for t in words] if all(t.isdigit() for t in words) else load_tokenizer(folder).encode(text)
+    ids = [int(t) for t in words] if all(t.isascii() and t.isdigit() for t in words) else load_tokenizer(folder).encode(text)
     if len(ids) < 2:
         raise InvalidArgument(f"{path}: {len(ids)} tokens, a prediction takes two")
     model = Model.load(folder, dtype=o.dtype)

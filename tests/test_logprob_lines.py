@@ -104,3 +104,10 @@ def test_a_perplexity_of_no_number_is_none(fake, tmp_path, monkeypatch):
     assert math.isnan(ScoreResult([TokenLogprob(1, -1.0, 0.0), TokenLogprob(1, math.nan, 0.0)]).perplexity)
     assert "perplexity nan" in perplexity(tmp_path, monkeypatch, "1 2 3", 9, math.nan)[0]
     assert "perplexity inf" in perplexity(tmp_path, monkeypatch, "1 2 3", 9, -math.inf)[0]
+
+
+@pytest.mark.parametrize("text", ["² ³", "1 ²"])
+def test_a_text_of_other_digits_is_text(fake, tmp_path, monkeypatch, text):
+    """(Superscripts are digits, and no numbers.)"""
+    monkeypatch.setattr("nncpu_b200.text.load_tokenizer", lambda folder: SimpleNamespace(encode=lambda t: list(t.encode())))
+    assert perplexity(tmp_path, monkeypatch, text, 99)[1] == [list(text.encode())]
