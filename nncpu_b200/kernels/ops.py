@@ -1690,6 +1690,8 @@ def qk_norm_rope_append_q4(qkv, q_gamma, k_gamma, eps: float, cos_sin, tok_seq, 
     lo's rounding).  Numbers beyond +-65504 count as that; a group with a NaN is NaN.  Keys are normed and rotated in 64 bits, so
     that a code does not hang on the order of a sum.  ``n_kv`` 0: qkv holds q only and nothing is appended.  A token of sequence -1, or
     whose position has no page, is not appended; two tokens of a call must not have the same place.  ``q_temp`` as in ``qk_norm_rope_append``."""
+    if q_out.dim() != 2 or (cos_sin is not None and cos_sin.dim() != 3):
+        _need(False, "qk_norm_rope_append_q4", f"queries to {list(q_out.shape)}" + ("" if cos_sin is None else f", a rotation of {list(cos_sin.shape)}"))
     n, rows = q_out.shape[0], qkv.shape
     half = 0 if cos_sin is None else cos_sin.shape[1]
     coef, every = q_temp if q_temp is not None else (0.0, 1)
@@ -1727,6 +1729,8 @@ _READ_Q4 = [_P, _P, _I, _P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I]
 def q4_read(k_pages, v_pages, block_table, tok_seq, tok_pos, k_out, v_out) -> None:
     """What a cache of 4 bits holds of given tokens, as numbers: keys and values of the token at position tok_pos[t] of sequence
     tok_seq[t] to ``k_out`` and ``v_out`` [n, n_kv * head_dim] (float32 or bfloat16).  A token of sequence -1, or without a page: zeros."""
+    if not (k_out.dim() == 2 and k_pages.dim() == 3 and k_pages.shape[1] > 0):
+        _need(False, "q4_read", f"pages of shape {list(k_pages.shape)}, keys to {list(k_out.shape)}")
     (n, lanes), pages = k_out.shape, k_pages.shape
     n_kv = pages[1]
     head_dim = lanes // n_kv
@@ -1742,6 +1746,8 @@ def q4_read(k_pages, v_pages, block_table, tok_seq, tok_pos, k_out, v_out) -> No
 
 def _attention_q4_check(fn: str, q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads: int, n_kv: int, head_dim: int,
                         window: int, keep: int, cap: float, sinks) -> int:
+    if q.dim() != 2:
+        _need(False, fn, f"queries of shape {list(q.shape)}")
     n, width = q.shape
     if not (n_kv > 0 and n_heads > 0 and n_heads % n_kv == 0 and width == n_heads * head_dim and out.shape == (n, width) and q.dtype is out.dtype
             and _q4_pages_ok(k_pages, v_pages, n_kv, head_dim) and _q4_places_ok(n, block_table, tok_seq, tok_pos)
