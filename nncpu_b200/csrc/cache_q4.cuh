@@ -3,7 +3,7 @@
 // A page holds kPage positions of one key/value head of D = 32 NG lanes, as keys or as values, in 40 D bytes.  The lanes lie in
 // groups of 32; lane x of a group is d c + m with c in 0..15 and the group's two float16 numbers:
 //   lo, hi = least and greatest of the group, each within +-65504 (float16's range: what lies beyond is taken as its end);
-//   d = half((hi - lo) / 15), m = half(lo), c = clamp(rint((x - m) (1 / d)), 0, 15), each operation rounded to 32 bits; d of 0: c = 0.
+//   d = half((hi - lo) (1 / 15)), m = half(lo), c = clamp(rint((x - m) (1 / d)), 0, 15), 1 / 15 and 1 / d rounded to 32 bits, as is each operation; d of 0: c = 0.
 // A group that holds a NaN is NaN as a whole (m is).
 //
 //   key page:    64 rows of D / 2 bytes; then 64 rows of NG pairs (d, m).
@@ -38,7 +38,7 @@ struct Q4Scale {
 };
 __device__ __forceinline__ Q4Scale q4_scale(float lo, float hi) {
     Q4Scale s;
-    s.d = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
+    s.d = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
     s.m = __float2half_rn(lo);
     const float d = __half2float(s.d);
     s.m32 = __half2float(s.m);
