@@ -1686,8 +1686,8 @@ def qk_norm_rope_append_q4(qkv, q_gamma, k_gamma, eps: float, cos_sin, tok_seq, 
     ``cos_sin`` float32 [n, half, 2] turns the pairs (i, i + half); pages uint8 [n_pages, n_kv, ``q4_page_bytes``].
 
     A head's lanes are cut in groups of 32.  With lo and hi the group's least and greatest number, a lane is d c + lo,
-    d = (hi - lo) / 15 and lo both float16, and c = round((x - lo) / d) one of 0 to 15: a number is off by at most half a step d (and
-    lo's rounding).  Numbers beyond +-65504 count as that; a group with a NaN is NaN.  Keys are normed and rotated in 64 bits, so
+    d = (hi - lo) * (1 / 15) and lo both float16, and c = round((x - lo) * (1 / d)) one of 0 to 15 (each operation, 1 / 15 and 1 / d among them,
+    is rounded to 32 bits): a number is off by at most half a step d (and lo's rounding).  Numbers beyond +-65504 count as that; a group with a NaN is NaN.  Keys are normed and rotated in 64 bits, so
     that a code does not hang on the order of a sum.  ``n_kv`` 0: qkv holds q only and nothing is appended.  A token of sequence -1, or
     whose position has no page, is not appended; two tokens of a call must not have the same place.  ``q_temp`` as in ``qk_norm_rope_append``."""
     if q_out.dim() != 2 or (cos_sin is not None and cos_sin.dim() != 3):
