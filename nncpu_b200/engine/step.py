@@ -202,7 +202,8 @@ class Engine:
         if q4:
             if kv_dtype != "q4":
                 raise InvalidArgument(f"a cache of {kv_dtype!r}: a torch type or 'q4'")
-            wrong = sorted({m.spec.kind for b in model.blocks for m in b.mixers() if not m.takes_q4()})
+            wrong = sorted({k for b in model.blocks if not b.takes_q4()
+                            for k in [m.spec.kind for m in b.mixers() if not m.takes_q4()] or [f"those of a {type(b).__name__}"]})
             if wrong:
                 raise UnsupportedModel(f"{model.spec.architecture}: a cache of 4 bits holds grouped-query attention with heads of whole "
                                        f"groups of {Q4_GROUP} lanes, keys and values apart (mixers here that are not: {', '.join(wrong)})")

@@ -161,8 +161,8 @@ class Mixer(Part):
         return None
 
     def takes_q4(self) -> bool:
-        """Whether this mixer can work on a cache of 4 bits (one without keys and values has nothing there)."""
-        return self.kv_request() is None
+        """Whether this mixer can work on a cache of 4 bits (one without keys and values, own or another's, has nothing there)."""
+        return self.kv_request() is None and not getattr(self, "shared_kv", False)
 
     def forward(self, ctx, x: torch.Tensor, residual: torch.Tensor, cache: EntryCache) -> None:
         raise NotImplementedError
@@ -186,6 +186,11 @@ class Block(Part):
         for v in vars(self).values():
             parts += v if isinstance(v, (list, tuple)) else [v]
         return [p for i, p in enumerate(parts) if isinstance(p, Mixer) and not any(p is q for q in parts[:i])]
+
+    def takes_q4(self) -> bool:
+        """Whether all mixers of this block can work on a cache of 4 bits, every one that asks for a cache among them."""
+        found = self.mixers()
+        return len(found) >= len(self.cache_requests()) and all(m.takes_q4() for m in found)
 
     def cache_requests(self) -> List[tuple]:
         """One (KVRequest or None, StateRequest or None) pair per mixer of the block, in the order in which
