@@ -67,7 +67,8 @@ __device__ __forceinline__ float closing_factor(const AttnQ4& p, int t, int h, f
 //     would lose what is left of c - 8.  sum_j p_j d_jg and sum_j p_j m_jg are a tensor-core step as well.
 //   * Queries enter as float16 times a power of two per head that makes the greatest at most 1 (exact for all but what is
 //     2^-14 below it).  Weights are float16 with 11 bits: p is taken against a reference below the maximum so that p and p d
-//     lie in float16's middle, and the reference moves when a weight passes 2^15 or a step passes what it allows.
+//     lie in float16's middle, and the reference moves when a weight passes 2^15 or a step passes what it allows.  (What is less than
+//     2^-36 of the greatest weight counts for nothing, 2^-22 where a step of the values is thousands.)
 // Rounded below 32 bits are: a weight p, and p d, both to 11 bits.
 //
 // A block is two warps, each of which takes one half of every page: it brings its 32 keys' codes and scales (5 KB for D = 128) to its
@@ -81,9 +82,10 @@ __device__ __forceinline__ float closing_factor(const AttnQ4& p, int t, int h, f
 // pairs of not too many pages (CLUSTER), a cluster of blocks shares each of them instead, and its parts meet in distributed
 // shared memory: one launch, and no way through global memory.
 //
-// Bound by instructions where there is much to read (some 300 a warp for 16 keys, a little over half of the issue slots): 64 sequences of up to
-// 8 000 keys, 32 heads over 8 of 128 lanes, 70 us for 328 MB (4 700 GB/s); 64 of 4 000 each 73 us where bfloat16 takes 154.  One
-// sequence of 2 500 keys takes 9.7 us, launch and latency.
+// Bound where there is much to read by the fixed latency between a warp's instructions, some 300 for 16 keys, at three warps a scheduler: 55 % of
+// the issue slots, 27 % of the tensor pipe and 60 % of DRAM are used.  64 sequences of up to 8 000 keys, 32 heads over 8 of 128 lanes, 70 us
+// for 328 MB (4 700 GB/s); 64 of 4 000 each 73 us where bfloat16 takes 154.  One sequence of 2 500 keys takes 9.7 us, launch and
+// latency; 12.0 where the call is told of 32 768 keys (the row, see cluster_of).
 // ---------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kStreamWarps = 2;

@@ -82,7 +82,8 @@ __device__ __forceinline__ void norm_rotate(F (&x)[NG], const void* gamma, int g
 }
 
 // A warp per (token, head of q, k or v): any sizes, types and strides.  Bound by instructions, its lanes' exchanges among them (2 048
-// tokens of 32 heads over 8 of 128 lanes with what is read back took 57 us; append_fast_kernel takes what models commonly have).
+// tokens of 32 heads over 8: 39 us with heads of 96 lanes, 71 of 256, whose bytes are worth 8 and 22; append_fast_kernel takes what
+// models commonly have).
 template <int NG>
 __global__ void __launch_bounds__(256) append_kernel(const Append a) {
     constexpr int D = 32 * NG;
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(256) read_kernel(const uint8_t* k_pages, const
 // head's own and in rows behind the sequence's end (whatever the cache holds there).  Page i of sequence b goes to page b * width + i,
 // and the table for the attention kernels is written too.  A block takes a page of keys or of values of one head, a thread eight
 // neighbouring lanes of a row at a time: grid = (width, 2 n_kv, n_seqs).  (2 048 positions of 8 heads of 128 lanes to float16: 5.5 us
-// for 2.6 MB read and 8.4 written; the attention over them takes 48.  To take the codes out inside the attention kernel would do it
+// for 2.6 MB read and 8.4 written; the attention over them takes 51.  To take the codes out inside the attention kernel would do it
 // again for every tile of queries: 16 times here.)
 struct Expand {
     const uint8_t* k_pages;

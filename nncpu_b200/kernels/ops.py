@@ -118,7 +118,7 @@ def launch_overlap(on: bool) -> None:
     product after a kernel of little shared memory and the float32 products of few rows (they ask for their first weights
     before they wait for that one's results), the tensor-core products (their set-up; up to 64 bfloat16 tokens also their first
     weight tiles; above, and for float32 products of 96 tokens and more and the norms, the first weights go into L2 only), prefill attention (its set-up), float32 attention token by token, the norms, the small kernels of routers,
-    routed experts, gates and the stream between them, and a 4-bit cache's append, reads and merge.
+    routed experts, gates and the stream between them, and a 4-bit cache's append, reads, attention by clusters and merge.
     On by default; off, every kernel waits for the one before it to be over, and the results are the same bits.  Where a product
     asks for its first weights themselves, the kernel of this library right before it in the stream must not be the one that
     writes them."""
@@ -1800,7 +1800,9 @@ def attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_head
                  longest: int = 0, scratch=None) -> None:
     """Causal attention of each token over its sequence's pages of a cache of 4 bits, token by token (decode steps, and a few tokens a
     sequence); q and out [n, n_heads * head_dim] of one type.  The options are those of ``attention``.  ``longest``: at least as many
-    keys as any token sees (0: as the block tables have room for).  ``scratch``: float32, ``attention_q4_scratch_floats``
+    keys as any token sees (0: as the block tables have room for; the kernel's form follows from it: clusters share a few sequences of
+    few keys, one of 2 500 keys takes 9.8 us, or 12.0 if it is told of 32 768).  Score caps beyond ``MAX_FAST_CAP`` and heads of more than 128 lanes
+    are left to a 32-bit kernel without tensor cores, as float32 queries are.  ``scratch``: float32, ``attention_q4_scratch_floats``
     elements for the same ``longest`` and ``cap`` (None: taken from the allocator).  A token of sequence -1 gives zeros; a page that
     is not there (an id outside the pages) holds no keys."""
     n = _attention_q4_check("attention_q4", q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_heads, n_kv, head_dim, window,
@@ -1826,7 +1828,8 @@ def attention_q4(q, k_pages, v_pages, block_table, tok_seq, tok_pos, out, n_head
 # its tokens are at most so many and its keys more than two pages (32 heads over 8, us, straight / taken out first: 8 behind 3 000 22 / 30, 24
 # behind 700 17 / 21, 24 behind 3 000 24 / 31, 48 behind 1 500 24.5 / 25.7, 64 behind 3 000 35.9 / 32.9; 24 behind none 15.6 / 11.5).  Longer ones, and several sequences, have their keys and values taken out of the codes once, for
 # all query tiles and heads: float16 for the tcgen05 kernel, float32 for the 32-bit one; so many positions at a time (of whole sequences,
-# one at least).
+# one at least).  (A captured step is told of as many keys as its context has room for, whatever its sequence holds: a new sequence's 24
+# tokens then take the 15.6, and 256 behind 1 000 take 34.0 in a context of 32 768, 27.8 if it is told of the keys that are there.)
 Q4_FEW_TOKENS = 48
 Q4_EXPAND_POSITIONS = 16384
 Q4_EXPAND_POSITIONS_F32 = 65536
@@ -1871,7 +1874,14 @@ def attention_q4_prompt(q, k_pages, v_pages, block_table, cu_seqlens, tok_seq, t
     """``attention_q4`` for prompts and portions of them: any number of tokens a sequence, at consecutive positions (``cu_seqlens``
     int32 [n_seqs + 1]: each sequence's first token).  ``longest``: at least as many keys as any token sees.  ``status``: an int32 word on
     the device that receives a code if a bounded wait runs out, as in ``attention_prefill_tc``.  ``scratch``: uint8,
-    ``attention_q4_prompt_scratch_bytes`` elements (None: taken from the allocator).  What is left in the rows of no sequence is not said;
+    ``attention_q4_prompt_scratch_bytes`` elements (None: taken from the allocator).
+
+    bfloat16 heads of up to 128 lanes attend on the tensor cores to keys that are taken out of their codes first, all that the sequences
+    hold, whatever a window leaves of them to be seen: the scratch is 4 bytes a position, key/value head and lane (of 16 384 positions of
+    several sequences, or one whole sequence, at a time), and many short portions behind long sequences pay for all of it (16 of 8
+    tokens behind 2 000: 145 us).  Float32 does the same while all sequences together have 65 536 positions at most.  Up to ``Q4_FEW_TOKENS`` of
+    one sequence, and whatever else has no such path (more lanes, a score cap with a distance bias or beyond ``MAX_FAST_CAP``, more
+    positions), go token by token through ``attention_q4``'s kernels.  What is left in the rows of no sequence is not said;
     a page that is not there may count as zeros, and a NaN that the cache holds may reach tokens before it in the same step, as in the
     attention over a bfloat16 cache."""
     fn = "attention_q4_prompt"

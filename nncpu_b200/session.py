@@ -49,7 +49,8 @@ class SessionParams:
     attention takes that, ``score`` says what it costs);
     ``max_batch``: sequences generated together (in either precision a
     sequence's logits depend on the others by rounding alone: the kernels of
-    a step follow from its size); ``system_prompt`` opens the
+    a step follow from its size; over a cache of 4 bits a rounding may move a code, and a code moves a logit by a
+    percent or so); ``system_prompt`` opens the
     session's conversation (crates/nncpu/src/session/mod.rs:37-83);
     ``reply_open`` is text the chat template puts at the start of every reply
     (Qwen3 without reasoning: ``"<think>\\n\\n</think>\\n\\n"``,
